@@ -100,6 +100,22 @@ int scm_ln_bwd_noalloc(const float* dy, const float* x, const float* mean, const
                        const float* dres, int64_t T, int D, float* dx, void* dx_bf16, float* dgamma, float* dbeta,
                        float* dres_colsum, int accumulate, void* stream);
 
+/* ---- LayerNorm of rows of any width, in the types of a wide or half-precision model (the pair above is the residual
+ *      stream's: f32, D <= 256).  It has no counterpart in the reference, which leaves its other norms to torch.
+ *      x [T,D] with row stride ldx elements (0: one row for all), last dimension contiguous, any alignment; y and dx
+ *      contiguous.  Types: f32 -> f32 or bf16, bf16 -> bf16, fp16 -> fp16; gamma, beta (either may be NULL: 1, 0),
+ *      statistics and parameter gradients f32.  0 < D <= 16384, 0 < T < 2^31.
+ *      mean, rstd [T]: both, or both NULL where no backward follows. */
+enum { SCM_F32 = 0, SCM_BF16 = 1, SCM_F16 = 2 };
+int scm_norm_fwd(const void* x, int x_type, int64_t ldx, const float* gamma, const float* beta, int64_t T, int D,
+                 float eps, void* y, int y_type, float* mean, float* rstd, void* stream);
+/* dy [T,D] in y's type, row stride lddy.  dx (x's type) and dgamma, dbeta are written; each may be NULL.
+ * ws: scm_norm_bwd_ws_floats(T,D) floats, NULL exactly when neither dgamma nor dbeta is wanted. */
+int64_t scm_norm_bwd_ws_floats(int64_t T, int D);
+int scm_norm_bwd(const void* dy, int y_type, int64_t lddy, const void* x, int x_type, int64_t ldx, const float* mean,
+                 const float* rstd, const float* gamma, int64_t T, int D, void* dx, float* ws, float* dgamma,
+                 float* dbeta, void* stream);
+
 /* ---- nn.Linear products: performer_pytorch.py:374 (to_q/k/v), :402 (to_out), :323,330 (FeedForward) ---- */
 /* Y[M,N] = A[M,K] * W[N,K]^T with a fused epilogue; A is bf16 or (a_f32) f32, W bf16, K % 8 == 0, N % 8 == 0,
  * leading dimensions multiples of 8 elements and 16-byte aligned bases.

@@ -49,7 +49,7 @@ static const char* const kKernelNames[K_COUNT] = {
     "gemm_skinny/bf16", "gemm_skinny/f32_bias_res", "gemm_skinny/gelu_dual", "gemm_skinny/dgelu", "gemm_skinny/f32",
     "gemm_skinny/bf16_bias", "wgrad", "wgrad/bias", "wgrad_reduce", "cast_weight", "embed_fwd", "embed_bwd", "ln_fwd", "ln_bwd", "head_fwd",
     "head_bwd", "colsum_reduce", "prep_omega", "favor_ctx_fwd", "favor_ctx_bwd", "favor_ctx_finalize",
-    "favor_apply_fwd", "favor_apply_bwd_q", "favor_apply_bwd_k", "favor_kfix", "s1_mask", "cross_entropy", "bin_cells", "omega_qr", "feature_map", "linear_attention", "ffn_chain_fwd", "reduce_batch", "gemm_ln_bwd", "gemm_res_ln", "adam_step", "cell_tail", "distill_tail"};
+    "favor_apply_fwd", "favor_apply_bwd_q", "favor_apply_bwd_k", "favor_kfix", "s1_mask", "cross_entropy", "bin_cells", "omega_qr", "feature_map", "linear_attention", "ffn_chain_fwd", "reduce_batch", "gemm_ln_bwd", "gemm_res_ln", "adam_step", "cell_tail", "distill_tail", "layer_norm"};
 struct TraceRec { int kid; double flops, bytes; hipEvent_t t0, t1; };
 static int g_trace_kid = -1;  // -1 off, K_COUNT = every kernel, else one kernel id
 static std::vector<TraceRec> g_trace;
@@ -209,6 +209,45 @@ int scm_gemm_ln_bwd(const void* A, int64_t lda, const void* W, int64_t ldw, int6
     const ColsumSegs seg{{dgamma, dbeta, dres_colsum, nullptr}, {0, D, 2 * D, 0}, {D, 2 * D, 3 * D, 0}};
     SCM_HIP(colsum_reduce(ws, gemm_ln_bwd_blocks((long)M), 3 * D, seg, 3, accumulate, s), "scm_gemm_ln_bwd(column sums)");
   }
+  return 0;
+}
+
+// ---------------------------------------------------------------------------- LayerNorm of any width
+static bool types_in_range(int a) { return a == SCM_F32 || a == SCM_BF16 || a == SCM_F16; }
+static int norm_check(const char* who, const void* x, int x_type, int64_t ldx, int y_type, int64_t T, int D) {
+  SCM_REQ(x, "%s: null pointer", who);
+  SCM_REQ(types_in_range(x_type) && types_in_range(y_type) && norm_types_ok(x_type, y_type),
+          "%s: types must be f32 -> f32 or bf16, bf16 -> bf16, fp16 -> fp16 (got %d -> %d)", who, x_type, y_type);
+  SCM_REQ(T > 0 && T < ((int64_t)1 << 31) && D > 0 && D <= NORM_MAX_D, "%s: need 0 < T < 2^31, 0 < D <= %d (got T=%lld D=%d)",
+          who, NORM_MAX_D, (long long)T, D);
+  SCM_REQ(ldx >= 0, "%s: negative row stride", who);
+  return 0;
+}
+int scm_norm_fwd(const void* x, int x_type, int64_t ldx, const float* gamma, const float* beta, int64_t T, int D,
+                 float eps, void* y, int y_type, float* mean, float* rstd, void* stream) {
+  if (int e = norm_check("scm_norm_fwd", x, x_type, ldx, y_type, T, D)) return e;
+  SCM_REQ(y && (mean != nullptr) == (rstd != nullptr), "scm_norm_fwd: y, and both or neither of mean and rstd");
+  NormArgs a{};
+  a.x = x; a.ldx = ldx; a.x_type = x_type; a.y_type = y_type; a.gamma = gamma; a.beta = beta; a.T = T; a.D = D;
+  a.eps = eps; a.y = y; a.mean = mean; a.rstd = rstd;
+  SCM_HIP(norm_fwd(a, (hipStream_t)stream), "scm_norm_fwd");
+  return 0;
+}
+int64_t scm_norm_bwd_ws_floats(int64_t T, int D) {
+  return T > 0 && D > 0 && D <= NORM_MAX_D ? (int64_t)norm_bwd_blocks(T, D) * 2 * D : 0;
+}
+int scm_norm_bwd(const void* dy, int y_type, int64_t lddy, const void* x, int x_type, int64_t ldx, const float* mean,
+                 const float* rstd, const float* gamma, int64_t T, int D, void* dx, float* ws, float* dgamma,
+                 float* dbeta, void* stream) {
+  if (int e = norm_check("scm_norm_bwd", x, x_type, ldx, y_type, T, D)) return e;
+  SCM_REQ(dy && lddy >= 0 && mean && rstd, "scm_norm_bwd: null pointer or negative row stride");
+  SCM_REQ(dx || dgamma || dbeta, "scm_norm_bwd: no gradient asked for");
+  SCM_REQ((ws != nullptr) == (dgamma || dbeta), "scm_norm_bwd: ws goes with dgamma / dbeta");
+  NormArgs a{};
+  a.x = x; a.ldx = ldx; a.x_type = x_type; a.y_type = y_type; a.gamma = gamma; a.T = T; a.D = D;
+  a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+  a.dy = dy; a.lddy = lddy; a.dx = dx; a.ws = ws;
+  SCM_HIP(norm_bwd(a, dgamma, dbeta, (hipStream_t)stream), "scm_norm_bwd");
   return 0;
 }
 

@@ -88,7 +88,7 @@ enum KernelId {   // one id per kernel symbol family that a profiler lists separ
   K_WGRAD = 12, K_WGRAD_BIAS, K_WGRAD_REDUCE, K_CAST, K_EMBED_FWD, K_EMBED_BWD, K_LN_FWD, K_LN_BWD, K_HEAD_FWD,
   K_HEAD_BWD, K_COLSUM, K_PREP_OMEGA, K_CTX_FWD, K_CTX_BWD, K_CTX_FINALIZE, K_APPLY_FWD, K_APPLY_BWD_Q,
   K_APPLY_BWD_K, K_KFIX, K_S1_MASK, K_CE, K_BIN, K_OMEGA_QR, K_FEATURE_MAP, K_LINEAR_ATTENTION, K_FFN_CHAIN_FWD,
-  K_REDUCE_BATCH, K_GEMM_LN_BWD, K_GEMM_RES_LN, K_ADAM, K_CELL_TAIL, K_DISTILL_TAIL, K_COUNT
+  K_REDUCE_BATCH, K_GEMM_LN_BWD, K_GEMM_RES_LN, K_ADAM, K_CELL_TAIL, K_DISTILL_TAIL, K_NORM, K_COUNT
 };
 void trace_begin(int kid, double flops, double bytes, hipStream_t s);
 void trace_end(int kid, hipStream_t s);
@@ -170,6 +170,21 @@ hipError_t colsum_reduce(const float* partial, int nblocks, int width, int lo, i
 using ReduceJob = ::scm_reduce_job;
 constexpr int RB_MAX = 40;                      // jobs per launch (they travel as kernel arguments)
 hipError_t reduce_batch(const ReduceJob* jobs, int n, hipStream_t s);
+
+// layer_norm.hip: LayerNorm of any width <= NORM_MAX_D
+constexpr int NORM_MAX_D = 16384;
+struct NormArgs {
+  const void* x; long ldx; int x_type, y_type;     // SCM_F32 / SCM_BF16 / SCM_F16
+  const float* gamma; const float* beta;
+  long T; int D; float eps;
+  void* y;                                         // forward: [T][D], and (both or neither) mean, rstd
+  float* mean; float* rstd;
+  const void* dy; long lddy; void* dx; float* ws;  // backward
+};
+bool norm_types_ok(int x_type, int y_type);
+int norm_bwd_blocks(long T, int D);
+hipError_t norm_fwd(const NormArgs& a, hipStream_t s);
+hipError_t norm_bwd(const NormArgs& a, float* dgamma, float* dbeta, hipStream_t s);
 
 // optim.hip
 using AdamItem = ::scm_adam_item;

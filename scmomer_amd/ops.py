@@ -5,6 +5,7 @@ Every function requires CUDA(HIP) tensors; nothing here computes on the host.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from dataclasses import dataclass
 from typing import Optional, Tuple
@@ -147,6 +148,86 @@ def ln_bwd(dy, x, mean, rstd, gamma, dres, dgamma, dbeta, dres_colsum, accumulat
         defer.append(colsum_job(ws, ws.numel() // (3 * d), 3 * d,
                                 [(dgamma, 0, d), (dbeta, d, 2 * d), (dres_colsum, 2 * d, 3 * d)], accumulate))
     return (dx, dxb) if with_bf16 else dx
+
+
+# ----------------------------------------------------------------------------- rows of any width and type
+SCM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+NORM_MAX_D = 16384
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(*tensors):
+    """context in which the launches go to the tensors' device (and its current stream); they must share one"""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("expected device tensors; scmomer_amd has no CPU path")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def rows_of(t: torch.Tensor, name: str) -> torch.Tensor:
+    """[T, D] form of a tensor [..., D] of one of SCM_TYPES: a view where one row stride describes it (an expanded
+    batch keeps stride 0), a contiguous copy otherwise"""
+    if t.dtype not in SCM_TYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name}: expected [..., D] with D >= 1, got {tuple(t.shape)}")
+    d = t.shape[-1]
+    r = t if t.dim() == 2 else t.reshape(t.numel() // d, d)
+    return r if d == 1 or r.stride(1) == 1 else r.contiguous()
+
+
+def norm_fwd(x: torch.Tensor, gamma, beta, eps: float, out_dtype=None, stats: bool = True):
+    """LayerNorm over the last dimension (rows_of(x) is what it reads).  -> (y [T, D], mean [T], rstd [T]), the
+    statistics None when stats is false"""
+    x = rows_of(x, "x")
+    t, d = x.shape
+    out_dtype = out_dtype or x.dtype
+    if d > NORM_MAX_D:
+        raise ValueError(f"layer norm: at most {NORM_MAX_D} columns (got {d})")
+    if out_dtype != x.dtype and (x.dtype, out_dtype) != (F32, BF16):
+        raise TypeError(f"layer norm: {x.dtype} in gives {x.dtype} out, or bfloat16 from float32 (asked for {out_dtype})")
+    for p, nm in ((gamma, "weight"), (beta, "bias")):
+        if p is not None:
+            _req(p, F32, nm)
+            if tuple(p.shape) != (d,):
+                raise ValueError(f"{nm}: expected [{d}], got {tuple(p.shape)}")
+    with _on_device(x, gamma, beta):
+        y = torch.empty((t, d), dtype=out_dtype, device=x.device)
+        mean = torch.empty(t, dtype=F32, device=x.device) if stats else None
+        rstd = torch.empty(t, dtype=F32, device=x.device) if stats else None
+        if t:
+            check(lib.scm_norm_fwd(_p(x), SCM_TYPES[x.dtype], x.stride(0), _p(gamma), _p(beta), t, d, float(eps), _p(y),
+                                   SCM_TYPES[out_dtype], _p(mean), _p(rstd), _stream()), "scm_norm_fwd")
+    return y, mean, rstd
+
+
+def norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean, rstd, gamma, want_dx: bool = True, want_dgamma: bool = True,
+             want_dbeta: bool = True):
+    """-> (dx [T, D] in x's type, dgamma f32 [D], dbeta f32 [D]), None for what is not wanted.  dy has the type of
+    norm_fwd's y."""
+    dy, x = rows_of(dy, "dy"), rows_of(x, "x")
+    t, d = x.shape
+    if dy.shape != x.shape:
+        raise ValueError(f"layer norm: dy {tuple(dy.shape)} for x {tuple(x.shape)}")
+    with _on_device(dy, x, mean, rstd, gamma):
+        dx = torch.empty((t, d), dtype=x.dtype, device=x.device) if want_dx else None
+        new = torch.empty if t else torch.zeros      # no rows: the sums are empty
+        dgamma = new(d, dtype=F32, device=x.device) if want_dgamma else None
+        dbeta = new(d, dtype=F32, device=x.device) if want_dbeta else None
+        if t and (want_dx or want_dgamma or want_dbeta):
+            ws = torch.empty(lib.scm_norm_bwd_ws_floats(t, d), dtype=F32, device=x.device) \
+                if want_dgamma or want_dbeta else None
+            check(lib.scm_norm_bwd(_p(dy), SCM_TYPES[dy.dtype], dy.stride(0), _p(x), SCM_TYPES[x.dtype], x.stride(0),
+                                   _p(mean), _p(rstd), _p(gamma), t, d, _p(dx), _p(ws), _p(dgamma), _p(dbeta),
+                                   _stream()), "scm_norm_bwd")
+    return dx, dgamma, dbeta
 
 
 def gemm_res_ln_supported(a: torch.Tensor, w: torch.Tensor) -> bool:
