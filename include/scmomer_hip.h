@@ -281,6 +281,28 @@ int64_t scm_linear_attention_ws_floats(int64_t BH, int N, int M);
 int scm_linear_attention(const float* qf, const float* kf, const float* v, int64_t BH, int N, int M, float* out,
                          float* ws, void* stream);
 
+/* ---- log probabilities read off rows of logits, for any vocabulary (scm_ce_fwd below is the loss of the RNA model's
+ *      own <= 8 classes).  No counterpart in the reference.  x [T,V] with row stride ldx elements (0: one row for
+ *      all), last dimension contiguous, any alignment, type SCM_F32 / SCM_BF16 / SCM_F16; z = x / temperature;
+ *      V <= 2^30.
+ *      Per row: lse = log sum exp z (may be NULL); logprob = z[target] - lse (target and logprob: both or neither),
+ *      0 where target == ignore_index, NaN for any other target outside [0,V); entropy = -sum p ln p (may be NULL);
+ *      the k <= min(64, V) tokens of the largest x in descending order, equal values by ascending index, NaN first,
+ *      with their log probabilities (top_index, top_logprob [T,k]).
+ *      A row of -inf only: lse, logprob, top_logprob -inf, entropy 0, the first k indices.  A row with NaN or +inf: NaN.
+ *      tape [T,2] (may be NULL): what scm_score_bwd reads.  ws: scm_score_ws_floats(T,V,k) floats, 8-byte aligned. */
+int64_t scm_score_ws_floats(int64_t T, int V, int k);
+int scm_score_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* target,
+                  int64_t ignore_index, int k, float* logprob, float* lse, float* entropy, float* top_logprob,
+                  int64_t* top_index, float* tape, float* ws, void* stream);
+/* dx [T,V] (x's type, contiguous) = the gradient of sum g_logprob logprob + g_lse lse + g_entropy entropy + g_top
+ * top_logprob (g_*: f32, [T] or [T,k], each may be NULL); entropy, top_index as the forward wrote them (the indices of
+ * a row distinct).  Rows of -inf only get 0. */
+int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* target,
+                  int64_t ignore_index, int k, const float* tape, const float* entropy, const int64_t* top_index,
+                  const float* g_logprob, const float* g_lse, const float* g_entropy, const float* g_top, void* dx,
+                  void* stream);
+
 /* ---- final LayerNorm + head: performer_pytorch.py:628-634 (Linear(dim,num_tokens)); rna_encoder.py:5-16
  *      (1x200 conv == dot product, + ReLU; C = 1, relu = 1) -------------------------------------- */
 /* enc (may be NULL) f32 [T,D] = LN(x); out (may be NULL when C == 0) f32 [T,C]. */

@@ -85,6 +85,9 @@ SIGNATURES = {
     "scm_ln_fwd": (i32, [vp, vp, vp, i64, i32, vp, vp, vp, vp]),
     "scm_ln_bwd_ws_floats": (i64, [i64, i32]),
     "scm_ln_bwd": (i32, [vp, vp, vp, vp, vp, vp, i64, i32, vp, vp, vp, vp, vp, vp, i32, vp]),
+    "scm_score_ws_floats": (i64, [i64, i32, i32]),
+    "scm_score_fwd": (i32, [vp, i32, i64, i64, i32, C.c_float, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "scm_score_bwd": (i32, [vp, i32, i64, i64, i32, C.c_float, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "scm_norm_fwd": (i32, [vp, i32, i64, vp, vp, i64, i32, C.c_float, vp, i32, vp, vp, vp]),
     "scm_norm_bwd_ws_floats": (i64, [i64, i32]),
     "scm_norm_bwd": (i32, [vp, i32, i64, vp, i32, i64, vp, vp, vp, i64, i32, vp, vp, vp, vp, vp]),

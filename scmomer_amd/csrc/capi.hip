@@ -49,7 +49,7 @@ static const char* const kKernelNames[K_COUNT] = {
     "gemm_skinny/bf16", "gemm_skinny/f32_bias_res", "gemm_skinny/gelu_dual", "gemm_skinny/dgelu", "gemm_skinny/f32",
     "gemm_skinny/bf16_bias", "wgrad", "wgrad/bias", "wgrad_reduce", "cast_weight", "embed_fwd", "embed_bwd", "ln_fwd", "ln_bwd", "head_fwd",
     "head_bwd", "colsum_reduce", "prep_omega", "favor_ctx_fwd", "favor_ctx_bwd", "favor_ctx_finalize",
-    "favor_apply_fwd", "favor_apply_bwd_q", "favor_apply_bwd_k", "favor_kfix", "s1_mask", "cross_entropy", "bin_cells", "omega_qr", "feature_map", "linear_attention", "ffn_chain_fwd", "reduce_batch", "gemm_ln_bwd", "gemm_res_ln", "adam_step", "cell_tail", "distill_tail", "layer_norm"};
+    "favor_apply_fwd", "favor_apply_bwd_q", "favor_apply_bwd_k", "favor_kfix", "s1_mask", "cross_entropy", "bin_cells", "omega_qr", "feature_map", "linear_attention", "ffn_chain_fwd", "reduce_batch", "gemm_ln_bwd", "gemm_res_ln", "adam_step", "cell_tail", "distill_tail", "layer_norm", "token_logprobs", "topk_distill"};
 struct TraceRec { int kid; double flops, bytes; hipEvent_t t0, t1; };
 static int g_trace_kid = -1;  // -1 off, K_COUNT = every kernel, else one kernel id
 static std::vector<TraceRec> g_trace;
@@ -248,6 +248,58 @@ int scm_norm_bwd(const void* dy, int y_type, int64_t lddy, const void* x, int x_
   a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.dy = dy; a.lddy = lddy; a.dx = dx; a.ws = ws;
   SCM_HIP(norm_bwd(a, dgamma, dbeta, (hipStream_t)stream), "scm_norm_bwd");
+  return 0;
+}
+
+// ---------------------------------------------------------------------------- rows of logits
+static int logits_check(const char* who, const void* x, int type, int64_t ldx, int64_t T, int V, int k, float temperature) {
+  SCM_REQ(x, "%s: null pointer", who);
+  SCM_REQ(types_in_range(type), "%s: type must be f32, bf16 or fp16 (got %d)", who, type);
+  SCM_REQ(T > 0 && T < ((int64_t)1 << 31) && V > 0 && V <= (1 << 30) && ldx >= 0,
+          "%s: need 0 < T < 2^31, 0 < V <= 2^30, ldx >= 0", who);
+  SCM_REQ(k >= 0 && k <= LOGITS_MAX_K, "%s: at most %d entries a row (got %d)", who, LOGITS_MAX_K, k);
+  SCM_REQ(temperature > 0.f && temperature < INFINITY, "%s: temperature must be positive and finite", who);
+  return 0;
+}
+static float log2e_over(float temperature) { return (float)(1.4426950408889634 / (double)temperature); }
+
+int64_t scm_score_ws_floats(int64_t T, int V, int k) {
+  if (T <= 0 || V <= 0 || k < 0 || k > LOGITS_MAX_K) return 0;
+  const int64_t S = score_segments(T, V, k);
+  return S > 1 ? T * S * (2 * (int64_t)k + 3) : 0;
+}
+int scm_score_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* target,
+                  int64_t ignore_index, int k, float* logprob, float* lse, float* entropy, float* top_logprob,
+                  int64_t* top_index, float* tape, float* ws, void* stream) {
+  if (int e = logits_check("scm_score_fwd", x, type, ldx, T, V, k, temperature)) return e;
+  SCM_REQ(k <= V, "scm_score_fwd: %d alternatives of %d tokens", k, V);
+  SCM_REQ((target != nullptr) == (logprob != nullptr), "scm_score_fwd: target goes with logprob");
+  SCM_REQ(k == 0 || (top_logprob && top_index), "scm_score_fwd: null pointer for the alternatives");
+  SCM_REQ(ws || scm_score_ws_floats(T, V, k) == 0, "scm_score_fwd: null workspace");
+  SCM_REQ(((uintptr_t)ws & 7) == 0, "scm_score_fwd: workspace must be 8-byte aligned");
+  ScoreArgs a{};
+  a.x = x; a.ldx = ldx; a.type = type; a.T = T; a.V = V; a.k = k; a.c = log2e_over(temperature); a.inv_t = 1.f / temperature;
+  a.target = target; a.ignore = ignore_index; a.logprob = logprob; a.lse = lse; a.entropy = entropy;
+  a.top_logprob = top_logprob; a.top_index = top_index; a.tape = tape;
+  a.part_top = (unsigned long*)ws;
+  a.part = ws ? ws + 2 * (int64_t)k * T * score_segments(T, V, k) : nullptr;
+  SCM_HIP(score_fwd(a, (hipStream_t)stream), "scm_score_fwd");
+  return 0;
+}
+int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* target,
+                  int64_t ignore_index, int k, const float* tape, const float* entropy, const int64_t* top_index,
+                  const float* g_logprob, const float* g_lse, const float* g_entropy, const float* g_top, void* dx,
+                  void* stream) {
+  if (int e = logits_check("scm_score_bwd", x, type, ldx, T, V, k, temperature)) return e;
+  SCM_REQ(tape && dx, "scm_score_bwd: null pointer");
+  SCM_REQ(!g_logprob || target, "scm_score_bwd: g_logprob needs target");
+  SCM_REQ(!g_entropy || entropy, "scm_score_bwd: g_entropy needs the entropy");
+  SCM_REQ(!g_top || (k > 0 && top_index), "scm_score_bwd: g_top needs the alternatives");
+  ScoreGradArgs a{};
+  a.x = x; a.ldx = ldx; a.type = type; a.T = T; a.V = V; a.k = k; a.c = log2e_over(temperature); a.inv_t = 1.f / temperature;
+  a.target = target; a.ignore = ignore_index; a.tape = tape; a.entropy = entropy; a.top_index = top_index;
+  a.g_logprob = g_logprob; a.g_lse = g_lse; a.g_entropy = g_entropy; a.g_top = g_top; a.dx = dx;
+  SCM_HIP(score_bwd(a, (hipStream_t)stream), "scm_score_bwd");
   return 0;
 }
 

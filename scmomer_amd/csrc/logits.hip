@@ -1,0 +1,489 @@
+// What is read off a row of logits x[0..V), z = x / temperature, f32 / bf16 / fp16, any V: lse = log sum exp z, the log
+// probability of a given token, the entropy, the k <= 64 most likely tokens; and the gradient of all of them.
+//
+// The logits are read once, in 16-byte chunks; every thread keeps a running maximum m and s = sum 2^((x - m) c),
+// c = log2(e) / temperature, in f32; threads, waves and workgroups join by rescaling to the larger maximum.  x - m is
+// formed first: a row of the type's lowest value is an ordinary (uniform) row, and -inf weighs nothing.
+//   V <= 64    one thread per row, 64 rows staged through LDS per wave
+//   V <= 2048  one wave per row
+//   else       256 threads per row, and where rows are too few to fill the card a row is split into segments of one
+//              workgroup each, whose partial results a second launch joins in segment order
+// What bounds them is HBM, and for 2-byte types the vector ALU nearly as much (an exponential costs four issue slots).
+#include "scm_softmax.hpp"
+
+namespace scm {
+
+// ---------------------------------------------------------------- order of the alternatives
+// Larger key = earlier: by value, equal values (-0 and +0 among them) by lower index, NaN before everything.
+// 0 is no key of any element.
+SCM_DEV uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);   // -0 + 0 = +0
+  const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return x != x ? 0xFFFFFFFEu : o;
+}
+SCM_DEV float unordered(uint32_t o) {
+  if (o == 0xFFFFFFFEu) return __uint_as_float(0x7FC00000u);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
+SCM_DEV uint64_t key_of(uint32_t o, int idx) { return ((uint64_t)o << 32) | (uint32_t)~idx; }
+SCM_DEV int key_index(uint64_t k) { return (int)~(uint32_t)k; }
+SCM_DEV float key_value(uint64_t k) { return unordered((uint32_t)(k >> 32)); }
+SCM_DEV uint64_t shfl64(uint64_t v, int mask) {
+  return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), mask) << 32) | (uint32_t)__shfl_xor((int)v, mask);
+}
+
+// ---------------------------------------------------------------- score: the k largest elements of a segment
+// A lower bound of the k-th largest element comes free with the statistics: the k-th largest of the threads' maxima
+// (each thread's maximum is an element of its own).  Only threads whose maximum reaches it look at their elements
+// again; what reaches it (about k of them) goes to LDS and is ranked there by counting.
+template <int NT>
+struct TopLds {
+  static constexpr int CAP = NT == 64 ? 512 : 1024;
+  uint64_t cand[CAP];
+  uint32_t best[NT];
+  int at[NT];
+  int count;
+  uint32_t thr;
+  int thr_at;
+  uint64_t red[NT / 64];
+};
+
+// Threshold (value, chunk) over the NT maxima, by the first wave: the k-th largest value, and among equal values the
+// chunk up to which the k-th place reaches.  Threads without elements hold value 0.
+template <int NT>
+SCM_DEV void top_threshold(TopLds<NT>& L, int k) {
+  constexpr int R = NT / 64;
+  const int l = threadIdx.x & 63;
+  uint32_t b[R];
+  int at[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) { b[r] = L.best[r * 64 + l]; at[r] = L.at[r * 64 + l]; }
+  uint32_t t = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cand = t | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] >= cand));
+    if (n >= k) t = cand;
+  }
+  // t == 0: fewer than k threads have elements; everything is a candidate
+  int need = k;
+#pragma unroll
+  for (int r = 0; r < R; ++r) need -= __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] > t));
+  int lim = 0;   // smallest bound with at least `need` equal maxima at chunks <= lim; all bits set: no bound
+  for (int bit = 30; bit >= 0; --bit) {
+    const int cand = lim | (1 << bit);
+    int n = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] == t && at[r] < cand));
+    if (n < need) lim = cand;
+  }
+  if (l == 0) { L.thr = t; L.thr_at = t ? lim : 0x7FFFFFFF; }
+}
+
+// Calls emit(rank, key) for the k largest keys of the segment, each from one thread.  best, at: the thread's maximum
+// (0: no elements) and the first of its chunks that holds it.  odd: the segment holds NaN or +inf (or may: then the
+// threads' maxima are not to be used).
+template <typename T, int NT, typename Emit>
+SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, int at, bool odd, TopLds<NT>& L, Emit emit) {
+  constexpr int E = Walk<T, NT>::E, U = Walk<T, NT>::U;
+  const int tid = threadIdx.x;
+  L.best[tid] = best;
+  L.at[tid] = at;
+  if (tid == 0) L.count = 0;
+  __syncthreads();
+  if (tid < 64) top_threshold<NT>(L, k);
+  __syncthreads();
+  const uint32_t thr = L.thr;
+  const int thr_at = L.thr_at;
+  if (!odd && best && (best > thr || (best == thr && at <= thr_at))) {
+    for (int s = 0; s < w.steps(); ++s) {
+      Chunk<T, E> raw[U];
+      w.load(s, raw);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c0 = w.first(s, u), chunk = c0 / E;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const uint32_t o = ordered((float)raw[u].e[j]);
+          if (c0 + j < w.len && (o > thr || (o == thr && chunk <= thr_at))) {
+            const int pos = atomicAdd(&L.count, 1);
+            if (pos < TopLds<NT>::CAP) L.cand[pos] = key_of(o, lo + c0 + j);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = L.count;
+  if (!odd && n <= TopLds<NT>::CAP) {
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t mine = L.cand[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += L.cand[j] > mine;
+      if (rank < k) emit(rank, mine);
+    }
+    return;
+  }
+  // more candidates than places (all large values in few threads' chunks), or NaN: k passes, each finding the largest
+  // key below the last one
+  uint64_t last = ~0ull;
+  const int found = k < w.len ? k : w.len;
+  for (int r = 0; r < found; ++r) {
+    uint64_t mine = 0;
+    for (int s = 0; s < w.steps(); ++s) {
+      Chunk<T, E> raw[U];
+      w.load(s, raw);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int i = w.first(s, u) + j;
+          const uint64_t key = key_of(ordered((float)raw[u].e[j]), lo + i);
+          if (i < w.len && key < last && key > mine) mine = key;
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const uint64_t x = shfl64(mine, o); mine = x > mine ? x : mine; }
+    if ((tid & 63) == 0) L.red[tid >> 6] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < NT / 64; ++v) mine = L.red[v] > mine ? L.red[v] : mine;
+    __syncthreads();
+    last = mine;
+    if (tid == 0) emit(r, mine);
+  }
+}
+
+// ---------------------------------------------------------------- score: what a row's statistics give
+struct RowScore {
+  float m, s, l2, inv_t;   // l2 = log2 s
+  SCM_DEV RowScore(const Stat& st, float inv_t_) : m(st.m), s(st.s), l2(log2_fast(st.s)), inv_t(inv_t_) {}
+  SCM_DEV float lse() const { return s == 0.f ? -INFINITY : m * inv_t + LN2 * l2; }
+  SCM_DEV float logp(float x) const { return s == 0.f ? -INFINITY : (x - m) * inv_t - LN2 * l2; }
+  SCM_DEV float entropy(float h) const { return s == 0.f ? 0.f : LN2 * (l2 - h / s); }
+};
+
+template <bool ENT>
+SCM_DEV void write_row(const ScoreArgs& a, long row, const Stat& st, float x_target, long long target) {
+  const RowScore r(st, a.inv_t);
+  if (a.target) {
+    float lp = __uint_as_float(0x7FC00000u);   // an index outside the vocabulary has no probability
+    if (target == a.ignore) lp = 0.f;
+    else if (target >= 0 && target < a.V) lp = r.logp(x_target);
+    a.logprob[row] = lp;
+  }
+  if (a.lse) a.lse[row] = r.lse();
+  if constexpr (ENT) a.entropy[row] = r.entropy(st.h);
+  if (a.tape) { a.tape[2 * row] = st.m; a.tape[2 * row + 1] = st.s; }
+}
+
+template <typename T, int NT, bool ENT, bool TOP>
+__global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_len) {
+  __shared__ Stat red[NT / 64];
+  __shared__ TopLds<TOP ? NT : 64> top;
+  typedef Walk<T, NT> W;
+  const long row = blockIdx.x / S;
+  const int seg = blockIdx.x % S, lo = seg * seg_len;
+  const W w{(const T*)a.x + row * a.ldx + lo, min(a.V - lo, seg_len)};
+  Stat st = stat_none();
+  float best = -INFINITY;
+  int at = threadIdx.x;
+  for (int s = 0; s < w.steps(); ++s) {
+    Chunk<T, W::E> raw[W::U];
+    w.load(s, raw);
+    float v[32], bm = LOWEST;
+#pragma unroll
+    for (int u = 0; u < W::U; ++u) {
+      const int n = w.len - w.first(s, u);
+      float cm = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < W::E; ++j) {
+        const float x = j < n ? (float)raw[u].e[j] : -INFINITY;
+        v[u * W::E + j] = x;
+        cm = fmaxf(cm, x);
+      }
+      bm = fmaxf(bm, cm);
+      if (TOP && cm > best) { best = cm; at = w.first(s, u) / W::E; }
+    }
+    stat_add<ENT>(st, v, bm, a.c);
+  }
+  st = stat_block<ENT, NT>(st, a.c, red);
+  const bool odd = !(st.s <= 3e38f);   // NaN
+  if (S > 1) {
+    const long slot = row * S + seg;
+    if (threadIdx.x == 0) { a.part[3 * slot] = st.m; a.part[3 * slot + 1] = st.s; a.part[3 * slot + 2] = st.h; }
+    if constexpr (TOP) {
+      uint64_t* out = a.part_top + slot * a.k;
+      for (int i = w.len + threadIdx.x; i < a.k; i += NT) out[i] = 0;   // a segment shorter than k
+      top_of_segment<T, NT>(w, lo, a.k, (int)threadIdx.x * W::E < w.len ? ordered(best) : 0u, at, odd, top,
+                            [&](int rank, uint64_t key) { out[rank] = key; });
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    const long long t = a.target ? a.target[row] : 0;
+    const float xt = a.target && t >= 0 && t < a.V ? (float)w.p[t] : 0.f;
+    write_row<ENT>(a, row, st, xt, t);
+  }
+  if constexpr (TOP) {
+    const RowScore r(st, a.inv_t);
+    top_of_segment<T, NT>(w, 0, a.k, (int)threadIdx.x * W::E < w.len ? ordered(best) : 0u, at, odd, top,
+                          [&](int rank, uint64_t key) {
+                            a.top_index[row * a.k + rank] = key_index(key);
+                            a.top_logprob[row * a.k + rank] = r.logp(key_value(key));
+                          });
+  }
+}
+
+// Joins the S segments of a row.  Their sorted lists: with p = ceil(k / S) and q = ceil(k / p), at least p q >= k
+// keys reach the q-th largest of the lists' p-th keys; those are collected and ranked by counting.
+template <typename T, bool ENT>
+__global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a, int S) {
+  __shared__ uint64_t cand[LOGITS_JOIN_KEYS];
+  __shared__ uint64_t head[LOGITS_MAX_SEGMENTS], thr;
+  __shared__ int count;
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x, l = tid & 63;
+  Stat st = stat_none();   // every wave joins them all: no exchange between waves
+  for (int i = l; i < S; i += 64) {
+    const float* p = a.part + 3 * (row * S + i);
+    st = stat_join<ENT>(st, Stat{p[0], p[1], p[2]}, a.c);
+  }
+  st = stat_wave<ENT>(st, a.c);
+  if (tid == 0) {
+    const long long t = a.target ? a.target[row] : 0;
+    const float xt = a.target && t >= 0 && t < a.V ? (float)((const T*)a.x)[row * a.ldx + t] : 0.f;
+    write_row<ENT>(a, row, st, xt, t);
+  }
+  if (!a.k) return;
+  const uint64_t* keys = a.part_top + row * S * a.k;
+  const int p = (a.k + S - 1) / S, q = (a.k + p - 1) / p;
+  for (int i = tid; i < S; i += 256) head[i] = keys[(long)i * a.k + p - 1];
+  if (tid == 0) { count = 0; thr = 1; }
+  __syncthreads();
+  for (int i = tid; i < S; i += 256) {
+    int rank = 0;
+    for (int j = 0; j < S; ++j) rank += head[j] > head[i];
+    if (rank == q - 1 && head[i]) thr = head[i];   // keys are distinct; an empty place (0) bounds nothing
+  }
+  __syncthreads();
+  const uint64_t t = thr;
+  for (int i = tid; i < S * a.k; i += 256) {
+    const uint64_t key = keys[i];
+    if (key >= t) cand[atomicAdd(&count, 1)] = key;   // at most S k <= LOGITS_JOIN_KEYS
+  }
+  __syncthreads();
+  const RowScore r(st, a.inv_t);
+  for (int i = tid; i < count; i += 256) {
+    const uint64_t mine = cand[i];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += cand[j] > mine;
+    if (rank < a.k) {
+      a.top_index[row * a.k + rank] = key_index(mine);
+      a.top_logprob[row * a.k + rank] = r.logp(key_value(mine));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- rows of at most 64 logits, one thread each
+template <typename T, bool ENT>
+__global__ __launch_bounds__(64) void score_small_kernel(ScoreArgs a) {
+  __shared__ uint32_t lds[64 * 65];
+  const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
+  const long row = (long)blockIdx.x * 64 + threadIdx.x;
+  stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
+  __syncthreads();
+  if ((int)threadIdx.x >= rows) return;
+  uint32_t* o = lds + threadIdx.x * pitch;
+  auto x = [&](int i) { return __uint_as_float(o[i]); };
+  Stat st = stat_none();
+  for (int i = 0; i < V; ++i) st.m = fmaxf(st.m, x(i));
+  for (int i = 0; i < V; ++i) {
+    const float d = (x(i) - st.m) * a.c, e = exp2_fast(d);
+    st.s += e;
+    if constexpr (ENT) st.h += e * fmaxf(d, -200.f);
+  }
+  const long long t = a.target ? a.target[row] : 0;
+  write_row<ENT>(a, row, st, a.target && t >= 0 && t < V ? x((int)t) : 0.f, t);
+  if (!a.k) return;
+  const RowScore r(st, a.inv_t);
+  for (int i = 0; i < V; ++i) o[i] = ordered(x(i));
+  for (int j = 0; j < a.k; ++j) {   // k <= V selections, each taken out
+    uint32_t b = 0;
+    int bi = 0;
+    for (int i = 0; i < V; ++i)
+      if (o[i] > b) { b = o[i]; bi = i; }
+    o[bi] = 0;
+    a.top_index[row * a.k + j] = bi;
+    a.top_logprob[row * a.k + j] = r.logp(unordered(b));
+  }
+}
+
+// ---------------------------------------------------------------- score: gradient
+// dz_i = sum_{named s} g_s [i == s] - p_i (sum g_s - g_lse) - g_H p_i (ln p_i + H)  =  .. + e_i (ca + cb d_i),
+// e_i = 2^d_i, d_i = (x_i - m) c, with the two coefficients of the row:
+struct ScoreGrad { float m, ca, cb, g_target; long long target; bool has_target; };
+SCM_DEV ScoreGrad score_grad(const ScoreGradArgs& a, long row, float g_top_sum) {
+  ScoreGrad r{};
+  r.m = a.tape[2 * row];
+  const float s = a.tape[2 * row + 1];
+  r.target = a.target ? a.target[row] : a.ignore;
+  const bool used = r.target != a.ignore && a.g_logprob;
+  r.has_target = used && r.target >= 0 && r.target < a.V;
+  r.g_target = r.has_target ? a.g_logprob[row] : 0.f;
+  float g = r.g_target + g_top_sum - (a.g_lse ? a.g_lse[row] : 0.f);
+  if (used && !r.has_target) g = __uint_as_float(0x7FC00000u);
+  const float gh = a.g_entropy ? a.g_entropy[row] : 0.f;
+  if (s != 0.f) {   // a row without anything above -inf has no gradient
+    const float f = a.inv_t / s;
+    r.ca = -(g + gh * (a.g_entropy ? a.entropy[row] - LN2 * log2_fast(s) : 0.f)) * f;
+    r.cb = -gh * LN2 * f;
+  } else {
+    r.has_target = false;
+  }
+  return r;
+}
+SCM_DEV float score_dx(const ScoreGrad& r, float x, float c) {
+  const float d = (x - r.m) * c;
+  return exp2_fast(d) * (r.ca + r.cb * fmaxf(d, -200.f));
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, int seg_len) {
+  __shared__ int target_named;
+  typedef Walk<T, NT> W;
+  const long row = blockIdx.x / S;
+  const int lo = (int)(blockIdx.x % S) * seg_len, tid = threadIdx.x;
+  const T* x = (const T*)a.x + row * a.ldx;
+  T* dx = (T*)a.dx + row * a.V;
+  const W w{x + lo, min(a.V - lo, seg_len)};
+  const int k = a.g_top ? a.k : 0;
+  // every wave adds the k <= 64 gradients of the alternatives up by itself
+  const float gt = wave_sum((tid & 63) < k ? a.g_top[row * k + (tid & 63)] : 0.f);
+  const ScoreGrad r = score_grad(a, row, gt);
+  if (tid == 0) target_named = 0;
+  for (int s = 0; s < w.steps(); ++s) {
+    Chunk<T, W::E> raw[W::U];
+    w.load(s, raw);
+#pragma unroll
+    for (int u = 0; u < W::U; ++u) {
+      float o[W::E];
+#pragma unroll
+      for (int j = 0; j < W::E; ++j) o[j] = score_dx(r, (float)raw[u].e[j], a.c);
+      store_chunk<T, W::E>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
+    }
+  }
+  // the named elements again, after the barrier: the last store to an address is theirs
+  __syncthreads();
+  const bool row_empty = a.tape[2 * row + 1] == 0.f;
+  if (tid < k && !row_empty) {
+    const long long i = a.top_index[row * k + tid];
+    float g = a.g_top[row * k + tid];
+    if (r.has_target && i == r.target) { g += r.g_target; target_named = 1; }
+    if (i >= lo && i < lo + w.len) dx[i] = (T)(score_dx(r, (float)x[i], a.c) + g * a.inv_t);
+  }
+  __syncthreads();
+  if (tid == 0 && r.has_target && !target_named && r.target >= lo && r.target < lo + w.len)
+    dx[r.target] = (T)(score_dx(r, (float)x[r.target], a.c) + r.g_target * a.inv_t);
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
+  __shared__ uint32_t lds[64 * 65];
+  const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
+  const long row = (long)blockIdx.x * 64 + threadIdx.x;
+  stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {
+    uint32_t* o = lds + threadIdx.x * pitch;
+    auto add = [&](long long i, float v) { o[i] = __float_as_uint(__uint_as_float(o[i]) + v); };
+    const int k = a.g_top ? a.k : 0;
+    float gt = 0.f;
+    for (int j = 0; j < k; ++j) gt += a.g_top[row * k + j];
+    const ScoreGrad r = score_grad(a, row, gt);
+    for (int i = 0; i < V; ++i) o[i] = __float_as_uint(score_dx(r, __uint_as_float(o[i]), a.c));
+    if (a.tape[2 * row + 1] != 0.f) {
+      for (int j = 0; j < k; ++j) add(a.top_index[row * k + j], a.g_top[row * k + j] * a.inv_t);
+      if (r.has_target) add(r.target, r.g_target * a.inv_t);
+    }
+  }
+  __syncthreads();
+  stage_rows<T, true>((T*)a.dx + (long)blockIdx.x * 64 * V, V, rows, V, lds, pitch);
+}
+
+// ---------------------------------------------------------------- host launchers
+// Segments per row: 1 where the rows alone fill the card (two workgroups per CU) or a row is short; else enough
+// workgroups for four per CU, of at least 2048 elements (one step of a workgroup is 8192), and no more than the join takes.
+int score_segments(long T, int V, int k) {
+  if (V <= 8192 || T >= 512) return 1;
+  long s = (1024 + T - 1) / T, most = (V + 2047) / 2048;
+  if (s > most) s = most;
+  if (s > LOGITS_MAX_SEGMENTS) s = LOGITS_MAX_SEGMENTS;
+  if (k && s * k > LOGITS_JOIN_KEYS) s = LOGITS_JOIN_KEYS / k;
+  return (int)s;
+}
+static int segment_length(int V, int S) { return ((V + S - 1) / S + 31) / 32 * 32; }
+// segments that really hold elements once the length is rounded
+static int segments_used(int V, int len) { return (V + len - 1) / len; }
+
+template <typename T, int NT>
+static void launch_score(const ScoreArgs& a, int S, int len, hipStream_t s) {
+  const dim3 g((unsigned)(a.T * S)), b(NT);
+  if (a.entropy && a.k) hipLaunchKernelGGL((score_kernel<T, NT, true, true>), g, b, 0, s, a, S, len);
+  else if (a.entropy) hipLaunchKernelGGL((score_kernel<T, NT, true, false>), g, b, 0, s, a, S, len);
+  else if (a.k) hipLaunchKernelGGL((score_kernel<T, NT, false, true>), g, b, 0, s, a, S, len);
+  else hipLaunchKernelGGL((score_kernel<T, NT, false, false>), g, b, 0, s, a, S, len);
+}
+template <typename T>
+static void score_typed(const ScoreArgs& a, hipStream_t s) {
+  if (a.V <= 64) {
+    const dim3 g((unsigned)((a.T + 63) / 64));
+    if (a.entropy) hipLaunchKernelGGL((score_small_kernel<T, true>), g, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((score_small_kernel<T, false>), g, dim3(64), 0, s, a);
+    return;
+  }
+  if (a.V <= 2048) return launch_score<T, 64>(a, 1, a.V, s);
+  int S = score_segments(a.T, a.V, a.k);
+  const int len = S > 1 ? segment_length(a.V, S) : a.V;
+  S = S > 1 ? segments_used(a.V, len) : 1;
+  launch_score<T, 256>(a, S, len, s);
+  if (S > 1) {
+    if (a.entropy) hipLaunchKernelGGL((score_join_kernel<T, true>), dim3((unsigned)a.T), dim3(256), 0, s, a, S);
+    else hipLaunchKernelGGL((score_join_kernel<T, false>), dim3((unsigned)a.T), dim3(256), 0, s, a, S);
+  }
+}
+template <typename T>
+static void score_bwd_typed(const ScoreGradArgs& a, hipStream_t s) {
+  if (a.V <= 64) {
+    hipLaunchKernelGGL((score_bwd_small_kernel<T>), dim3((unsigned)((a.T + 63) / 64)), dim3(64), 0, s, a);
+  } else if (a.V <= 2048) {
+    hipLaunchKernelGGL((score_bwd_kernel<T, 64>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+  } else {
+    // the gradient of an element needs the row's two coefficients only: segments at will, 8192 elements are one step
+    const int len = logits_bwd_segment(a.T, a.V), S = segments_used(a.V, len);
+    hipLaunchKernelGGL((score_bwd_kernel<T, 256>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
+  }
+}
+// At least 8192 elements per workgroup; longer where that leaves more workgroups than a launch takes (2^31 - 1).
+int logits_bwd_segment(long T, int V) {
+  int len = 8192;
+  while ((long)segments_used(V, len) * T > 0x7FFFFFFFL) len *= 2;
+  return len;
+}
+hipError_t score_fwd(const ScoreArgs& a, hipStream_t s) {
+  Traced tr(K_SCORE, 0, s);
+  if (a.type == SCM_F32) score_typed<float>(a, s);
+  else if (a.type == SCM_BF16) score_typed<bf16>(a, s);
+  else score_typed<f16>(a, s);
+  return hipGetLastError();
+}
+hipError_t score_bwd(const ScoreGradArgs& a, hipStream_t s) {
+  Traced tr(K_SCORE, 0, s);
+  if (a.type == SCM_F32) score_bwd_typed<float>(a, s);
+  else if (a.type == SCM_BF16) score_bwd_typed<bf16>(a, s);
+  else score_bwd_typed<f16>(a, s);
+  return hipGetLastError();
+}
+
+}  // namespace scm

@@ -88,7 +88,7 @@ enum KernelId {   // one id per kernel symbol family that a profiler lists separ
   K_WGRAD = 12, K_WGRAD_BIAS, K_WGRAD_REDUCE, K_CAST, K_EMBED_FWD, K_EMBED_BWD, K_LN_FWD, K_LN_BWD, K_HEAD_FWD,
   K_HEAD_BWD, K_COLSUM, K_PREP_OMEGA, K_CTX_FWD, K_CTX_BWD, K_CTX_FINALIZE, K_APPLY_FWD, K_APPLY_BWD_Q,
   K_APPLY_BWD_K, K_KFIX, K_S1_MASK, K_CE, K_BIN, K_OMEGA_QR, K_FEATURE_MAP, K_LINEAR_ATTENTION, K_FFN_CHAIN_FWD,
-  K_REDUCE_BATCH, K_GEMM_LN_BWD, K_GEMM_RES_LN, K_ADAM, K_CELL_TAIL, K_DISTILL_TAIL, K_NORM, K_COUNT
+  K_REDUCE_BATCH, K_GEMM_LN_BWD, K_GEMM_RES_LN, K_ADAM, K_CELL_TAIL, K_DISTILL_TAIL, K_NORM, K_SCORE, K_TOPK_DISTILL, K_COUNT
 };
 void trace_begin(int kid, double flops, double bytes, hipStream_t s);
 void trace_end(int kid, hipStream_t s);
@@ -185,6 +185,32 @@ bool norm_types_ok(int x_type, int y_type);
 int norm_bwd_blocks(long T, int D);
 hipError_t norm_fwd(const NormArgs& a, hipStream_t s);
 hipError_t norm_bwd(const NormArgs& a, float* dgamma, float* dbeta, hipStream_t s);
+
+// logits.hip, topk_distill.hip: rows of logits
+constexpr int LOGITS_MAX_K = 64;          // alternatives / teacher entries per row: one lane each
+constexpr int LOGITS_MAX_SEGMENTS = 64;   // workgroups that share a row
+constexpr int LOGITS_JOIN_KEYS = 2048;    // segments x alternatives that the join takes
+struct ScoreArgs {
+  const void* x; long ldx; int type; long T; int V, k;
+  float c, inv_t;                     // log2(e) / temperature, 1 / temperature
+  const int64_t* target; long long ignore;
+  float* logprob; float* lse; float* entropy;      // entropy may be null, logprob goes with target
+  float* top_logprob; int64_t* top_index;
+  float* tape;                        // [T][2] maximum and sum, or null
+  unsigned long* part_top; float* part;            // split rows: [T][S][k] keys, [T][S][3] statistics
+};
+struct ScoreGradArgs {
+  const void* x; long ldx; int type; long T; int V, k;
+  float c, inv_t;
+  const int64_t* target; long long ignore;
+  const float* tape; const float* entropy; const int64_t* top_index;
+  const float* g_logprob; const float* g_lse; const float* g_entropy; const float* g_top;   // each may be null
+  void* dx;
+};
+int score_segments(long T, int V, int k);
+int logits_bwd_segment(long T, int V);
+hipError_t score_fwd(const ScoreArgs& a, hipStream_t s);
+hipError_t score_bwd(const ScoreGradArgs& a, hipStream_t s);
 
 // optim.hip
 using AdamItem = ::scm_adam_item;

@@ -1,0 +1,96 @@
+// What the kernels that read rows of logits share: running softmax statistics and their joins, the walk of a workgroup
+// over a row (or a segment of one), and the staging of short rows.
+#pragma once
+#include "scm_chunk.hpp"
+
+namespace scm {
+
+constexpr float LOWEST = -3.402823466e38f;
+constexpr float LN2 = 0.6931471805599453f;
+
+SCM_DEV float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+
+// ---------------------------------------------------------------- softmax statistics
+// m: maximum of the elements (LOWEST where there are none above it), s = sum 2^((x-m)c), h = sum 2^((x-m)c) (x-m)c.
+// s == 0: no element above -inf.  s is NaN where an element is NaN or +inf.
+struct Stat { float m, s, h; };
+SCM_DEV Stat stat_none() { return {LOWEST, 0.f, 0.f}; }
+// The factor for a maximum that grew: 2^-200 is 0 in f32, and the bound keeps 0 * inf out of h.
+SCM_DEV float grown(float from, float to, float c) { return fmaxf((from - to) * c, -200.f); }
+template <bool ENT>
+SCM_DEV Stat stat_join(const Stat& a, const Stat& b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  const float da = grown(a.m, m, c), db = grown(b.m, m, c);
+  const float fa = exp2_fast(da), fb = exp2_fast(db);
+  Stat r{m, a.s * fa + b.s * fb, 0.f};
+  if constexpr (ENT) r.h = fa * (a.h + da * a.s) + fb * (b.h + db * b.s);
+  return r;
+}
+template <bool ENT>
+SCM_DEV Stat stat_wave(Stat v, float c) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    Stat w{__shfl_xor(v.m, o), __shfl_xor(v.s, o), 0.f};
+    if constexpr (ENT) w.h = __shfl_xor(v.h, o);
+    v = (threadIdx.x & o) ? stat_join<ENT>(w, v, c) : stat_join<ENT>(v, w, c);   // the same order in both lanes
+  }
+  return v;
+}
+// Over the NT threads of the workgroup, in every thread.  red: NT / 64 entries.
+template <bool ENT, int NT>
+SCM_DEV Stat stat_block(Stat v, float c, Stat* red) {
+  v = stat_wave<ENT>(v, c);
+  if constexpr (NT == 64) return v;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  Stat r = red[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) r = stat_join<ENT>(r, red[w], c);
+  return r;
+}
+
+// Per-thread view of a segment [lo, lo + len) of a row: chunk i of the thread is chunk tid + NT * i of the segment.
+template <typename T, int NT>
+struct Walk {
+  static constexpr int E = 16 / sizeof(T), U = 32 / E;   // U chunks = 32 elements a thread and step
+  const T* p;
+  int len;
+  SCM_DEV int steps() const { return (len + NT * U * E - 1) / (NT * U * E); }
+  SCM_DEV int first(int step, int u) const { return ((step * U + u) * NT + (int)threadIdx.x) * E; }
+  SCM_DEV void load(int step, Chunk<T, E> (&raw)[U]) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = load_chunk<T, E>(p + first(step, u), len - first(step, u));
+  }
+};
+
+// Adds 32 elements to a thread's running statistics.
+template <bool ENT>
+SCM_DEV void stat_add(Stat& st, const float (&v)[32], float bm, float c) {
+  const float m = fmaxf(st.m, bm);
+  const float d0 = grown(st.m, m, c), f = exp2_fast(d0);
+  float s = st.s * f, h = ENT ? f * (st.h + d0 * st.s) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float d = (v[j] - m) * c, e = exp2_fast(d);
+    s += e;
+    if constexpr (ENT) h += e * fmaxf(d, -200.f);
+  }
+  st = {m, s, h};
+}
+
+// Rows of at most 64 logits, one thread each: 64 rows go through LDS (row stride odd: no bank conflicts along a
+// column) as f32 bits, read and written along memory.
+template <typename T, bool STORE>
+SCM_DEV void stage_rows(T* p, long ld, int rows, int V, uint32_t* lds, int pitch) {
+  const int dr = 64 / V, dc = 64 % V;
+  int r = threadIdx.x / V, c = threadIdx.x % V;
+  while (r < rows) {
+    if constexpr (STORE) p[r * ld + c] = (T)__uint_as_float(lds[r * pitch + c]);
+    else lds[r * pitch + c] = __float_as_uint((float)p[r * ld + c]);
+    r += dr;
+    c += dc;
+    if (c >= V) { c -= V; ++r; }
+  }
+}
+
+}  // namespace scm

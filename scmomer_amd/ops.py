@@ -623,6 +623,84 @@ def s1_accuracy(logits: torch.Tensor, labels: torch.Tensor, pad_id: int):
     return ratio, counts
 
 
+# ----------------------------------------------------------------------------- rows of logits
+LOGITS_MAX_K = 64
+
+
+def _logits_rows(logits: torch.Tensor, temperature: float, k: int) -> torch.Tensor:
+    x = rows_of(logits, "logits")
+    if not x.is_cuda:
+        raise ValueError("logits: expected a device tensor; scmomer_amd has no CPU path")
+    if x.shape[1] > 1 << 30:
+        raise ValueError(f"logits: at most 2^30 classes (got {x.shape[1]})")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 0 <= k <= LOGITS_MAX_K:
+        raise ValueError(f"at most {LOGITS_MAX_K} entries per row (got {k})")
+    return x
+
+
+def _row_vector(t: torch.Tensor, rows: int, dtype, name: str) -> torch.Tensor:
+    """one value per row of the logits, contiguous"""
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a device tensor; scmomer_amd has no CPU path")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.numel() != rows:
+        raise ValueError(f"{name}: {t.numel()} values for {rows} rows of logits")
+    return t.contiguous()
+
+
+def score_fwd(logits, targets, k: int = 0, temperature: float = 1.0, ignore_index: int = -100, entropy: bool = True,
+              tape: bool = False):
+    """Rows of logits [..., V] -> (logprob [T] or None, entropy [T] or None, lse [T], top_logprob [T, k] or None,
+    top_index int64 [T, k] or None, tape [T, 2] or None); what score_bwd needs is the tape, entropy and top_index"""
+    x = _logits_rows(logits, temperature, k)
+    t, v = x.shape
+    if k > v:
+        raise ValueError(f"{k} alternatives of {v} classes")
+    if targets is not None:
+        if targets.shape != logits.shape[:-1]:
+            raise ValueError(f"targets: expected {tuple(logits.shape[:-1])}, got {tuple(targets.shape)}")
+        targets = _row_vector(targets, t, torch.int64, "targets")
+    dev = x.device
+    with _on_device(x, targets):
+        lp = torch.empty(t, dtype=F32, device=dev) if targets is not None else None
+        lse = torch.empty(t, dtype=F32, device=dev)
+        ent = torch.empty(t, dtype=F32, device=dev) if entropy else None
+        tlp = torch.empty((t, k), dtype=F32, device=dev) if k else None
+        tix = torch.empty((t, k), dtype=torch.int64, device=dev) if k else None
+        mz = torch.empty((t, 2), dtype=F32, device=dev) if tape else None
+        if t:
+            n = lib.scm_score_ws_floats(t, v, k)
+            ws = torch.empty(n, dtype=F32, device=dev) if n else None
+            check(lib.scm_score_fwd(_p(x), SCM_TYPES[x.dtype], x.stride(0), t, v, temperature, _p(targets), ignore_index, k,
+                                    _p(lp), _p(lse), _p(ent), _p(tlp), _p(tix), _p(mz), _p(ws), _stream()), "scm_score_fwd")
+    return lp, ent, lse, tlp, tix, mz
+
+
+def score_bwd(logits, targets, tape, entropy, top_index, g_logprob, g_entropy, g_lse, g_top, temperature: float = 1.0,
+              ignore_index: int = -100) -> torch.Tensor:
+    """-> the gradient [T, V] in the logits' type; each g_* is a tensor of its output's size or None"""
+    k = top_index.shape[1] if top_index is not None else 0
+    x = _logits_rows(logits, temperature, k)
+    t, v = x.shape
+    g_logprob, g_entropy, g_lse = (g if g is None else g.to(F32).reshape(-1).contiguous() for g in (g_logprob, g_entropy, g_lse))
+    g_top = g_top if g_top is None else g_top.to(F32).reshape(t, k).contiguous()
+    for g, nm in ((g_logprob, "logprob"), (g_entropy, "entropy"), (g_lse, "lse")):
+        if g is not None and g.numel() != t:
+            raise ValueError(f"gradient of {nm}: {g.numel()} values for {t} rows")
+    if targets is not None:
+        targets = _row_vector(targets, t, torch.int64, "targets")
+    with _on_device(x, targets, tape, entropy, top_index, g_logprob, g_entropy, g_lse, g_top):
+        dx = torch.empty((t, v), dtype=x.dtype, device=x.device)
+        if t:
+            check(lib.scm_score_bwd(_p(x), SCM_TYPES[x.dtype], x.stride(0), t, v, temperature, _p(targets), ignore_index, k,
+                                    _p(tape), _p(entropy), _p(top_index), _p(g_logprob), _p(g_lse), _p(g_entropy), _p(g_top),
+                                    _p(dx), _stream()), "scm_score_bwd")
+    return dx
+
+
 # ----------------------------------------------------------------------------- cell-embedding tail
 def cell_tail_supported(p: int, hd: int, o: int) -> bool:
     return p <= 1024 and hd <= 1024 and o <= 1024 and p + hd <= 1024 and (p + hd) % 64 == 0

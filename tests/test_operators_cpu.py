@@ -49,3 +49,51 @@ def test_norm_workspace_sizes():
     assert lib.scm_norm_bwd_ws_floats(0, 8) == 0 and lib.scm_norm_bwd_ws_floats(8, 16385) == 0
     assert lib.scm_norm_bwd_ws_floats(1, 7) == 14
     assert lib.scm_norm_bwd_ws_floats(1 << 30, 4096) <= 2 * 4096 * 2048
+
+
+def test_token_logprobs_needs_device_tensors():
+    from scmomer_amd.logits import token_logprobs
+    with pytest.raises(ValueError):
+        token_logprobs(torch.randn(2, 8), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(TypeError):
+        token_logprobs(torch.zeros(2, 8, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("change", [dict(x=None), dict(type=3), dict(ldx=-1), dict(T=0), dict(T=1 << 31), dict(V=0),
+                                    dict(V=(1 << 30) + 1), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("inf")),
+                                    dict(tau=float("nan")), dict(k=-1), dict(k=65), dict(k=9), dict(target=None),
+                                    dict(logprob=None), dict(top=None), dict(index=None), dict(V=100000, k=3, ws=None),
+                                    dict(ws_off=4)])
+def test_score_fwd_rejects(change):
+    from scmomer_amd._lib import lib
+    keep, a = _addr()
+    k = dict(x=a, type=0, ldx=8, T=1, V=8, tau=1.0, target=a, k=2, logprob=a, top=a, index=a, ws=a, ws_off=0)
+    k.update(change)
+    ws = k["ws"] + k["ws_off"] if k["ws"] else None
+    rc = lib.scm_score_fwd(k["x"], k["type"], k["ldx"], k["T"], k["V"], k["tau"], k["target"], -100, k["k"], k["logprob"],
+                           a, a, k["top"], k["index"], a, ws, None)
+    assert rc < 0 and b"scm_score_fwd" in lib.scm_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(x=None), dict(tape=None), dict(dx=None), dict(target=None), dict(entropy=None),
+                                    dict(index=None), dict(k=0), dict(type=-1), dict(tau=0.0)])
+def test_score_bwd_rejects(change):
+    from scmomer_amd._lib import lib
+    keep, a = _addr()
+    k = dict(x=a, type=0, tau=1.0, target=a, k=2, tape=a, entropy=a, index=a, dx=a)
+    k.update(change)
+    rc = lib.scm_score_bwd(k["x"], k["type"], 8, 1, 8, k["tau"], k["target"], -100, k["k"], k["tape"], k["entropy"],
+                           k["index"], a, a, a, a, k["dx"], None)
+    assert rc < 0 and b"scm_score_bwd" in lib.scm_last_error()
+
+
+def test_score_workspace_holds_every_split():
+    """a split row's keys and statistics fit the workspace, and the join's limits hold"""
+    from scmomer_amd._lib import lib
+    for t in (1, 3, 100, 511, 512, 100000):
+        for v in (1, 64, 8192, 8193, 131072, 1 << 30):
+            for k in (0, 1, 20, 64):
+                n = lib.scm_score_ws_floats(t, v, k)
+                s = n // (t * (2 * k + 3))
+                assert n == s * t * (2 * k + 3) and s <= 64 and s * k <= 2048 and s != 1
+    assert lib.scm_score_ws_floats(1, 100, 65) == 0 and lib.scm_score_ws_floats(0, 100, 1) == 0
