@@ -303,6 +303,33 @@ int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
                   const float* g_logprob, const float* g_lse, const float* g_entropy, const float* g_top, void* dx,
                   void* stream);
 
+/* ---- distillation towards a teacher's top log probabilities, for any vocabulary (the S3 distillation further down is
+ *      an MSE between embeddings).  No counterpart in the reference.  x, T, V, ldx, type, temperature as scm_score_fwd;
+ *      index int64 [T,k], logprob f32 [T,k], 1 <= k <= 64: the teacher's entries at the same temperature, as
+ *      scm_score_fwd writes them; index < 0: entry not used.  Per row, with q = exp(logprob) and p = softmax(z):
+ *        tail != 0: KL(q, r || p at the entries, p elsewhere), r = max(0, 1 - sum q) the bucket of all other tokens
+ *                   (left out where the student gives all of those -inf);
+ *        tail == 0: KL(q / sum q || p at the entries).
+ *      An index named twice counts with both its q; index >= V or NaN make the row's loss and gradient NaN; a row of
+ *      -inf only has loss and gradient 0.  weight [T] (may be NULL: 1): row_loss = weight * loss, rows of weight 0 are
+ *      not read; loss (one float, may be NULL in the forward) = sum of row_loss, divided by the sum of the weights when
+ *      mean; wsum (one float, may be NULL): that sum.  The loss is not multiplied by temperature^2.
+ *      tape: scm_topk_distill_tape_floats floats (0 for V <= 64), NULL in the forward where no backward follows;
+ *      ws: scm_topk_distill_ws_floats floats.
+ *      bwd: dx [T,V] (x's type, contiguous) = gloss[0] (gloss_rows: gloss[t]) * the gradient of the loss (row_loss).
+ *      step: loss, and dx = scale * its gradient, without a backward of its own; a row is read from memory once. */
+int64_t scm_topk_distill_tape_floats(int64_t T, int V, int k);
+int64_t scm_topk_distill_ws_floats(int64_t T, int V);
+int scm_topk_distill_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
+                         const float* logprob, int k, int tail, const float* weight, int mean, float* row_loss,
+                         float* loss, float* wsum, float* tape, float* ws, void* stream);
+int scm_topk_distill_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
+                         const float* logprob, int k, int tail, const float* weight, int mean, const float* wsum,
+                         const float* gloss, int gloss_rows, const float* tape, void* dx, void* stream);
+int scm_topk_distill_step(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
+                          const float* logprob, int k, int tail, const float* weight, int mean, float scale,
+                          float* row_loss, float* loss, float* wsum, float* tape, float* ws, void* dx, void* stream);
+
 /* ---- final LayerNorm + head: performer_pytorch.py:628-634 (Linear(dim,num_tokens)); rna_encoder.py:5-16
  *      (1x200 conv == dot product, + ReLU; C = 1, relu = 1) -------------------------------------- */
 /* enc (may be NULL) f32 [T,D] = LN(x); out (may be NULL when C == 0) f32 [T,C]. */

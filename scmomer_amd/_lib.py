@@ -88,6 +88,12 @@ SIGNATURES = {
     "scm_score_ws_floats": (i64, [i64, i32, i32]),
     "scm_score_fwd": (i32, [vp, i32, i64, i64, i32, C.c_float, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "scm_score_bwd": (i32, [vp, i32, i64, i64, i32, C.c_float, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "scm_topk_distill_tape_floats": (i64, [i64, i32, i32]),
+    "scm_topk_distill_ws_floats": (i64, [i64, i32]),
+    "scm_topk_distill_fwd": (i32, [vp, i32, i64, i64, i32, C.c_float, vp, vp, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp]),
+    "scm_topk_distill_bwd": (i32, [vp, i32, i64, i64, i32, C.c_float, vp, vp, i32, i32, vp, i32, vp, vp, i32, vp, vp, vp]),
+    "scm_topk_distill_step": (i32, [vp, i32, i64, i64, i32, C.c_float, vp, vp, i32, i32, vp, i32, C.c_float, vp, vp, vp, vp,
+                                    vp, vp, vp]),
     "scm_norm_fwd": (i32, [vp, i32, i64, vp, vp, i64, i32, C.c_float, vp, i32, vp, vp, vp]),
     "scm_norm_bwd_ws_floats": (i64, [i64, i32]),
     "scm_norm_bwd": (i32, [vp, i32, i64, vp, i32, i64, vp, vp, vp, i64, i32, vp, vp, vp, vp, vp]),

@@ -303,6 +303,64 @@ int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
   return 0;
 }
 
+int64_t scm_topk_distill_tape_floats(int64_t T, int V, int k) {
+  return T > 0 && V > 64 && k > 0 && k <= LOGITS_MAX_K ? T * (2 + (int64_t)k) : 0;
+}
+int64_t scm_topk_distill_ws_floats(int64_t T, int V) {
+  if (T <= 0 || V <= 64) return 0;
+  const int64_t S = distill_segments(T, V);
+  return S > 1 ? 2 * T * S : 0;
+}
+static int distill_topk_args(const char* who, DistillTopkArgs& a, const void* x, int type, int64_t ldx, int64_t T, int V,
+                             float temperature, const int64_t* index, const float* logprob, int k, int tail,
+                             const float* weight, int mean, float* tape) {
+  if (int e = logits_check(who, x, type, ldx, T, V, k, temperature)) return e;
+  SCM_REQ(k > 0 && index && logprob, "%s: no teacher entries", who);
+  SCM_REQ(T * distill_segments(T, V) < ((int64_t)1 << 31), "%s: too many rows", who);
+  a = DistillTopkArgs{};
+  a.x = x; a.ldx = ldx; a.type = type; a.T = T; a.V = V; a.k = k; a.tail = tail != 0; a.mean = mean != 0;
+  a.c = log2e_over(temperature); a.inv_t = 1.f / temperature; a.index = index; a.lp = logprob; a.weight = weight;
+  if (tape && V > 64) { a.tape = tape; a.g_top = tape + 2 * T; }
+  return 0;
+}
+int scm_topk_distill_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
+                         const float* logprob, int k, int tail, const float* weight, int mean, float* row_loss,
+                         float* loss, float* wsum, float* tape, float* ws, void* stream) {
+  DistillTopkArgs a;
+  if (int e = distill_topk_args("scm_topk_distill_fwd", a, x, type, ldx, T, V, temperature, index, logprob, k, tail, weight,
+                                mean, tape)) return e;
+  SCM_REQ(row_loss, "scm_topk_distill_fwd: null pointer");
+  SCM_REQ(ws || scm_topk_distill_ws_floats(T, V) == 0, "scm_topk_distill_fwd: null workspace");
+  a.row_loss = row_loss; a.part = ws;
+  SCM_HIP(topk_distill_fwd(a, loss, wsum, (hipStream_t)stream), "scm_topk_distill_fwd");
+  return 0;
+}
+int scm_topk_distill_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
+                         const float* logprob, int k, int tail, const float* weight, int mean, const float* wsum,
+                         const float* gloss, int gloss_rows, const float* tape, void* dx, void* stream) {
+  DistillTopkArgs a;
+  if (int e = distill_topk_args("scm_topk_distill_bwd", a, x, type, ldx, T, V, temperature, index, logprob, k, tail, weight,
+                                mean, const_cast<float*>(tape))) return e;
+  SCM_REQ(gloss && dx && (tape || V <= 64), "scm_topk_distill_bwd: null pointer");
+  SCM_REQ(!(mean && weight) || wsum, "scm_topk_distill_bwd: a weighted mean needs the weights' sum");
+  a.gloss = gloss; a.gloss_rows = gloss_rows != 0; a.wsum = weight ? wsum : nullptr; a.dx = dx;
+  SCM_HIP(topk_distill_bwd(a, (hipStream_t)stream), "scm_topk_distill_bwd");
+  return 0;
+}
+int scm_topk_distill_step(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
+                          const float* logprob, int k, int tail, const float* weight, int mean, float scale,
+                          float* row_loss, float* loss, float* wsum, float* tape, float* ws, void* dx, void* stream) {
+  DistillTopkArgs a;
+  if (int e = distill_topk_args("scm_topk_distill_step", a, x, type, ldx, T, V, temperature, index, logprob, k, tail, weight,
+                                mean, tape)) return e;
+  SCM_REQ(row_loss && loss && dx && (tape || V <= 64), "scm_topk_distill_step: null pointer");
+  SCM_REQ(!(mean && weight) || wsum, "scm_topk_distill_step: a weighted mean needs room for the weights' sum");
+  SCM_REQ(ws || scm_topk_distill_ws_floats(T, V) == 0, "scm_topk_distill_step: null workspace");
+  a.row_loss = row_loss; a.part = ws; a.scale = scale; a.wsum = weight && mean ? wsum : nullptr; a.dx = dx;
+  SCM_HIP(topk_distill_step(a, loss, wsum, (hipStream_t)stream), "scm_topk_distill_step");
+  return 0;
+}
+
 int scm_gemm_res_ln_supported(int64_t M, int D, int K, int64_t lda, int64_t ldw) {
   return (M > 0 && M < (1ll << 31) && D > 0 && K > 0 && lda % 8 == 0 && ldw % 8 == 0 && lda >= K && ldw >= K &&
           gemm_res_ln_supported((long)M, D, K, (long)lda, (long)ldw)) ? 1 : 0;

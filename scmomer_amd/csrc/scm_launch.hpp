@@ -212,6 +212,22 @@ int logits_bwd_segment(long T, int V);
 hipError_t score_fwd(const ScoreArgs& a, hipStream_t s);
 hipError_t score_bwd(const ScoreGradArgs& a, hipStream_t s);
 
+struct DistillTopkArgs {
+  const void* x; long ldx; int type; long T; int V, k, tail, mean;
+  float c, inv_t;
+  const int64_t* index; const float* lp;           // [T][k]
+  const float* weight;                             // [T] or null
+  float* row_loss;                                 // [T]
+  float* tape; float* g_top;                       // V > 64: [T][2], [T][k], or null
+  float* part;                                     // split rows: [T][S][2]
+  const float* wsum; const float* gloss; int gloss_rows; float scale;   // gradient: gloss or scale
+  void* dx;
+};
+int distill_segments(long T, int V);
+hipError_t topk_distill_fwd(const DistillTopkArgs& a, float* out, float* wsum_out, hipStream_t s);
+hipError_t topk_distill_bwd(const DistillTopkArgs& a, hipStream_t s);
+hipError_t topk_distill_step(const DistillTopkArgs& a, float* out, float* wsum, hipStream_t s);
+
 // optim.hip
 using AdamItem = ::scm_adam_item;
 struct AdamScalars { float grad_scale, max_norm, one_minus_beta1, beta2, one_minus_beta2, eps, step_size, bc2_sqrt; };

@@ -1,0 +1,424 @@
+// Distillation from a teacher's k named log probabilities.  Per row, with z = x / temperature the student's logits,
+// entries (i_j, l_j), q_j = exp l_j, R the vocabulary without the named tokens:
+//   tail bucket:   r = max(0, 1 - sum q_j);     renormalised:  q_j /= sum q_j, r = 0
+//   L    = sum_j q_j (l_j - z_{i_j} + lse) + r (ln r - lse_R + lse)          lse over all tokens, lse_R over R
+//   dz_i = A p_i - [i named] sum_{i_j = i} q_j - [i in R] r exp(z_i - lse_R),   A = sum q_j + r
+// The named tokens are left out of the running sum (a bit per token in LDS tells them apart) and join it afterwards, so
+// lse_R is exact where the student is nearly sure of them: no difference of nearly equal sums is formed.  For i in R
+// the gradient is one exponential times a factor of the row, cr = A p(R) / s_R - r / s_R:  dz_i = cr 2^((x_i - m_R) c).
+// Conventions: i_j < 0 is an unused entry; an index named twice counts once in R's complement and with both its q; where
+// the student has nothing in R (-inf throughout) r is left out; a row of -inf only and a row of weight 0 have loss and
+// gradient 0; i_j >= V and NaN give NaN.
+//
+// Bound by HBM: the loss reads the logits once, the gradient reads them once more and writes once; the two in one pass
+// (one workgroup per row) read a row the second time while it is still in the caches.
+#include "scm_softmax.hpp"
+
+namespace scm {
+
+constexpr int DISTILL_SEGMENT = 131072;   // tokens whose bits fit a workgroup's 16 KB
+
+// ---------------------------------------------------------------- one row's end: lane j of a wave holds entry j
+struct DistillRow {
+  float loss, m, cr;   // the loss; reference maximum and factor of the gradient in R
+  float g;             // lane j: gradient at its named token
+};
+SCM_DEV double wave_sum_f64(double v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// rest: statistics over R.  idx (< 0: unused), lp, x (the student's logit there) of this lane's entry.
+SCM_DEV DistillRow distill_row(const DistillTopkArgs& a, const Stat& rest, long long idx, float lp, float x) {
+  const int lane = threadIdx.x & 63;
+  const bool used = idx >= 0;
+  const bool beyond = __builtin_amdgcn_ballot_w64(used && idx >= a.V) != 0;
+  // the first of equal indices, and the sum of q over them
+  double q = used ? exp((double)lp) : 0.0;
+  const double total = wave_sum_f64(q);
+  float r = 0.f;
+  if (a.tail) {
+    r = rest.s == 0.f ? 0.f : (float)fmax(0.0, 1.0 - total);
+    if (total != total) r = (float)total;
+  } else if (total > 0.0) {
+    q /= total;
+    lp -= (float)log(total);
+  }
+  const float qf = (float)q;
+  float qsum = 0.f;
+  bool first = used;
+  for (int j = 0; j < a.k; ++j) {
+    const long long ij = __shfl(idx, j);
+    const float qj = __shfl(qf, j);
+    if (used && ij == idx) {
+      qsum += qj;
+      if (j < lane) first = false;
+    }
+  }
+  // all tokens: R and the named ones
+  const float m = wave_max(fmaxf(rest.m, used ? x : LOWEST));
+  const float f = exp2_fast(fmaxf((rest.m - m) * a.c, -200.f));
+  const float e = used ? exp2_fast((x - m) * a.c) : 0.f;
+  const float z = rest.s * f + wave_sum(first ? e : 0.f);
+  const float l2 = log2_fast(z);
+  const float logp = (x - m) * a.inv_t - LN2 * l2;
+  float loss = wave_sum(used && qf > 0.f ? qf * (lp - logp) : 0.f);
+  if (r > 0.f) loss += r * (logf(r) - ((rest.m - m) * a.inv_t + LN2 * (log2_fast(rest.s) - l2)));
+  const float big_a = (float)wave_sum_f64(q) + r;
+  DistillRow o;
+  o.loss = loss;
+  o.m = rest.m;
+  o.cr = rest.s == 0.f ? 0.f : big_a * f / z - r / rest.s;
+  o.g = big_a * e / z - qsum;
+  if (z == 0.f) { o.loss = 0.f; o.cr = 0.f; o.g = 0.f; }   // nothing above -inf
+  if (beyond || total != total || rest.s != rest.s || z != z) o.loss = o.cr = o.g = __uint_as_float(0x7FC00000u);
+  return o;
+}
+// weight of a row, and what its gradient is scaled by
+SCM_DEV float row_scale(const DistillTopkArgs& a, long row, float w) {
+  const float g = a.gloss ? a.gloss[a.gloss_rows ? row : 0] : a.scale;
+  return g * w * a.inv_t / (a.mean ? (a.wsum ? a.wsum[0] : (float)a.T) : 1.f);
+}
+
+// ---------------------------------------------------------------- statistics over R of a segment
+template <int NT>
+struct NamedBits {
+  static constexpr int WORDS = NT == 64 ? 2048 / 32 : DISTILL_SEGMENT / 32;
+  uint32_t w[WORDS];
+};
+// Marks the named tokens of [lo, lo + len).  Ends with a barrier.
+template <int NT>
+SCM_DEV void mark_named(NamedBits<NT>& bits, const int64_t* idx, int k, int lo, int len) {
+  for (int i = threadIdx.x; i < (len + 31) / 32; i += NT) bits.w[i] = 0;
+  __syncthreads();
+  if ((int)threadIdx.x < k) {
+    const long long i = idx[threadIdx.x] - lo;
+    if (i >= 0 && i < len) atomicOr(&bits.w[i >> 5], 1u << (i & 31));
+  }
+  __syncthreads();
+}
+template <typename T, int NT>
+SCM_DEV Stat rest_of_segment(const Walk<T, NT>& w, const NamedBits<NT>& bits, float c) {
+  typedef Walk<T, NT> W;
+  Stat st = stat_none();
+  for (int s = 0; s < w.steps(); ++s) {
+    Chunk<T, W::E> raw[W::U];
+    w.load(s, raw);
+    float v[32], bm = LOWEST;
+#pragma unroll
+    for (int u = 0; u < W::U; ++u) {
+      const int i0 = w.first(s, u), n = w.len - i0;
+      const uint32_t named = n > 0 ? bits.w[i0 >> 5] >> (i0 & 31) : 0u;   // this chunk's bits, lowest first
+#pragma unroll
+      for (int j = 0; j < W::E; ++j) {
+        const float x = (j < n && !((named >> j) & 1)) ? (float)raw[u].e[j] : -INFINITY;
+        v[u * W::E + j] = x;
+        bm = fmaxf(bm, x);
+      }
+    }
+    stat_add<false>(st, v, bm, c);
+  }
+  return st;
+}
+
+// Gradient of a segment from (m, cr), then the named tokens over it.
+template <typename T, int NT>
+SCM_DEV void distill_write(const Walk<T, NT>& w, T* dx, int lo, float m, float cr, float c) {
+  typedef Walk<T, NT> W;
+  for (int s = 0; s < w.steps(); ++s) {
+    Chunk<T, W::E> raw[W::U];
+    w.load(s, raw);
+#pragma unroll
+    for (int u = 0; u < W::U; ++u) {
+      float o[W::E];
+#pragma unroll
+      for (int j = 0; j < W::E; ++j) o[j] = cr * exp2_fast(((float)raw[u].e[j] - m) * c);
+      store_chunk<T, W::E>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
+    }
+  }
+}
+template <typename T, int NT>
+SCM_DEV void zero_write(T* dx, int len) {
+  constexpr int E = 16 / sizeof(T);
+  const float none[E] = {};
+  for (int i = threadIdx.x * E; i < len; i += NT * E) store_chunk<T, E>(dx + i, none, len - i);
+}
+
+// ---------------------------------------------------------------- V > 64
+// GRAD: loss and gradient in one launch (S = 1).  Otherwise the loss, and (tape, g_top given) what the backward reads;
+// with S > 1 the segment's statistics go to part for distill_join_kernel.
+template <typename T, int NT, bool GRAD>
+__global__ __launch_bounds__(NT) void distill_kernel(DistillTopkArgs a, int S, int seg_len) {
+  __shared__ Stat red[NT / 64];
+  __shared__ NamedBits<NT> bits;
+  __shared__ float row_m, row_cr;
+  const long row = blockIdx.x / S;
+  const int seg = blockIdx.x % S, lo = seg * seg_len, tid = threadIdx.x;
+  const T* x = (const T*)a.x + row * a.ldx;
+  const Walk<T, NT> w{x + lo, min(a.V - lo, seg_len)};
+  T* dx = GRAD ? (T*)a.dx + row * a.V : nullptr;
+  const float wt = a.weight ? a.weight[row] : 1.f;
+  if (wt == 0.f) {
+    if constexpr (GRAD) zero_write<T, NT>(dx, a.V);
+    if (S == 1) {
+      if (tid == 0) a.row_loss[row] = 0.f;
+      if (a.tape && tid < a.k) a.g_top[row * a.k + tid] = 0.f;
+      if (a.tape && tid == 0) a.tape[2 * row] = a.tape[2 * row + 1] = 0.f;
+    }
+    return;
+  }
+  const int64_t* index = a.index + row * a.k;
+  mark_named<NT>(bits, index, a.k, lo, w.len);
+  const Stat st = stat_block<false, NT>(rest_of_segment<T, NT>(w, bits, a.c), a.c, red);
+  if (S > 1) {
+    if (tid == 0) { a.part[2 * (row * S + seg)] = st.m; a.part[2 * (row * S + seg) + 1] = st.s; }
+    return;
+  }
+  long long idx = -1;
+  float g = 0.f;
+  if (tid < 64) {
+    float lp = 0.f, xi = 0.f;
+    if (tid < a.k) {
+      idx = index[tid];
+      lp = a.lp[row * a.k + tid];
+      if (idx >= 0 && idx < a.V) xi = (float)x[idx];
+    }
+    const DistillRow r = distill_row(a, st, idx, lp, xi);
+    g = r.g;
+    if (tid == 0) { a.row_loss[row] = wt * r.loss; row_m = r.m; row_cr = r.cr; }
+    if (a.tape) {
+      if (tid == 0) { a.tape[2 * row] = r.m; a.tape[2 * row + 1] = r.cr; }
+      if (tid < a.k) a.g_top[row * a.k + tid] = g;
+    }
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    const float sc = row_scale(a, row, wt);
+    distill_write<T, NT>(w, dx, 0, row_m, row_cr * sc, a.c);
+    __syncthreads();   // the last store to a named token is this one; equal indices hold equal values
+    if (tid < a.k && idx >= 0 && idx < a.V) dx[idx] = (T)(g * sc);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(DistillTopkArgs a, int S) {
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float wt = a.weight ? a.weight[row] : 1.f;
+  if (wt == 0.f) {
+    if (tid == 0) a.row_loss[row] = 0.f;
+    if (a.tape && tid < a.k) a.g_top[row * a.k + tid] = 0.f;
+    if (a.tape && tid == 0) a.tape[2 * row] = a.tape[2 * row + 1] = 0.f;
+    return;
+  }
+  Stat st = stat_none();
+  for (int i = tid; i < S; i += 64)
+    st = stat_join<false>(st, Stat{a.part[2 * (row * S + i)], a.part[2 * (row * S + i) + 1], 0.f}, a.c);
+  st = stat_wave<false>(st, a.c);
+  long long idx = -1;
+  float lp = 0.f, xi = 0.f;
+  if (tid < a.k) {
+    idx = a.index[row * a.k + tid];
+    lp = a.lp[row * a.k + tid];
+    if (idx >= 0 && idx < a.V) xi = (float)((const T*)a.x)[row * a.ldx + idx];
+  }
+  const DistillRow r = distill_row(a, st, idx, lp, xi);
+  if (tid == 0) a.row_loss[row] = wt * r.loss;
+  if (a.tape) {
+    if (tid == 0) { a.tape[2 * row] = r.m; a.tape[2 * row + 1] = r.cr; }
+    if (tid < a.k) a.g_top[row * a.k + tid] = r.g;
+  }
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillTopkArgs a, int S, int seg_len) {
+  const long row = blockIdx.x / S;
+  const int lo = (int)(blockIdx.x % S) * seg_len, tid = threadIdx.x;
+  const Walk<T, NT> w{(const T*)a.x + row * a.ldx + lo, min(a.V - lo, seg_len)};
+  T* dx = (T*)a.dx + row * a.V;
+  const float wt = a.weight ? a.weight[row] : 1.f;
+  if (wt == 0.f) { zero_write<T, NT>(dx + lo, w.len); return; }
+  const float sc = row_scale(a, row, wt);
+  distill_write<T, NT>(w, dx, lo, a.tape[2 * row], a.tape[2 * row + 1] * sc, a.c);
+  __syncthreads();
+  if (tid < a.k) {
+    const long long i = a.index[row * a.k + tid];
+    if (i >= lo && i < lo + w.len) dx[i] = (T)(a.g_top[row * a.k + tid] * sc);
+  }
+}
+
+// ---------------------------------------------------------------- V <= 64: a thread per row, a bit per token
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
+  __shared__ uint32_t lds[64 * 65];
+  const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
+  const long row = (long)blockIdx.x * 64 + threadIdx.x;
+  stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {
+    uint32_t* o = lds + threadIdx.x * pitch;
+    auto x = [&](int i) { return __uint_as_float(o[i]); };
+    const float wt = a.weight ? a.weight[row] : 1.f;
+    float loss = 0.f;
+    if (wt != 0.f) {
+      const int64_t* index = a.index + row * a.k;
+      const float* lps = a.lp + row * a.k;
+      unsigned long long named = 0;
+      bool beyond = false;
+      double total = 0.0;
+      for (int j = 0; j < a.k; ++j) {
+        const long long i = index[j];
+        if (i < 0) continue;
+        if (i >= V) { beyond = true; continue; }
+        named |= 1ull << i;
+        total += exp((double)lps[j]);
+      }
+      Stat all = stat_none(), rest = stat_none();
+      for (int i = 0; i < V; ++i) {
+        all.m = fmaxf(all.m, x(i));
+        if (!((named >> i) & 1)) rest.m = fmaxf(rest.m, x(i));
+      }
+      for (int i = 0; i < V; ++i) {
+        all.s += exp2_fast((x(i) - all.m) * a.c);
+        if (!((named >> i) & 1)) rest.s += exp2_fast((x(i) - rest.m) * a.c);
+      }
+      const float l2 = log2_fast(all.s);
+      float r = 0.f, log_total = 0.f;
+      double per = 1.0;
+      if (a.tail) r = rest.s == 0.f ? 0.f : (float)fmax(0.0, 1.0 - total);
+      else if (total > 0.0) { per = 1.0 / total; log_total = (float)log(total); }
+      const float big_a = (float)(total * per) + r;
+      for (int j = 0; j < a.k; ++j) {
+        const long long i = index[j];
+        if (i < 0 || i >= V) continue;
+        const float lp = lps[j], q = (float)(exp((double)lp) * per);
+        if (q > 0.f) loss += q * (lp - log_total - ((x((int)i) - all.m) * a.inv_t - LN2 * l2));
+      }
+      if (r > 0.f) loss += r * (logf(r) - ((rest.m - all.m) * a.inv_t + LN2 * (log2_fast(rest.s) - l2)));
+      const bool empty = all.s == 0.f, broken = beyond || total != total || all.s != all.s;
+      if (empty) loss = 0.f;
+      if (broken) loss = __uint_as_float(0x7FC00000u);
+      loss *= wt;
+      if constexpr (GRAD) {
+        const float sc = row_scale(a, row, wt);
+        const float ca = big_a / all.s * sc, cr = rest.s == 0.f ? 0.f : r / rest.s * sc;
+        for (int i = 0; i < V; ++i) {
+          float g = ca * exp2_fast((x(i) - all.m) * a.c);
+          if (!((named >> i) & 1) && cr != 0.f) g -= cr * exp2_fast((x(i) - rest.m) * a.c);
+          o[i] = __float_as_uint(empty ? 0.f : broken ? __uint_as_float(0x7FC00000u) : g);
+        }
+        if (!empty && !broken)
+          for (int j = 0; j < a.k; ++j) {
+            const long long i = index[j];
+            if (i >= 0) o[i] = __float_as_uint(x((int)i) - (float)(exp((double)lps[j]) * per) * sc);
+          }
+      }
+    } else if constexpr (GRAD) {
+      for (int i = 0; i < V; ++i) o[i] = 0u;
+    }
+    if (a.row_loss) a.row_loss[row] = loss;
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    stage_rows<T, true>((T*)a.dx + (long)blockIdx.x * 64 * V, V, rows, V, lds, pitch);
+  }
+}
+
+// ---------------------------------------------------------------- sums over the rows
+// out[0] = sum row_loss (mean: / sum weight), wsum_out = sum weight.  One workgroup, f64, a fixed order.
+__global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ row_loss,
+                                                           const float* __restrict__ weight, long T, int mean,
+                                                           float* __restrict__ out, float* __restrict__ wsum_out) {
+  __shared__ double red[2][16];
+  double s = 0.0, w = 0.0;
+#pragma unroll 8
+  for (long i = threadIdx.x; i < T; i += 1024) {
+    if (row_loss) s += (double)row_loss[i];
+    if (weight) w += (double)weight[i];
+  }
+  s = wave_sum_f64(s);
+  w = wave_sum_f64(w);
+  if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = s; red[1][threadIdx.x >> 6] = w; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = w = 0.0;
+    for (int k = 0; k < 16; ++k) { s += red[0][k]; w += red[1][k]; }
+    if (!weight) w = (double)T;
+    if (out) out[0] = (float)(mean ? s / w : s);
+    if (wsum_out) wsum_out[0] = (float)w;
+  }
+}
+
+// ---------------------------------------------------------------- host launchers
+// Segments per row: as for the scores (two workgroups per CU fill the card), and never more tokens than the bits hold.
+int distill_segments(long T, int V) {
+  const long least = (V + DISTILL_SEGMENT - 1) / DISTILL_SEGMENT;
+  if (V <= 8192 || T >= 512) return (int)least;
+  long s = (1024 + T - 1) / T, most = (V + 2047) / 2048;
+  if (s > most) s = most;
+  if (s > LOGITS_MAX_SEGMENTS) s = LOGITS_MAX_SEGMENTS;
+  return (int)(s > least ? s : least);
+}
+static int seg_len_of(int V, int S) { return ((V + S - 1) / S + 31) / 32 * 32; }
+
+template <typename T>
+static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s) {
+  if (a.V <= 64) {
+    const dim3 g((unsigned)((a.T + 63) / 64));
+    if (grad) hipLaunchKernelGGL((distill_small_kernel<T, true>), g, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((distill_small_kernel<T, false>), g, dim3(64), 0, s, a);
+    return;
+  }
+  int S = distill_segments(a.T, a.V);
+  const bool one = S == 1 && loss && grad;
+  if (one) a.tape = a.g_top = nullptr;   // for a backward of its own only
+  if (loss) {
+    if (a.V <= 2048) {
+      if (one) hipLaunchKernelGGL((distill_kernel<T, 64, true>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+      else hipLaunchKernelGGL((distill_kernel<T, 64, false>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+    } else {
+      const int len = S > 1 ? seg_len_of(a.V, S) : a.V;
+      S = (a.V + len - 1) / len;
+      if (one) hipLaunchKernelGGL((distill_kernel<T, 256, true>), dim3((unsigned)a.T), dim3(256), 0, s, a, 1, a.V);
+      else hipLaunchKernelGGL((distill_kernel<T, 256, false>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
+      if (S > 1) hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)a.T), dim3(64), 0, s, a, S);
+    }
+  }
+  if (grad && !one) {
+    if (a.V <= 2048) {
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 64>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+    } else {
+      const int len = logits_bwd_segment(a.T, a.V), sb = (a.V + len - 1) / len;
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)(a.T * sb)), dim3(256), 0, s, a, sb, len);
+    }
+  }
+}
+static void distill_dispatch(const DistillTopkArgs& a, bool loss, bool grad, hipStream_t s) {
+  if (a.type == SCM_F32) distill_typed<float>(a, loss, grad, s);
+  else if (a.type == SCM_BF16) distill_typed<bf16>(a, loss, grad, s);
+  else distill_typed<f16>(a, loss, grad, s);
+}
+hipError_t topk_distill_fwd(const DistillTopkArgs& a, float* out, float* wsum_out, hipStream_t s) {
+  Traced tr(K_TOPK_DISTILL, 0, s);
+  distill_dispatch(a, true, false, s);
+  if (out)
+    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, a.row_loss, a.weight, a.T, a.mean, out, wsum_out);
+  return hipGetLastError();
+}
+hipError_t topk_distill_bwd(const DistillTopkArgs& a, hipStream_t s) {
+  Traced tr(K_TOPK_DISTILL, 0, s);
+  distill_dispatch(a, false, true, s);
+  return hipGetLastError();
+}
+hipError_t topk_distill_step(const DistillTopkArgs& a, float* out, float* wsum, hipStream_t s) {
+  Traced tr(K_TOPK_DISTILL, 0, s);
+  // the gradient of a mean needs the weights' sum first
+  if (a.weight && a.mean)
+    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, (const float*)nullptr, a.weight, a.T, 0,
+                       (float*)nullptr, wsum);
+  distill_dispatch(a, true, true, s);
+  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, a.row_loss, a.weight, a.T, a.mean, out, (float*)nullptr);
+  return hipGetLastError();
+}
+
+}  // namespace scm

@@ -1,5 +1,6 @@
 """What a program reads off a model's logits, and what it trains them towards, for any number of classes: log
-probabilities of given tokens with entropy and top alternatives (token_logprobs).  The RNA model's own masked cross
+probabilities of given tokens with entropy and top alternatives (token_logprobs), and distillation from a teacher's top
+log probabilities (topk_distillation, topk_distillation_grad).  The RNA model's own masked cross
 entropy over its at most eight expression classes is s1.masked_cross_entropy.
 """
 from __future__ import annotations
@@ -62,3 +63,54 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, k, temperature, ignore_index, entropy))
     return TokenLogprobs(*_shaped(logits.shape[:-1], ops.score_fwd(logits, targets, k, temperature, ignore_index, entropy)[:5]))
+
+
+class _TopkDistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_index, top_logprob, temperature, tail, weight, reduction):
+        op = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction)
+        rows, loss, wsum, tape = op.forward(reduction != "none", True)
+        ctx.opts = (temperature, tail, reduction)
+        ctx.save_for_backward(logits, top_index, top_logprob, weight, wsum, tape)
+        return rows.view(logits.shape[:-1]) if loss is None else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gloss):
+        logits, top_index, top_logprob, weight, wsum, tape = ctx.saved_tensors
+        temperature, tail, reduction = ctx.opts
+        op = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction)
+        return op.backward(gloss, wsum, tape).view(logits.shape), None, None, None, None, None, None
+
+
+def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *, temperature: float = 1.0,
+                      tail: bool = True, weight: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
+    """KL divergence from a teacher's top log probabilities to softmax(logits / temperature).
+
+    logits [..., V]: f32, bf16 or fp16 on the GPU, any row stride; top_index int64 [..., k], top_logprob f32 [..., k],
+    1 <= k <= 64: the teacher's entries at the same temperature, as token_logprobs returns them (a negative index is an
+    entry not used; one named twice counts with both probabilities; one outside the vocabulary makes the row NaN).
+    ``tail``: what the entries leave of the teacher's mass is one more class against the student's mass on all other
+    tokens; otherwise the entries are renormalised.  ``weight`` f32 [...]: rows of weight 0 (padding) are not looked at.
+    reduction 'mean' divides by the sum of the weights (nan when that is 0), 'none' returns weight * loss per row.  The
+    loss is f32 and not multiplied by temperature^2.  A row of -inf throughout counts with loss and gradient 0.
+
+    Differentiable once, in the logits only.  The result does not depend on the order in which workgroups run."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TopkDistillFn.apply(logits, top_index, top_logprob, temperature, tail, weight, reduction)
+    op = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction)
+    rows, loss, _, _ = op.forward(reduction != "none", False)
+    return rows.view(logits.shape[:-1]) if loss is None else loss
+
+
+@torch.no_grad()
+def topk_distillation_grad(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *,
+                           temperature: float = 1.0, tail: bool = True, weight: Optional[torch.Tensor] = None,
+                           reduction: str = "mean", scale: float = 1.0):
+    """(loss, scale * d loss / d logits) of topk_distillation ('mean' or 'sum') in one pass over the logits, for a loop
+    that runs the model's backward itself: ``loss, d = topk_distillation_grad(logits, ..., scale=1 / grad_acc)``,
+    ``logits.backward(d)``.  The gradient has the logits' type and shape."""
+    if reduction == "none":
+        raise ValueError("topk_distillation_grad: reduction must be 'mean' or 'sum'")
+    loss, dx = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction).step(float(scale))
+    return loss, dx.view(logits.shape)

@@ -701,6 +701,85 @@ def score_bwd(logits, targets, tape, entropy, top_index, g_logprob, g_entropy, g
     return dx
 
 
+class TopkDistill:
+    """The checked operands of one distillation from top log probabilities; see the C ABI for the definition."""
+
+    def __init__(self, logits, index, logprob, temperature: float, tail: bool, weight, reduction: str):
+        if index.dim() != logits.dim() or index.shape[:-1] != logits.shape[:-1] or index.shape != logprob.shape:
+            raise ValueError(f"teacher entries {tuple(index.shape)} and {tuple(logprob.shape)} for logits {tuple(logits.shape)}")
+        self.k = index.shape[-1]
+        if self.k < 1:
+            raise ValueError("no teacher entries")
+        if reduction not in ("mean", "sum", "none"):
+            raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+        self.x = x = _logits_rows(logits, temperature, self.k)
+        t = self.rows = x.shape[0]
+        for v, dt, nm in ((index, torch.int64, "top_index"), (logprob, F32, "top_logprob")):
+            if v.dtype != dt:
+                raise TypeError(f"{nm}: expected {dt}, got {v.dtype}")
+        if weight is not None:
+            if weight.shape != logits.shape[:-1]:
+                raise ValueError(f"weight: expected {tuple(logits.shape[:-1])}, got {tuple(weight.shape)}")
+            weight = _row_vector(weight, t, F32, "weight")
+        for v in (logprob, weight):
+            if v is not None and v.requires_grad:
+                raise ValueError("the teacher's log probabilities and the weights take no gradient: detach them")
+        self.index, self.logprob, self.weight = index.contiguous(), logprob.contiguous(), weight
+        self.temperature, self.tail, self.mean = temperature, int(bool(tail)), int(reduction == "mean")
+        _on_device(x, index, logprob, weight)
+
+    def _common(self):
+        x = self.x
+        return (_p(x), SCM_TYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], self.temperature, _p(self.index),
+                _p(self.logprob), self.k, self.tail, _p(self.weight), self.mean)
+
+    def _new(self, n):
+        return torch.empty(n, dtype=F32, device=self.x.device) if n else None
+
+    def forward(self, want_sum: bool, want_tape: bool):
+        """-> (row losses f32 [T], loss f32 [] or None, sum of the weights [1] or None, tape or None)"""
+        t, v = self.x.shape
+        with _on_device(self.x):
+            rows = torch.empty(t, dtype=F32, device=self.x.device)
+            if not t:      # an empty sum; its mean is 0 / 0
+                loss = rows.new_full((), float("nan") if self.mean else 0.0) if want_sum else None
+                return rows, loss, None, None
+            loss, wsum = (torch.empty((), dtype=F32, device=self.x.device), self._new(1)) if want_sum else (None, None)
+            tape = self._new(lib.scm_topk_distill_tape_floats(t, v, self.k)) if want_tape else None
+            ws = self._new(lib.scm_topk_distill_ws_floats(t, v))
+            check(lib.scm_topk_distill_fwd(*self._common(), _p(rows), _p(loss), _p(wsum), _p(tape), _p(ws), _stream()),
+                  "scm_topk_distill_fwd")
+        return rows, loss, wsum, tape
+
+    def backward(self, gloss, wsum, tape):
+        """gloss: the incoming gradient, one value or (reduction 'none') one per row -> dlogits [T, V]"""
+        x = self.x
+        gloss = gloss.to(F32).reshape(-1).contiguous()
+        with _on_device(x, gloss, wsum, tape):
+            dx = torch.empty(tuple(x.shape), dtype=x.dtype, device=x.device)
+            if x.shape[0]:
+                check(lib.scm_topk_distill_bwd(*self._common(), _p(wsum), _p(gloss), int(wsum is None), _p(tape), _p(dx),
+                                               _stream()), "scm_topk_distill_bwd")
+        return dx
+
+    def step(self, scale: float):
+        """-> (loss f32 [], dlogits [T, V] = scale * its gradient)"""
+        x = self.x
+        t, v = x.shape
+        with _on_device(x):
+            dx = torch.empty((t, v), dtype=x.dtype, device=x.device)
+            if not t:
+                return self.forward(True, False)[1], dx
+            loss = torch.empty((), dtype=F32, device=x.device)
+            buf = self._new(t + 1)      # the rows' losses, the sum of the weights
+            tape = self._new(lib.scm_topk_distill_tape_floats(t, v, self.k))
+            ws = self._new(lib.scm_topk_distill_ws_floats(t, v))
+            p = buf.data_ptr()
+            check(lib.scm_topk_distill_step(*self._common(), scale, p, _p(loss), p + 4 * t, _p(tape), _p(ws), _p(dx), _stream()),
+                  "scm_topk_distill_step")
+        return loss, dx
+
+
 # ----------------------------------------------------------------------------- cell-embedding tail
 def cell_tail_supported(p: int, hd: int, o: int) -> bool:
     return p <= 1024 and hd <= 1024 and o <= 1024 and p + hd <= 1024 and (p + hd) % 64 == 0

@@ -41,7 +41,7 @@ def _exact(x, target, k, tau, ignore=-100):
     m = torch.where(m == -INF, 0.0, m)
     s = torch.exp(z - m).sum(-1, keepdim=True)
     lse = m + torch.log(s)
-    logp = torch.where(lse == -INF, -INF, z - lse)
+    logp = torch.where(lse == -INF, -INF, (z - m) - torch.log(s))     # z - lse would lose log s next to 3e38
     p = torch.exp(logp)
     ent = -torch.where(p > 0, p * logp, 0.0).sum(-1)
     r = dict(lse=lse[..., 0], logp=logp, p=p, ent=ent)
@@ -66,13 +66,14 @@ def _check(out, x, target, k, tau):
     n = _terms(x.shape[-1])
     span = 4 * U * (x.double() / tau).masked_fill(~torch.isfinite(x), 0.0).abs().amax(-1)
     _close(out.lse, r["lse"], n * U + span, "lse")
+    near = lambda lp: n * U + 8 * U * lp.abs().masked_fill(~torch.isfinite(lp), 0.0)      # x - m and the result rounded
     if target is not None:
-        _close(out.logprob, r["lp"], n * U + 2 * span, "logprob")
+        _close(out.logprob, r["lp"], near(r["lp"]), "logprob")
     if out.entropy is not None:
-        _close(out.entropy, r["ent"], 2 * n * U * (1 + r["ent"].abs()) + span, "entropy")
+        _close(out.entropy, r["ent"], 2 * n * U * (1 + r["ent"].abs()), "entropy")
     if k:
         assert torch.equal(out.top_index, r["idx"])
-        _close(out.top_logprob, r["top"], n * U + 2 * span[..., None], "top")
+        _close(out.top_logprob, r["top"], near(r["top"]), "top")
     return r
 
 

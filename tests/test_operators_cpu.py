@@ -97,3 +97,45 @@ def test_score_workspace_holds_every_split():
                 s = n // (t * (2 * k + 3))
                 assert n == s * t * (2 * k + 3) and s <= 64 and s * k <= 2048 and s != 1
     assert lib.scm_score_ws_floats(1, 100, 65) == 0 and lib.scm_score_ws_floats(0, 100, 1) == 0
+
+
+def test_topk_distillation_needs_device_tensors():
+    from scmomer_amd.logits import topk_distillation, topk_distillation_grad
+    x, idx, lp = torch.randn(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+    for f in (topk_distillation, topk_distillation_grad):
+        with pytest.raises(ValueError):
+            f(x, idx, lp)
+
+
+@pytest.mark.parametrize("entry", ["fwd", "bwd", "step"])
+@pytest.mark.parametrize("change", [dict(x=None), dict(type=7), dict(T=0), dict(V=0), dict(ldx=-2), dict(tau=0.0), dict(k=0),
+                                    dict(k=65), dict(index=None), dict(lp=None), dict(rows=None), dict(dx=None),
+                                    dict(tape=None, V=100), dict(wsum=None), dict(ws=None, V=100000), dict(gloss=None),
+                                    dict(T=(1 << 31) - 1, V=1 << 30)])
+def test_topk_distill_rejects(entry, change):
+    from scmomer_amd._lib import lib
+    only = {"rows": ("fwd", "step"), "dx": ("bwd", "step"), "tape": ("bwd", "step"), "wsum": ("bwd", "step"),
+            "ws": ("fwd", "step"), "gloss": ("bwd",)}
+    if any(entry not in only.get(n, (entry,)) for n in change):
+        pytest.skip("not an argument of this entry point, or allowed there")
+    keep, a = _addr()
+    k = dict(x=a, type=0, ldx=8, T=1, V=8, tau=1.0, index=a, lp=a, k=2, rows=a, dx=a, tape=a, wsum=a, ws=a, gloss=a)
+    k.update(change)
+    head = (k["x"], k["type"], k["ldx"], k["T"], k["V"], k["tau"], k["index"], k["lp"], k["k"], 1, a, 1)
+    if entry == "fwd":
+        rc = lib.scm_topk_distill_fwd(*head, k["rows"], a, k["wsum"], k["tape"], k["ws"], None)
+    elif entry == "bwd":
+        rc = lib.scm_topk_distill_bwd(*head, k["wsum"], k["gloss"], 0, k["tape"], k["dx"], None)
+    else:
+        rc = lib.scm_topk_distill_step(*head, 1.0, k["rows"], a, k["wsum"], k["tape"], k["ws"], k["dx"], None)
+    assert rc < 0 and f"scm_topk_distill_{entry}".encode() in lib.scm_last_error()
+
+
+def test_topk_distill_workspaces():
+    from scmomer_amd._lib import lib
+    assert lib.scm_topk_distill_tape_floats(10, 64, 5) == 0 and lib.scm_topk_distill_tape_floats(10, 65, 5) == 70
+    assert lib.scm_topk_distill_ws_floats(1000, 131072) == 0                 # one workgroup per row
+    assert lib.scm_topk_distill_ws_floats(1000, 131073) == 4000              # more tokens than a workgroup marks
+    for t in (1, 7, 511):
+        n = lib.scm_topk_distill_ws_floats(t, 100000)
+        assert n % (2 * t) == 0 and 2 <= n // (2 * t) <= 64
