@@ -23,8 +23,10 @@ class TokenLogprobs(NamedTuple):
     top_index: Optional[torch.Tensor]     # int64 [..., k]
 
 
-def _shaped(shape, outs):
-    lp, ent, lse, tlp, tix = outs
+def _shaped(logits, lp, ent, lse, tlp, tix):
+    if logits.dim() == 2:
+        return lp, ent, lse, tlp, tix
+    shape = logits.shape[:-1]
     return (lp if lp is None else lp.view(shape), ent if ent is None else ent.view(shape), lse.view(shape),
             tlp if tlp is None else tlp.view(*shape, tlp.shape[1]), tix if tix is None else tix.view(*shape, tix.shape[1]))
 
@@ -32,20 +34,26 @@ def _shaped(shape, outs):
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, k, temperature, ignore_index, entropy):
-        *outs, tape = ops.score_fwd(logits, targets, k, temperature, ignore_index, entropy, tape=True)
+        lp, ent, lse, tlp, tix, tape = ops.score_fwd(logits, targets, k, temperature, ignore_index, entropy, tape=True)
         ctx.set_materialize_grads(False)
         ctx.opts = (temperature, ignore_index)
-        ctx.save_for_backward(logits, targets, tape, outs[1], outs[4])
+        ctx.save_for_backward(logits, targets, ent, tix, tape)
         if k:
-            ctx.mark_non_differentiable(outs[4])
-        return _shaped(logits.shape[:-1], outs)
+            ctx.mark_non_differentiable(tix)
+        return _shaped(logits, lp, ent, lse, tlp, tix)
+
+    @staticmethod
+    def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
+        if torch.is_grad_enabled():
+            return _TokenLogprobsFn._once(ctx, g_logprob, g_entropy, g_lse, g_top, _)
+        logits, targets, entropy, top_index, tape = ctx.saved_tensors
+        dx = ops.score_bwd(logits, targets, tape, entropy, top_index, g_logprob, g_entropy, g_lse, g_top, *ctx.opts)
+        return dx if logits.dim() == 2 else dx.view(logits.shape), None, None, None, None, None
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
-        logits, targets, tape, entropy, top_index = ctx.saved_tensors
-        dx = ops.score_bwd(logits, targets, tape, entropy, top_index, g_logprob, g_entropy, g_lse, g_top, *ctx.opts)
-        return dx.view(logits.shape), None, None, None, None, None
+    def _once(ctx, *grads):      # under create_graph: what comes back refuses to be differentiated again
+        return _TokenLogprobsFn.backward(ctx, *grads)
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, *, k: int = 0, temperature: float = 1.0,
@@ -62,7 +70,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     constant, as for torch.topk)."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, k, temperature, ignore_index, entropy))
-    return TokenLogprobs(*_shaped(logits.shape[:-1], ops.score_fwd(logits, targets, k, temperature, ignore_index, entropy)[:5]))
+    return TokenLogprobs(*_shaped(logits, *ops.score_fwd(logits, targets, k, temperature, ignore_index, entropy)[:5]))
 
 
 class _TopkDistillFn(torch.autograd.Function):
@@ -72,15 +80,21 @@ class _TopkDistillFn(torch.autograd.Function):
         rows, loss, wsum, tape = op.forward(reduction != "none", True)
         ctx.opts = (temperature, tail, reduction)
         ctx.save_for_backward(logits, top_index, top_logprob, weight, wsum, tape)
-        return rows.view(logits.shape[:-1]) if loss is None else loss
+        return loss if loss is not None else rows if logits.dim() == 2 else rows.view(logits.shape[:-1])
+
+    @staticmethod
+    def backward(ctx, gloss):
+        if torch.is_grad_enabled():
+            return _TopkDistillFn._once(ctx, gloss)
+        logits, top_index, top_logprob, weight, wsum, tape = ctx.saved_tensors
+        temperature, tail, reduction = ctx.opts
+        dx = ops.TopkDistill.again(logits, top_index, top_logprob, temperature, tail, weight, reduction).backward(gloss, wsum, tape)
+        return dx if logits.dim() == 2 else dx.view(logits.shape), None, None, None, None, None, None
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, gloss):
-        logits, top_index, top_logprob, weight, wsum, tape = ctx.saved_tensors
-        temperature, tail, reduction = ctx.opts
-        op = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction)
-        return op.backward(gloss, wsum, tape).view(logits.shape), None, None, None, None, None, None
+    def _once(ctx, gloss):      # under create_graph: what comes back refuses to be differentiated again
+        return _TopkDistillFn.backward(ctx, gloss)
 
 
 def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *, temperature: float = 1.0,
@@ -100,10 +114,9 @@ def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob
         return _TopkDistillFn.apply(logits, top_index, top_logprob, temperature, tail, weight, reduction)
     op = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction)
     rows, loss, _, _ = op.forward(reduction != "none", False)
-    return rows.view(logits.shape[:-1]) if loss is None else loss
+    return loss if loss is not None else rows.view(logits.shape[:-1])
 
 
-@torch.no_grad()
 def topk_distillation_grad(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *,
                            temperature: float = 1.0, tail: bool = True, weight: Optional[torch.Tensor] = None,
                            reduction: str = "mean", scale: float = 1.0):
@@ -112,5 +125,5 @@ def topk_distillation_grad(logits: torch.Tensor, top_index: torch.Tensor, top_lo
     ``logits.backward(d)``.  The gradient has the logits' type and shape."""
     if reduction == "none":
         raise ValueError("topk_distillation_grad: reduction must be 'mean' or 'sum'")
-    loss, dx = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction).step(float(scale))
-    return loss, dx.view(logits.shape)
+    loss, dx = ops.TopkDistill(logits.detach(), top_index, top_logprob, temperature, tail, weight, reduction).step(scale)
+    return loss, dx if logits.dim() == 2 else dx.view(logits.shape)

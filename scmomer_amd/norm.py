@@ -15,16 +15,23 @@ from . import ops
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):
-        y, mean, rstd = ops.norm_fwd(x, weight, bias, eps, out_dtype)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        return y.view(x.shape)
+        y, stats = ops.norm_fwd(x, weight, bias, eps, out_dtype)
+        ctx.save_for_backward(x, weight, stats)
+        return y if x.dim() == 2 else y.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            return _LayerNormFn._once(ctx, dy)
+        x, weight, stats = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        dx, dw, db = ops.norm_bwd(dy, x, stats, weight, want[0], want[1], want[2])
+        return dx if dx is None or x.dim() == 2 else dx.view(x.shape), dw, db, None, None
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = ops.norm_bwd(dy, x, mean, rstd, weight, *ctx.needs_input_grad[:3])
-        return dx.view(x.shape) if dx is not None else None, dw, db, None, None
+    def _once(ctx, dy):      # under create_graph: what comes back refuses to be differentiated again
+        return _LayerNormFn.backward(ctx, dy)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
