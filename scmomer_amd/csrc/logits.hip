@@ -34,8 +34,9 @@ SCM_DEV uint64_t shfl64(uint64_t v, int mask) {
 
 // ---------------------------------------------------------------- score: the k largest elements of a segment
 // A lower bound of the k-th largest element comes free with the statistics: the k-th largest of the threads' maxima
-// (each thread's maximum is an element of its own).  Only threads whose maximum reaches it look at their elements
-// again; what reaches it (about k of them) goes to LDS and is ranked there by counting.
+// (each thread's maximum is an element of its own).  Only the elements of threads whose maximum reaches it (k or a few
+// more) are looked at again, by the 64 lanes of the thread's wave together; what reaches the bound goes to LDS and is
+// ranked there by counting.
 template <int NT>
 struct TopLds {
   static constexpr int CAP = NT == 64 ? 512 : 1024;
@@ -47,11 +48,14 @@ struct TopLds {
   int thr_at;
   uint64_t red[NT / 64];
 };
-
+// Low bits of ordered() that carry nothing: the same for all values of one sign of a 16-bit type.
+template <typename T> constexpr int order_spare = 0;
+template <> constexpr int order_spare<bf16> = 16;
+template <> constexpr int order_spare<f16> = 13;
 // Threshold (value, chunk) over the NT maxima, by the first wave: the k-th largest value, and among equal values the
 // chunk up to which the k-th place reaches.  Threads without elements hold value 0.
 template <int NT>
-SCM_DEV void top_threshold(TopLds<NT>& L, int k) {
+SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
   constexpr int R = NT / 64;
   const int l = threadIdx.x & 63;
   uint32_t b[R];
@@ -59,26 +63,31 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k) {
 #pragma unroll
   for (int r = 0; r < R; ++r) { b[r] = L.best[r * 64 + l]; at[r] = L.at[r * 64 + l]; }
   uint32_t t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  int reach = 64 * R, above = 0;   // how many maxima are >= t, and > t
+  for (int bit = 31; bit >= spare; --bit) {
     const uint32_t cand = t | (1u << bit);
     int n = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] >= cand));
-    if (n >= k) t = cand;
+    if (n >= k) { t = cand; reach = n; } else { above = n; }
   }
-  // t == 0: fewer than k threads have elements; everything is a candidate
-  int need = k;
+  // t is the k-th largest value with its spare low bits 0 (0: fewer than k threads hold elements, every element is a
+  // candidate); maxima from t to t + 2^spare - 1 are the equal ones.  The last bits that were refused count those above.
+  const uint32_t top = t | ((1u << spare) - 1u);
+  int lim = 0x7FFFFFFF;
+  if (t && reach > k) {
+    // more equal maxima than places: the smallest bound with enough of them at chunks <= lim
+    const int need = k - above;
+    lim = 0;
+    for (int bit = 31 - __builtin_clz(chunks | 1); bit >= 0; --bit) {
+      const int cand = lim | (1 << bit);
+      int n = 0;
 #pragma unroll
-  for (int r = 0; r < R; ++r) need -= __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] > t));
-  int lim = 0;   // smallest bound with at least `need` equal maxima at chunks <= lim; all bits set: no bound
-  for (int bit = 30; bit >= 0; --bit) {
-    const int cand = lim | (1 << bit);
-    int n = 0;
-#pragma unroll
-    for (int r = 0; r < R; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] == t && at[r] < cand));
-    if (n < need) lim = cand;
+      for (int r = 0; r < R; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] >= t && b[r] <= top && at[r] < cand));
+      if (n < need) lim = cand;
+    }
   }
-  if (l == 0) { L.thr = t; L.thr_at = t ? lim : 0x7FFFFFFF; }
+  if (l == 0) { L.thr = t; L.thr_at = lim; }
 }
 
 // Calls emit(rank, key) for the k largest keys of the segment, each from one thread.  best, at: the thread's maximum
@@ -86,29 +95,31 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k) {
 // threads' maxima are not to be used).
 template <typename T, int NT, typename Emit>
 SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, int at, bool odd, TopLds<NT>& L, Emit emit) {
-  constexpr int E = Walk<T, NT>::E, U = Walk<T, NT>::U;
-  const int tid = threadIdx.x;
+  constexpr int E = Walk<T, NT>::E, U = Walk<T, NT>::U, SPARE = order_spare<T>;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int chunks = (w.len + E - 1) / E;
   L.best[tid] = best;
   L.at[tid] = at;
   if (tid == 0) L.count = 0;
   __syncthreads();
-  if (tid < 64) top_threshold<NT>(L, k);
+  if (tid < 64) top_threshold<NT>(L, k, chunks, SPARE);
   __syncthreads();
-  const uint32_t thr = L.thr;
+  const uint32_t thr = L.thr, thr_top = thr | ((1u << SPARE) - 1u);
   const int thr_at = L.thr_at;
-  if (!odd && best && (best > thr || (best == thr && at <= thr_at))) {
-    for (int s = 0; s < w.steps(); ++s) {
-      Chunk<T, E> raw[U];
-      w.load(s, raw);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c0 = w.first(s, u), chunk = c0 / E;
+  if (!odd) {
+    auto in = [&](uint32_t o, int chunk) { return o > thr_top || (o >= thr && chunk <= thr_at); };
+    unsigned long long todo = __builtin_amdgcn_ballot_w64(best && in(best, at));
+    while (todo) {   // the chunks of one thread of this wave: tid - lane + src, + NT, ...
+      const int src = tid - lane + __builtin_ctzll(todo);
+      todo &= todo - 1;
+      for (int c = src + NT * lane; c < chunks; c += NT * 64) {
+        const Chunk<T, E> raw = load_chunk<T, E>(w.p + (long)c * E, w.len - c * E);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const uint32_t o = ordered((float)raw[u].e[j]);
-          if (c0 + j < w.len && (o > thr || (o == thr && chunk <= thr_at))) {
+          const uint32_t o = ordered((float)raw.e[j]);
+          if (in(o, c) && c * E + j < w.len) {
             const int pos = atomicAdd(&L.count, 1);
-            if (pos < TopLds<NT>::CAP) L.cand[pos] = key_of(o, lo + c0 + j);
+            if (pos < TopLds<NT>::CAP) L.cand[pos] = key_of(o, lo + c * E + j);
           }
         }
       }
@@ -132,7 +143,7 @@ SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, 
   for (int r = 0; r < found; ++r) {
     uint64_t mine = 0;
     for (int s = 0; s < w.steps(); ++s) {
-      Chunk<T, E> raw[U];
+      typename Walk<T, NT>::Raw raw;
       w.load(s, raw);
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -189,25 +200,22 @@ __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_l
   Stat st = stat_none();
   float best = -INFINITY;
   int at = threadIdx.x;
-  for (int s = 0; s < w.steps(); ++s) {
-    Chunk<T, W::E> raw[W::U];
-    w.load(s, raw);
+  w.run([&](int s, const typename W::Raw& raw) {
     float v[32], bm = LOWEST;
+    w.values(s, raw, v);
 #pragma unroll
     for (int u = 0; u < W::U; ++u) {
-      const int n = w.len - w.first(s, u);
-      float cm = -INFINITY;
+      float cm = v[u * W::E];
 #pragma unroll
-      for (int j = 0; j < W::E; ++j) {
-        const float x = j < n ? (float)raw[u].e[j] : -INFINITY;
-        v[u * W::E + j] = x;
-        cm = fmaxf(cm, x);
-      }
+      for (int j = 1; j < W::E; ++j) cm = fmaxf(cm, v[u * W::E + j]);
       bm = fmaxf(bm, cm);
-      if (TOP && cm > best) { best = cm; at = w.first(s, u) / W::E; }
+      if constexpr (TOP) {
+        at = cm > best ? (s * W::U + u) * NT + (int)threadIdx.x : at;
+        best = fmaxf(best, cm);
+      }
     }
     stat_add<ENT>(st, v, bm, a.c);
-  }
+  });
   st = stat_block<ENT, NT>(st, a.c, red);
   const bool odd = !(st.s <= 3e38f);   // NaN
   if (S > 1) {
@@ -363,9 +371,7 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, i
   const float gt = wave_sum((tid & 63) < k ? a.g_top[row * k + (tid & 63)] : 0.f);
   const ScoreGrad r = score_grad(a, row, gt);
   if (tid == 0) target_named = 0;
-  for (int s = 0; s < w.steps(); ++s) {
-    Chunk<T, W::E> raw[W::U];
-    w.load(s, raw);
+  w.run([&](int s, const typename W::Raw& raw) {
 #pragma unroll
     for (int u = 0; u < W::U; ++u) {
       float o[W::E];
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, i
       for (int j = 0; j < W::E; ++j) o[j] = score_dx(r, (float)raw[u].e[j], a.c);
       store_chunk<T, W::E>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
     }
-  }
+  });
   // the named elements again, after the barrier: the last store to an address is theirs
   __syncthreads();
   const bool row_empty = a.tape[2 * row + 1] == 0.f;

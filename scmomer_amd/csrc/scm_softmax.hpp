@@ -49,17 +49,53 @@ SCM_DEV Stat stat_block(Stat v, float c, Stat* red) {
   return r;
 }
 
-// Per-thread view of a segment [lo, lo + len) of a row: chunk i of the thread is chunk tid + NT * i of the segment.
+// Per-thread view of a segment [lo, lo + len) of a row, in steps of 32 elements (U chunks) a thread: chunk u of step s is
+// chunk (s U + u) NT + tid of the segment.
 template <typename T, int NT>
 struct Walk {
-  static constexpr int E = 16 / sizeof(T), U = 32 / E;   // U chunks = 32 elements a thread and step
+  static constexpr int E = 16 / sizeof(T), U = 32 / E, STEP = NT * U * E;
+  typedef Chunk<T, E> Raw[U];
   const T* p;
   int len;
-  SCM_DEV int steps() const { return (len + NT * U * E - 1) / (NT * U * E); }
+  SCM_DEV int steps() const { return (len + STEP - 1) / STEP; }
   SCM_DEV int first(int step, int u) const { return ((step * U + u) * NT + (int)threadIdx.x) * E; }
-  SCM_DEV void load(int step, Chunk<T, E> (&raw)[U]) const {
+  SCM_DEV void load(int step, Raw& raw) const {
+    if ((step + 1) * STEP <= len) {   // the same for all threads
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = load_chunk<T, E>(p + first(step, u), len - first(step, u));
+      for (int u = 0; u < U; ++u) __builtin_memcpy(&raw[u], p + first(step, u), sizeof(raw[u]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = load_chunk<T, E>(p + first(step, u), len - first(step, u));
+    }
+  }
+  // f(step, raw) for every step; the next step's loads are on their way meanwhile
+  template <typename F>
+  SCM_DEV void run(F f) const {
+    const int n = steps();
+    Raw a, b;
+    load(0, a);
+    for (int s = 0; s < n; s += 2) {
+      if (s + 1 < n) load(s + 1, b);
+      f(s, a);
+      if (s + 1 < n) {
+        if (s + 2 < n) load(s + 2, a);
+        f(s + 1, b);
+      }
+    }
+  }
+  // the elements of a step as f32, -inf past the end
+  SCM_DEV void values(int step, const Raw& raw, float (&v)[32]) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[u * E + j] = (float)raw[u].e[j];
+    if ((step + 1) * STEP > len) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (first(step, u) + j >= len) v[u * E + j] = -INFINITY;
+    }
   }
 };
 

@@ -101,23 +101,24 @@ template <typename T, int NT>
 SCM_DEV Stat rest_of_segment(const Walk<T, NT>& w, const NamedBits<NT>& bits, float c) {
   typedef Walk<T, NT> W;
   Stat st = stat_none();
-  for (int s = 0; s < w.steps(); ++s) {
-    Chunk<T, W::E> raw[W::U];
-    w.load(s, raw);
+  w.run([&](int s, const typename W::Raw& raw) {
     float v[32], bm = LOWEST;
+    w.values(s, raw, v);
 #pragma unroll
     for (int u = 0; u < W::U; ++u) {
-      const int i0 = w.first(s, u), n = w.len - i0;
-      const uint32_t named = n > 0 ? bits.w[i0 >> 5] >> (i0 & 31) : 0u;   // this chunk's bits, lowest first
+      const int i0 = w.first(s, u);
+      const uint32_t word = i0 < w.len ? bits.w[i0 >> 5] >> (i0 & 31) : 0u;   // this chunk's bits, lowest first
+      const uint32_t named = word & ((1u << W::E) - 1u);
+      if (named) {   // at most k chunks of a row
 #pragma unroll
-      for (int j = 0; j < W::E; ++j) {
-        const float x = (j < n && !((named >> j) & 1)) ? (float)raw[u].e[j] : -INFINITY;
-        v[u * W::E + j] = x;
-        bm = fmaxf(bm, x);
+        for (int j = 0; j < W::E; ++j)
+          if ((named >> j) & 1) v[u * W::E + j] = -INFINITY;
       }
     }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) bm = fmaxf(bm, v[j]);
     stat_add<false>(st, v, bm, c);
-  }
+  });
   return st;
 }
 
@@ -125,9 +126,7 @@ SCM_DEV Stat rest_of_segment(const Walk<T, NT>& w, const NamedBits<NT>& bits, fl
 template <typename T, int NT>
 SCM_DEV void distill_write(const Walk<T, NT>& w, T* dx, int lo, float m, float cr, float c) {
   typedef Walk<T, NT> W;
-  for (int s = 0; s < w.steps(); ++s) {
-    Chunk<T, W::E> raw[W::U];
-    w.load(s, raw);
+  w.run([&](int s, const typename W::Raw& raw) {
 #pragma unroll
     for (int u = 0; u < W::U; ++u) {
       float o[W::E];
@@ -135,7 +134,7 @@ SCM_DEV void distill_write(const Walk<T, NT>& w, T* dx, int lo, float m, float c
       for (int j = 0; j < W::E; ++j) o[j] = cr * exp2_fast(((float)raw[u].e[j] - m) * c);
       store_chunk<T, W::E>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
     }
-  }
+  });
 }
 template <typename T, int NT>
 SCM_DEV void zero_write(T* dx, int len) {
