@@ -10,59 +10,80 @@
 
 namespace scm {
 
-// Threads of a workgroup and rows it holds at once, for L lanes per row.
-constexpr int norm_threads(int L) { return L < 256 ? 256 : L; }
+// Threads of a workgroup for L lanes per row: L <= 64 several rows at once, else one.
+constexpr int norm_threads(int L) { return L <= 64 ? 256 : L; }
 
-template <typename TX, typename TY, int L, int EPT>
+// What a group of L lanes holds of a row: CPT chunks of E elements a lane, lane-interleaved.
+template <typename T, int E, int L, int CPT>
+struct RowSlice {
+  Chunk<T, E> c[CPT];
+  SCM_DEV void load(const T* row, const int (&col)[CPT], int D, bool there) {
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) c[i] = load_chunk<T, E>(row + col[i], there ? D - col[i] : 0);
+  }
+};
+
+// A group's next row is on its way while one is worked on.
+template <typename TX, typename TY, int L, int EPT, bool STREAM>
 __global__ __launch_bounds__(norm_threads(L)) void norm_fwd_kernel(const TX* __restrict__ x, long ldx,
                                                                    const float* __restrict__ gamma,
                                                                    const float* __restrict__ beta, long T, int D,
                                                                    float eps, TY* __restrict__ y,
                                                                    float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int E = 16 / sizeof(TX), CPT = EPT / E, RPB = norm_threads(L) / L, NW = L / 64;
+  // gamma, beta in registers; longer slices of 2-byte types read them (from the caches) row by row
+  constexpr bool HOLD = EPT <= 8 || sizeof(TX) == 4;
   __shared__ f32x2 part[2][NW > 1 ? NW : 1];
   __shared__ float part_n[NW > 1 ? NW : 1];
   const int lane = threadIdx.x % L, grp = threadIdx.x / L;
-  int col[CPT], n[CPT];
-  float g[CPT][E], b[CPT][E], cnt = 0.f;
+  const long stride = (long)gridDim.x * RPB;
+  long row = (long)blockIdx.x * RPB + grp;
+  int col[CPT];
+  float cnt = 0.f;
 #pragma unroll
   for (int c = 0; c < CPT; ++c) {
     col[c] = (c * L + lane) * E;
-    n[c] = D - col[c];
-    cnt += (float)max(0, min(n[c], E));
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      g[c][j] = (gamma && j < n[c]) ? gamma[col[c] + j] : 1.f;
-      b[c][j] = (beta && j < n[c]) ? beta[col[c] + j] : 0.f;
-    }
+    cnt += (float)max(0, min(D - col[c], E));
   }
-  float wave_n = 0.f;   // columns of this wave (L > 64)
+  RowSlice<TX, E, L, CPT> cur, nxt;
+  cur.load(x + row * ldx, col, D, row < T);
+  Chunk<float, E> g[CPT], b[CPT];
+  auto affine = [&](int c) {
+    if (gamma) g[c] = load_chunk<float, E>(gamma + col[c], D - col[c]);
+    if (beta) b[c] = load_chunk<float, E>(beta + col[c], D - col[c]);
+  };
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) { g[c].e[j] = 1.f; b[c].e[j] = 0.f; }
+    if constexpr (HOLD) affine(c);
+  }
+  float wave_n = 1.f;   // columns of this wave (L > 64)
   if constexpr (L > 64) {
     wave_n = wave_sum(cnt);
     if ((threadIdx.x & 63) == 0) part_n[threadIdx.x >> 6] = wave_n;
     wave_n = fmaxf(wave_n, 1.f);
   }
   const float inv_d = 1.f / (float)D;
-  const long stride = (long)gridDim.x * RPB;
-  long row = (long)blockIdx.x * RPB + grp;
-  Chunk<TX, E> cur[CPT], nxt[CPT];
-#pragma unroll
-  for (int c = 0; c < CPT; ++c) cur[c] = load_chunk<TX, E>(x + row * ldx + col[c], row < T ? n[c] : 0);
   for (int par = 0; row < T; row += stride, par ^= 1) {
-    const bool more = row + stride < T;
-#pragma unroll
-    for (int c = 0; c < CPT; ++c) nxt[c] = load_chunk<TX, E>(x + (row + stride) * ldx + col[c], more ? n[c] : 0);
-    float v[CPT][E], s = 0.f, q = 0.f;
+    nxt.load(x + (row + stride) * ldx, col, D, row + stride < T);
+    float s = 0.f, q = 0.f;
 #pragma unroll
     for (int c = 0; c < CPT; ++c)
 #pragma unroll
-      for (int j = 0; j < E; ++j) { v[c][j] = (float)cur[c].e[j]; s += v[c][j]; }
+      for (int j = 0; j < E; ++j) s += (float)cur.c[c].e[j];
     // the mean over this row (L <= 64) or over this wave's columns (L > 64), then the squares around it
     const float mu0 = L > 64 ? wave_sum(s) / wave_n : lanes_sum<L>(s) * inv_d;
 #pragma unroll
-    for (int c = 0; c < CPT; ++c)
+    for (int c = 0; c < CPT; ++c) {
+      if (D - col[c] >= E) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) { const float d = j < n[c] ? v[c][j] - mu0 : 0.f; q += d * d; }
+        for (int j = 0; j < E; ++j) { const float d = (float)cur.c[c].e[j] - mu0; q += d * d; }
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) { const float d = col[c] + j < D ? (float)cur.c[c].e[j] - mu0 : 0.f; q += d * d; }
+      }
+    }
     float mu = mu0, m2;
     if constexpr (L > 64) {
       // the waves' (mean, sum of squares) join exactly: m2 = sum_w m2_w + n_w (mu_w - mu)^2
@@ -82,18 +103,20 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_fwd_kernel(const TX* __r
     const float rs = 1.f / sqrtf(m2 * inv_d + eps);
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
+      if constexpr (!HOLD) affine(c);
       float o[E];
 #pragma unroll
-      for (int j = 0; j < E; ++j) o[j] = (v[c][j] - mu) * rs * g[c][j] + b[c][j];
-      store_chunk<TY, E>(y + row * D + col[c], o, n[c]);
-      cur[c] = nxt[c];
+      for (int j = 0; j < E; ++j) o[j] = ((float)cur.c[c].e[j] - mu) * rs * g[c].e[j] + b[c].e[j];
+      store_chunk<TY, E, STREAM>(y + row * D + col[c], o, D - col[c]);
     }
+    cur = nxt;
     if (mean && lane == 0) { mean[row] = mu; rstd[row] = rs; }
   }
 }
 
-// partial (may be null) [gridDim.x][2][D]: this workgroup's sums of dy xh and of dy.  dx may be null.
-template <typename TX, typename TY, int L, int EPT>
+// partial (may be null) [gridDim.x][2][D]: this workgroup's sums of dy xh and of dy.  dx may be null.  AHEAD: rows of a
+// group that are on their way while one is worked on.
+template <typename TX, typename TY, int L, int EPT, int AHEAD, bool STREAM>
 __global__ __launch_bounds__(norm_threads(L)) void norm_bwd_kernel(const TY* __restrict__ dy, long lddy,
                                                                    const TX* __restrict__ x, long ldx,
                                                                    const float* __restrict__ mean,
@@ -101,50 +124,50 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_bwd_kernel(const TY* __r
                                                                    const float* __restrict__ gamma, long T, int D,
                                                                    TX* __restrict__ dx, float* __restrict__ partial) {
   constexpr int E = 16 / sizeof(TX), CPT = EPT / E, RPB = norm_threads(L) / L, NW = L / 64;
+  constexpr bool HOLD = EPT <= 8;
   __shared__ f32x2 part[2][NW > 1 ? NW : 1];
   __shared__ float red[RPB > 1 ? RPB : 1][2][RPB > 1 ? L * EPT : 1];
   const int lane = threadIdx.x % L, grp = threadIdx.x / L;
-  int col[CPT], n[CPT];
-  float g[CPT][E], ag[CPT][E], ab[CPT][E];
-#pragma unroll
-  for (int c = 0; c < CPT; ++c) {
-    col[c] = (c * L + lane) * E;
-    n[c] = D - col[c];
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      g[c][j] = (gamma && j < n[c]) ? gamma[col[c] + j] : 1.f;
-      ag[c][j] = ab[c][j] = 0.f;
-    }
-  }
-  const float inv_d = 1.f / (float)D;
   const long stride = (long)gridDim.x * RPB;
   long row = (long)blockIdx.x * RPB + grp;
-  Chunk<TX, E> cx[CPT], nx[CPT];
-  Chunk<TY, E> cy[CPT], ny[CPT];
+  int col[CPT];
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) col[c] = (c * L + lane) * E;
+  struct Rows { RowSlice<TX, E, L, CPT> x; RowSlice<TY, E, L, CPT> y; float mu, rs; } buf[AHEAD + 1];
+  auto fetch = [&](Rows& r, long at) {
+    const bool there = at < T;
+    r.x.load(x + at * ldx, col, D, there);
+    r.y.load(dy + at * lddy, col, D, there);
+    r.mu = there ? mean[at] : 0.f;
+    r.rs = there ? rstd[at] : 0.f;
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) fetch(buf[k], row + k * stride);
+  Chunk<float, E> g[CPT];
+  float ag[CPT][E], ab[CPT][E];
 #pragma unroll
   for (int c = 0; c < CPT; ++c) {
-    cx[c] = load_chunk<TX, E>(x + row * ldx + col[c], row < T ? n[c] : 0);
-    cy[c] = load_chunk<TY, E>(dy + row * lddy + col[c], row < T ? n[c] : 0);
-  }
-  for (int par = 0; row < T; row += stride, par ^= 1) {
-    const bool more = row + stride < T;
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) {
-      nx[c] = load_chunk<TX, E>(x + (row + stride) * ldx + col[c], more ? n[c] : 0);
-      ny[c] = load_chunk<TY, E>(dy + (row + stride) * lddy + col[c], more ? n[c] : 0);
-    }
-    const float mu = mean[row], rs = rstd[row];
+    for (int j = 0; j < E; ++j) { g[c].e[j] = 1.f; ag[c][j] = ab[c][j] = 0.f; }
+    if (HOLD && gamma) g[c] = load_chunk<float, E>(gamma + col[c], D - col[c]);
+  }
+  const float inv_d = 1.f / (float)D;
+  for (int par = 0; row < T; row += stride, par ^= 1) {
+    fetch(buf[AHEAD], row + AHEAD * stride);
+    const float mu = buf[0].mu, rs = buf[0].rs;
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int c = 0; c < CPT; ++c)
+    for (int c = 0; c < CPT; ++c) {
+      if (!HOLD && gamma) g[c] = load_chunk<float, E>(gamma + col[c], D - col[c]);
 #pragma unroll
       for (int j = 0; j < E; ++j) {   // a column past D has dy = 0 and adds nothing anywhere
-        const float d = (float)cy[c].e[j], xh = ((float)cx[c].e[j] - mu) * rs, gd = d * g[c][j];
+        const float d = (float)buf[0].y.c[c].e[j], xh = ((float)buf[0].x.c[c].e[j] - mu) * rs, gd = d * g[c].e[j];
         s1 += gd;
         s2 += gd * xh;
         ag[c][j] += d * xh;
         ab[c][j] += d;
       }
+    }
     if constexpr (L > 64) {
       s1 = wave_sum(s1);
       s2 = wave_sum(s2);
@@ -159,20 +182,20 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_bwd_kernel(const TY* __r
     }
     s1 *= inv_d;
     s2 *= inv_d;
+    if (dx) {
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) {
-      if (dx) {
+      for (int c = 0; c < CPT; ++c) {
         float o[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const float xh = ((float)cx[c].e[j] - mu) * rs;
-          o[j] = rs * ((float)cy[c].e[j] * g[c][j] - s1 - xh * s2);
+          const float xh = ((float)buf[0].x.c[c].e[j] - mu) * rs;
+          o[j] = rs * ((float)buf[0].y.c[c].e[j] * g[c].e[j] - s1 - xh * s2);
         }
-        store_chunk<TX, E>(dx + row * D + col[c], o, n[c]);
+        store_chunk<TX, E, STREAM>(dx + row * D + col[c], o, D - col[c]);
       }
-      cx[c] = nx[c];
-      cy[c] = ny[c];
     }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) buf[k] = buf[k + 1];
   }
   if (!partial) return;
   float* out = partial + (long)blockIdx.x * 2 * D;
@@ -192,8 +215,8 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_bwd_kernel(const TY* __r
   } else {
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
-      store_chunk<float, E>(out + col[c], ag[c], n[c]);
-      store_chunk<float, E>(out + D + col[c], ab[c], n[c]);
+      store_chunk<float, E>(out + col[c], ag[c], D - col[c]);
+      store_chunk<float, E>(out + D + col[c], ab[c], D - col[c]);
     }
   }
 }
@@ -222,53 +245,64 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
 }
 
 // ---------------------------------------------------------------- host launchers
-// Lanes per row and elements per lane: the fewest lanes that hold a row at 16 elements each, and 8 where half the
-// registers do (more rows in flight).
+// Lanes per row and elements per lane: 8 elements each as long as 1024 threads hold the row.  (16 elements on half the
+// lanes: 8192 x 4096 bf16 forward 59 us, against 50 us; the registers of a longer slice cost waves.)
 struct NormShape { int L, ept; };
 static NormShape norm_shape(int D) {
   if (D <= 128) return {16, 8};
-  if (D <= 256) return {16, 16};
+  if (D <= 256) return {32, 8};
   if (D <= 512) return {64, 8};
-  if (D <= 1024) return {64, 16};
+  if (D <= 1024) return {128, 8};
   if (D <= 2048) return {256, 8};
-  if (D <= 4096) return {256, 16};
-  if (D <= 8192) return {512, 16};
+  if (D <= 4096) return {512, 8};
+  if (D <= 8192) return {1024, 8};
   return {1024, 16};
 }
-static int norm_rows_per_block(int D) { const int L = norm_shape(D).L; return norm_threads(L) / L; }
-// workgroups of the backward pass: every one leaves 2 D partial sums behind, so no more than fill the card
-int norm_bwd_blocks(long T, int D) {
-  const int rpb = norm_rows_per_block(D);
-  const long b = (T + rpb - 1) / rpb;
-  return (int)(b < 512 ? b : 512);
+// Workgroups: 1024 threads per CU in either direction, each group going on from row to row with its loads ahead.  More
+// start-up (gamma, beta, first rows) than they hide: forward 8192 x 4096 bf16 with 2048 threads per CU 50 us, 1024: 46 us;
+// fewer of them in the backward pass leave less partial sums but hide less: 512: 74 us, 1024: 58 us.
+static long norm_blocks(long T, int D) {
+  const int nt = norm_threads(norm_shape(D).L), rpb = nt / norm_shape(D).L;
+  const long b = (T + rpb - 1) / rpb, cap = 256L * (1024 / nt);
+  return b < cap ? b : cap;
 }
+int norm_bwd_blocks(long T, int D) { return (int)norm_blocks(T, D); }
 
-template <typename TX, typename TY, int L, int EPT>
-static void launch_fwd(const NormArgs& a, hipStream_t s) {
-  constexpr int RPB = norm_threads(L) / L;
-  const long want = (a.T + RPB - 1) / RPB, cap = 256 * (2048 / norm_threads(L));
-  hipLaunchKernelGGL((norm_fwd_kernel<TX, TY, L, EPT>), dim3((unsigned)(want < cap ? want : cap)), dim3(norm_threads(L)),
-                     0, s, (const TX*)a.x, a.ldx, a.gamma, a.beta, a.T, a.D, a.eps, (TY*)a.y, a.mean, a.rstd);
+template <typename TX, typename TY, int L, int EPT, bool STREAM>
+static void launch_shape(bool fwd, const NormArgs& a, hipStream_t s) {
+  constexpr int AHEAD_B = EPT <= 8 ? 1 : 0;   // 16 elements: two sums per column and two rows are all the registers there are
+  const dim3 g((unsigned)norm_blocks(a.T, a.D)), b(norm_threads(L));
+  if (fwd)
+    hipLaunchKernelGGL((norm_fwd_kernel<TX, TY, L, EPT, STREAM>), g, b, 0, s, (const TX*)a.x, a.ldx, a.gamma, a.beta, a.T,
+                       a.D, a.eps, (TY*)a.y, a.mean, a.rstd);
+  else
+    hipLaunchKernelGGL((norm_bwd_kernel<TX, TY, L, EPT, AHEAD_B, STREAM>), g, b, 0, s, (const TY*)a.dy, a.lddy,
+                       (const TX*)a.x, a.ldx, a.mean, a.rstd, a.gamma, a.T, a.D, (TX*)a.dx, a.ws);
 }
-template <typename TX, typename TY, int L, int EPT>
-static void launch_bwd(const NormArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((norm_bwd_kernel<TX, TY, L, EPT>), dim3(norm_bwd_blocks(a.T, a.D)), dim3(norm_threads(L)), 0, s,
-                     (const TY*)a.dy, a.lddy, (const TX*)a.x, a.ldx, a.mean, a.rstd, a.gamma, a.T, a.D, (TX*)a.dx, a.ws);
+template <typename TX, typename TY, bool STREAM>
+static void launch_typed(bool fwd, const NormArgs& a, hipStream_t s) {
+  switch (norm_shape(a.D).L) {
+    case 16: return launch_shape<TX, TY, 16, 8, STREAM>(fwd, a, s);
+    case 32: return launch_shape<TX, TY, 32, 8, STREAM>(fwd, a, s);
+    case 64: return launch_shape<TX, TY, 64, 8, STREAM>(fwd, a, s);
+    case 128: return launch_shape<TX, TY, 128, 8, STREAM>(fwd, a, s);
+    case 256: return launch_shape<TX, TY, 256, 8, STREAM>(fwd, a, s);
+    case 512: return launch_shape<TX, TY, 512, 8, STREAM>(fwd, a, s);
+    default:
+      if (norm_shape(a.D).ept == 8) return launch_shape<TX, TY, 1024, 8, STREAM>(fwd, a, s);
+      return launch_shape<TX, TY, 1024, 16, STREAM>(fwd, a, s);
+  }
 }
 template <typename TX, typename TY>
-static void launch_shape(bool fwd, const NormArgs& a, hipStream_t s) {
-  const NormShape k = norm_shape(a.D);
-#define SCM_NORM_CASE(L_, E_) \
-  if (k.L == L_ && k.ept == E_) { if (fwd) launch_fwd<TX, TY, L_, E_>(a, s); else launch_bwd<TX, TY, L_, E_>(a, s); return; }
-  SCM_NORM_CASE(16, 8) SCM_NORM_CASE(16, 16) SCM_NORM_CASE(64, 8) SCM_NORM_CASE(64, 16)
-  SCM_NORM_CASE(256, 8) SCM_NORM_CASE(256, 16) SCM_NORM_CASE(512, 16) SCM_NORM_CASE(1024, 16)
-#undef SCM_NORM_CASE
+static void launch_sized(bool fwd, const NormArgs& a, hipStream_t s) {
+  if (a.T * a.D * (long)(fwd ? sizeof(TY) : sizeof(TX)) > STREAM_BYTES) launch_typed<TX, TY, true>(fwd, a, s);
+  else launch_typed<TX, TY, false>(fwd, a, s);
 }
 static void norm_launch(bool fwd, const NormArgs& a, hipStream_t s) {
-  if (a.x_type == SCM_F32 && a.y_type == SCM_F32) launch_shape<float, float>(fwd, a, s);
-  else if (a.x_type == SCM_F32) launch_shape<float, bf16>(fwd, a, s);
-  else if (a.x_type == SCM_BF16) launch_shape<bf16, bf16>(fwd, a, s);
-  else launch_shape<f16, f16>(fwd, a, s);
+  if (a.x_type == SCM_F32 && a.y_type == SCM_F32) launch_sized<float, float>(fwd, a, s);
+  else if (a.x_type == SCM_F32) launch_sized<float, bf16>(fwd, a, s);
+  else if (a.x_type == SCM_BF16) launch_sized<bf16, bf16>(fwd, a, s);
+  else launch_sized<f16, f16>(fwd, a, s);
 }
 bool norm_types_ok(int x_type, int y_type) {
   return (x_type == SCM_F32 && (y_type == SCM_F32 || y_type == SCM_BF16)) ||

@@ -35,15 +35,14 @@ SCM_DEV uint64_t shfl64(uint64_t v, int mask) {
 // ---------------------------------------------------------------- score: the k largest elements of a segment
 // A lower bound of the k-th largest element comes free with the statistics: the k-th largest of the threads' maxima
 // (each thread's maximum is an element of its own).  Only the elements of threads whose maximum reaches it (k or a few
-// more) are looked at again, by the 64 lanes of the thread's wave together; what reaches the bound goes to LDS and is
-// ranked there by counting.
+// more) are looked at again, by the whole workgroup; what reaches the bound goes to LDS and is ranked there by counting.
 template <int NT>
 struct TopLds {
   static constexpr int CAP = NT == 64 ? 512 : 1024;
   uint64_t cand[CAP];
   uint32_t best[NT];
   int at[NT];
-  int count;
+  int count, threads;
   uint32_t thr;
   int thr_at;
   uint64_t red[NT / 64];
@@ -96,31 +95,31 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
 template <typename T, int NT, typename Emit>
 SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, int at, bool odd, TopLds<NT>& L, Emit emit) {
   constexpr int E = Walk<T, NT>::E, U = Walk<T, NT>::U, SPARE = order_spare<T>;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x;
   const int chunks = (w.len + E - 1) / E;
   L.best[tid] = best;
   L.at[tid] = at;
-  if (tid == 0) L.count = 0;
+  if (tid == 0) L.count = L.threads = 0;
   __syncthreads();
   if (tid < 64) top_threshold<NT>(L, k, chunks, SPARE);
   __syncthreads();
   const uint32_t thr = L.thr, thr_top = thr | ((1u << SPARE) - 1u);
   const int thr_at = L.thr_at;
   if (!odd) {
+    // the threads that reach it, then their chunks (thread t: t, t + NT, ...) spread over the whole workgroup
     auto in = [&](uint32_t o, int chunk) { return o > thr_top || (o >= thr && chunk <= thr_at); };
-    unsigned long long todo = __builtin_amdgcn_ballot_w64(best && in(best, at));
-    while (todo) {   // the chunks of one thread of this wave: tid - lane + src, + NT, ...
-      const int src = tid - lane + __builtin_ctzll(todo);
-      todo &= todo - 1;
-      for (int c = src + NT * lane; c < chunks; c += NT * 64) {
-        const Chunk<T, E> raw = load_chunk<T, E>(w.p + (long)c * E, w.len - c * E);
+    if (best && in(best, at)) L.at[atomicAdd(&L.threads, 1)] = tid;
+    __syncthreads();
+    const int per = (chunks + NT - 1) / NT, pairs = L.threads * per;
+    for (int i = tid; i < pairs; i += NT) {
+      const int c = L.at[i / per] + NT * (i % per);
+      const Chunk<T, E> raw = load_chunk<T, E>(w.p + (long)c * E, w.len - c * E);
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const uint32_t o = ordered((float)raw.e[j]);
-          if (in(o, c) && c * E + j < w.len) {
-            const int pos = atomicAdd(&L.count, 1);
-            if (pos < TopLds<NT>::CAP) L.cand[pos] = key_of(o, lo + c * E + j);
-          }
+      for (int j = 0; j < E; ++j) {
+        const uint32_t o = ordered((float)raw.e[j]);
+        if (in(o, c) && c * E + j < w.len) {
+          const int pos = atomicAdd(&L.count, 1);
+          if (pos < TopLds<NT>::CAP) L.cand[pos] = key_of(o, lo + c * E + j);
         }
       }
     }
@@ -357,7 +356,7 @@ SCM_DEV float score_dx(const ScoreGrad& r, float x, float c) {
   return exp2_fast(d) * (r.ca + r.cb * fmaxf(d, -200.f));
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool STREAM>
 __global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, int seg_len) {
   __shared__ int target_named;
   typedef Walk<T, NT> W;
@@ -377,7 +376,7 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, i
       float o[W::E];
 #pragma unroll
       for (int j = 0; j < W::E; ++j) o[j] = score_dx(r, (float)raw[u].e[j], a.c);
-      store_chunk<T, W::E>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
+      store_chunk<T, W::E, STREAM>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
     }
   });
   // the named elements again, after the barrier: the last store to an address is theirs
@@ -459,17 +458,22 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((score_join_kernel<T, false>), dim3((unsigned)a.T), dim3(256), 0, s, a, S);
   }
 }
-template <typename T>
+template <typename T, bool STREAM>
 static void score_bwd_typed(const ScoreGradArgs& a, hipStream_t s) {
   if (a.V <= 64) {
     hipLaunchKernelGGL((score_bwd_small_kernel<T>), dim3((unsigned)((a.T + 63) / 64)), dim3(64), 0, s, a);
   } else if (a.V <= 2048) {
-    hipLaunchKernelGGL((score_bwd_kernel<T, 64>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+    hipLaunchKernelGGL((score_bwd_kernel<T, 64, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
   } else {
     // the gradient of an element needs the row's two coefficients only: segments at will, 8192 elements are one step
     const int len = logits_bwd_segment(a.T, a.V), S = segments_used(a.V, len);
-    hipLaunchKernelGGL((score_bwd_kernel<T, 256>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
+    hipLaunchKernelGGL((score_bwd_kernel<T, 256, STREAM>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
   }
+}
+template <typename T>
+static void score_bwd_sized(const ScoreGradArgs& a, hipStream_t s) {
+  if (a.T * a.V * (long)sizeof(T) > STREAM_BYTES) score_bwd_typed<T, true>(a, s);
+  else score_bwd_typed<T, false>(a, s);
 }
 // At least 8192 elements per workgroup; longer where that leaves more workgroups than a launch takes (2^31 - 1).
 int logits_bwd_segment(long T, int V) {
@@ -486,9 +490,9 @@ hipError_t score_fwd(const ScoreArgs& a, hipStream_t s) {
 }
 hipError_t score_bwd(const ScoreGradArgs& a, hipStream_t s) {
   Traced tr(K_SCORE, 0, s);
-  if (a.type == SCM_F32) score_bwd_typed<float>(a, s);
-  else if (a.type == SCM_BF16) score_bwd_typed<bf16>(a, s);
-  else score_bwd_typed<f16>(a, s);
+  if (a.type == SCM_F32) score_bwd_sized<float>(a, s);
+  else if (a.type == SCM_BF16) score_bwd_sized<bf16>(a, s);
+  else score_bwd_sized<f16>(a, s);
   return hipGetLastError();
 }
 

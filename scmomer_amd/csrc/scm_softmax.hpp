@@ -99,6 +99,17 @@ struct Walk {
   }
 };
 
+// Between two uses of a chunk that stays in registers: keeps the compiler from holding on to its f32 values (twice the
+// registers) instead of unpacking them again.
+template <typename T, int E>
+SCM_DEV void stay_packed(Chunk<T, E>& c) {
+  if constexpr (sizeof(T) == 4) return;   // f32 is as it lies
+  u32x4 w = __builtin_bit_cast(u32x4, c);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { uint32_t x = w[i]; asm volatile("" : "+v"(x)); w[i] = x; }
+  c = __builtin_bit_cast(Chunk<T, E>, w);
+}
+
 // Adds 32 elements to a thread's running statistics.
 template <bool ENT>
 SCM_DEV void stat_add(Stat& st, const float (&v)[32], float bm, float c) {

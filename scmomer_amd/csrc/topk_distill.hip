@@ -123,7 +123,7 @@ SCM_DEV Stat rest_of_segment(const Walk<T, NT>& w, const NamedBits<NT>& bits, fl
 }
 
 // Gradient of a segment from (m, cr), then the named tokens over it.
-template <typename T, int NT>
+template <typename T, int NT, bool STREAM>
 SCM_DEV void distill_write(const Walk<T, NT>& w, T* dx, int lo, float m, float cr, float c) {
   typedef Walk<T, NT> W;
   w.run([&](int s, const typename W::Raw& raw) {
@@ -132,7 +132,7 @@ SCM_DEV void distill_write(const Walk<T, NT>& w, T* dx, int lo, float m, float c
       float o[W::E];
 #pragma unroll
       for (int j = 0; j < W::E; ++j) o[j] = cr * exp2_fast(((float)raw[u].e[j] - m) * c);
-      store_chunk<T, W::E>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
+      store_chunk<T, W::E, STREAM>(dx + lo + w.first(s, u), o, w.len - w.first(s, u));
     }
   });
 }
@@ -146,7 +146,7 @@ SCM_DEV void zero_write(T* dx, int len) {
 // ---------------------------------------------------------------- V > 64
 // GRAD: loss and gradient in one launch (S = 1).  Otherwise the loss, and (tape, g_top given) what the backward reads;
 // with S > 1 the segment's statistics go to part for distill_join_kernel.
-template <typename T, int NT, bool GRAD>
+template <typename T, int NT, bool GRAD, bool STREAM = false>
 __global__ __launch_bounds__(NT) void distill_kernel(DistillTopkArgs a, int S, int seg_len) {
   __shared__ Stat red[NT / 64];
   __shared__ NamedBits<NT> bits;
@@ -193,10 +193,93 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillTopkArgs a, int S, i
   if constexpr (GRAD) {
     __syncthreads();
     const float sc = row_scale(a, row, wt);
-    distill_write<T, NT>(w, dx, 0, row_m, row_cr * sc, a.c);
+    distill_write<T, NT, STREAM>(w, dx, 0, row_m, row_cr * sc, a.c);
     __syncthreads();   // the last store to a named token is this one; equal indices hold equal values
     if (tid < a.k && idx >= 0 && idx < a.V) dx[idx] = (T)(g * sc);
   }
+}
+
+// Loss and gradient of a row that stays in registers between its one read and its one write: STEPS x 32 elements a thread
+// (at most 64 registers).
+template <typename T, int NT, int STEPS, bool STREAM>
+__global__ __launch_bounds__(NT) void distill_resident_kernel(DistillTopkArgs a) {
+  __shared__ Stat red[NT / 64];
+  __shared__ uint32_t bits[STEPS * NT];   // STEPS NT 32 tokens
+  __shared__ float row_m, row_cr;
+  typedef Walk<T, NT> W;
+  constexpr int E = W::E, U = W::U;
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x;
+  T* dx = (T*)a.dx + row * a.V;
+  const float wt = a.weight ? a.weight[row] : 1.f;
+  if (wt == 0.f) {
+    zero_write<T, NT>(dx, a.V);
+    if (tid == 0) a.row_loss[row] = 0.f;
+    return;
+  }
+  const W w{(const T*)a.x + row * a.ldx, a.V};
+  typename W::Raw raw[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) w.load(s, raw[s]);
+  // entries (first wave) and the bits of the named tokens
+  long long idx = -1;
+  float lp = 0.f, xi = 0.f;
+  if (tid < a.k) {
+    idx = a.index[row * a.k + tid];
+    lp = a.lp[row * a.k + tid];
+    if (idx >= 0 && idx < a.V) xi = (float)w.p[idx];
+  }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) bits[s * NT + tid] = 0;
+  __syncthreads();
+  if (tid < a.k && idx >= 0 && idx < a.V) atomicOr(&bits[idx >> 5], 1u << (idx & 31));
+  __syncthreads();
+  // the maximum over R first, then one exponential per element around it; named tokens and what lies past the end
+  // become -inf in the registers
+  Stat st = stat_none();
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i0 = w.first(s, u), n = a.V - i0;
+      const uint32_t named = (bits[i0 >> 5] >> (i0 & 31)) & ((1u << E) - 1u);
+      if (named || n < E) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (((named >> j) & 1) || j >= n) raw[s][u].e[j] = (T)-INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < E; ++j) st.m = fmaxf(st.m, (float)raw[s][u].e[j]);
+      stay_packed(raw[s][u]);
+    }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) st.s += exp2_fast(((float)raw[s][u].e[j] - st.m) * a.c);
+      stay_packed(raw[s][u]);
+    }
+  st = stat_block<false, NT>(st, a.c, red);
+  float g = 0.f;
+  if (tid < 64) {
+    const DistillRow r = distill_row(a, st, idx, lp, xi);
+    g = r.g;
+    if (tid == 0) { a.row_loss[row] = wt * r.loss; row_m = r.m; row_cr = r.cr; }
+  }
+  __syncthreads();
+  const float sc = row_scale(a, row, wt), m = row_m, cr = row_cr * sc;
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float o[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) o[j] = cr * exp2_fast(((float)raw[s][u].e[j] - m) * a.c);
+      store_chunk<T, E, STREAM>(dx + w.first(s, u), o, a.V - w.first(s, u));
+    }
+  __syncthreads();   // the last store to a named token is this one; equal indices hold equal values
+  if (tid < a.k && idx >= 0 && idx < a.V) dx[idx] = (T)(g * sc);
 }
 
 template <typename T>
@@ -229,7 +312,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(DistillTopkArgs a, int
   }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool STREAM>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillTopkArgs a, int S, int seg_len) {
   const long row = blockIdx.x / S;
   const int lo = (int)(blockIdx.x % S) * seg_len, tid = threadIdx.x;
@@ -238,7 +321,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillTopkArgs a, int 
   const float wt = a.weight ? a.weight[row] : 1.f;
   if (wt == 0.f) { zero_write<T, NT>(dx + lo, w.len); return; }
   const float sc = row_scale(a, row, wt);
-  distill_write<T, NT>(w, dx, lo, a.tape[2 * row], a.tape[2 * row + 1] * sc, a.c);
+  distill_write<T, NT, STREAM>(w, dx, lo, a.tape[2 * row], a.tape[2 * row + 1] * sc, a.c);
   __syncthreads();
   if (tid < a.k) {
     const long long i = a.index[row * a.k + tid];
@@ -360,7 +443,23 @@ int distill_segments(long T, int V) {
 }
 static int seg_len_of(int V, int S) { return ((V + S - 1) / S + 31) / 32 * 32; }
 
-template <typename T>
+// Loss and gradient of rows that fit a workgroup's registers.  false: they do not, or (2-byte types above 32768) would
+// leave one workgroup per CU, whose reading, reducing and writing then follow each other: 4096 x 65536 bf16 319 us,
+// against 259 us for the kernel that reads the row again from the last-level cache; 8192 x 32768: 231 against 287 us.
+template <typename T, bool STREAM>
+static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
+  constexpr int MAX = 64 / (32 * (int)sizeof(T) / 4);   // steps in 64 registers: 4 for 2-byte types, 2 for f32
+  const dim3 g((unsigned)a.T);
+  if (a.V <= 64 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM>), g, dim3(64), 0, s, a);
+  else if (a.V <= 256 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM>), g, dim3(256), 0, s, a);
+  else if (a.V <= 256 * 64) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 2, STREAM>), g, dim3(256), 0, s, a);
+  else if (a.V <= 256 * 32 * MAX) hipLaunchKernelGGL((distill_resident_kernel<T, 256, MAX, STREAM>), g, dim3(256), 0, s, a);
+  else if (sizeof(T) == 4 && a.V <= 512 * 64) hipLaunchKernelGGL((distill_resident_kernel<float, 512, 2, STREAM>), g, dim3(512), 0, s, a);
+  else if (sizeof(T) == 4 && a.V <= 1024 * 64) hipLaunchKernelGGL((distill_resident_kernel<float, 1024, 2, STREAM>), g, dim3(1024), 0, s, a);
+  else return false;
+  return true;
+}
+template <typename T, bool STREAM>
 static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s) {
   if (a.V <= 64) {
     const dim3 g((unsigned)((a.T + 63) / 64));
@@ -369,33 +468,41 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
     return;
   }
   int S = distill_segments(a.T, a.V);
-  const bool one = S == 1 && loss && grad;
-  if (one) a.tape = a.g_top = nullptr;   // for a backward of its own only
+  if (S == 1 && loss && grad) {
+    a.tape = a.g_top = nullptr;   // for a backward of its own only
+    // (512 threads: two workgroups per CU, whose rows fit the last-level cache together; 256: 2048 x 131072 364 us, 512: 334 us)
+    if (!launch_resident<T, STREAM>(a, s))
+      hipLaunchKernelGGL((distill_kernel<T, 512, true, STREAM>), dim3((unsigned)a.T), dim3(512), 0, s, a, 1, a.V);
+    return;
+  }
   if (loss) {
     if (a.V <= 2048) {
-      if (one) hipLaunchKernelGGL((distill_kernel<T, 64, true>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
-      else hipLaunchKernelGGL((distill_kernel<T, 64, false>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+      hipLaunchKernelGGL((distill_kernel<T, 64, false>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
     } else {
       const int len = S > 1 ? seg_len_of(a.V, S) : a.V;
       S = (a.V + len - 1) / len;
-      if (one) hipLaunchKernelGGL((distill_kernel<T, 256, true>), dim3((unsigned)a.T), dim3(256), 0, s, a, 1, a.V);
-      else hipLaunchKernelGGL((distill_kernel<T, 256, false>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
+      hipLaunchKernelGGL((distill_kernel<T, 256, false>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
       if (S > 1) hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)a.T), dim3(64), 0, s, a, S);
     }
   }
-  if (grad && !one) {
+  if (grad) {
     if (a.V <= 2048) {
-      hipLaunchKernelGGL((distill_bwd_kernel<T, 64>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 64, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
     } else {
       const int len = logits_bwd_segment(a.T, a.V), sb = (a.V + len - 1) / len;
-      hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)(a.T * sb)), dim3(256), 0, s, a, sb, len);
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 256, STREAM>), dim3((unsigned)(a.T * sb)), dim3(256), 0, s, a, sb, len);
     }
   }
 }
+template <typename T>
+static void distill_sized(const DistillTopkArgs& a, bool loss, bool grad, hipStream_t s) {
+  if (grad && a.T * a.V * (long)sizeof(T) > STREAM_BYTES) distill_typed<T, true>(a, loss, grad, s);
+  else distill_typed<T, false>(a, loss, grad, s);
+}
 static void distill_dispatch(const DistillTopkArgs& a, bool loss, bool grad, hipStream_t s) {
-  if (a.type == SCM_F32) distill_typed<float>(a, loss, grad, s);
-  else if (a.type == SCM_BF16) distill_typed<bf16>(a, loss, grad, s);
-  else distill_typed<f16>(a, loss, grad, s);
+  if (a.type == SCM_F32) distill_sized<float>(a, loss, grad, s);
+  else if (a.type == SCM_BF16) distill_sized<bf16>(a, loss, grad, s);
+  else distill_sized<f16>(a, loss, grad, s);
 }
 hipError_t topk_distill_fwd(const DistillTopkArgs& a, float* out, float* wsum_out, hipStream_t s) {
   Traced tr(K_TOPK_DISTILL, 0, s);
