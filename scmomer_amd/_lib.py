@@ -174,3 +174,18 @@ def check(code: int, what: str):
     if code != 0:
         msg = lib.scm_last_error().decode("utf-8", "replace")
         raise ScmError(f"{what} failed ({code}): {msg}")
+
+
+def _load_torch_ops():
+    """The torch functions over the C ABI (csrc/torch_ops.cpp), calling into `lib`."""
+    import torch  # noqa: F401  (its libraries first)
+    try:
+        from . import _torch_ops
+    except ImportError as e:
+        raise ImportError(f"{os.path.join(_HERE, '_torch_ops.so')} is missing or does not match this torch: build it with "
+                          "`make -C scmomer_amd/csrc`. There is no fallback path.") from e
+    _torch_ops.bind(lambda name: C.cast(getattr(lib, name), C.c_void_p).value)
+    return _torch_ops
+
+
+torch_ops = _load_torch_ops()

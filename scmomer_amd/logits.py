@@ -8,9 +8,8 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import ops
+from ._lib import torch_ops
 
 
 class TokenLogprobs(NamedTuple):
@@ -21,39 +20,6 @@ class TokenLogprobs(NamedTuple):
     lse: torch.Tensor                     # f32 [...]: log of the sum of exponentials
     top_logprob: Optional[torch.Tensor]   # f32 [..., k], descending
     top_index: Optional[torch.Tensor]     # int64 [..., k]
-
-
-def _shaped(logits, lp, ent, lse, tlp, tix):
-    if logits.dim() == 2:
-        return lp, ent, lse, tlp, tix
-    shape = logits.shape[:-1]
-    return (lp if lp is None else lp.view(shape), ent if ent is None else ent.view(shape), lse.view(shape),
-            tlp if tlp is None else tlp.view(*shape, tlp.shape[1]), tix if tix is None else tix.view(*shape, tix.shape[1]))
-
-
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, k, temperature, ignore_index, entropy):
-        lp, ent, lse, tlp, tix, tape = ops.score_fwd(logits, targets, k, temperature, ignore_index, entropy, tape=True)
-        ctx.set_materialize_grads(False)
-        ctx.opts = (temperature, ignore_index)
-        ctx.save_for_backward(logits, targets, ent, tix, tape)
-        if k:
-            ctx.mark_non_differentiable(tix)
-        return _shaped(logits, lp, ent, lse, tlp, tix)
-
-    @staticmethod
-    def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
-        if torch.is_grad_enabled():
-            return _TokenLogprobsFn._once(ctx, g_logprob, g_entropy, g_lse, g_top, _)
-        logits, targets, entropy, top_index, tape = ctx.saved_tensors
-        dx = ops.score_bwd(logits, targets, tape, entropy, top_index, g_logprob, g_entropy, g_lse, g_top, *ctx.opts)
-        return dx if logits.dim() == 2 else dx.view(logits.shape), None, None, None, None, None
-
-    @staticmethod
-    @once_differentiable
-    def _once(ctx, *grads):      # under create_graph: what comes back refuses to be differentiated again
-        return _TokenLogprobsFn.backward(ctx, *grads)
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, *, k: int = 0, temperature: float = 1.0,
@@ -68,33 +34,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
 
     Differentiable once in the logits, through every output but ``top_index`` (the choice of the alternatives is a
     constant, as for torch.topk)."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, k, temperature, ignore_index, entropy))
-    return TokenLogprobs(*_shaped(logits, *ops.score_fwd(logits, targets, k, temperature, ignore_index, entropy)[:5]))
-
-
-class _TopkDistillFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_index, top_logprob, temperature, tail, weight, reduction):
-        op = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction)
-        rows, loss, wsum, tape = op.forward(reduction != "none", True)
-        ctx.opts = (temperature, tail, reduction)
-        ctx.save_for_backward(logits, top_index, top_logprob, weight, wsum, tape)
-        return loss if loss is not None else rows if logits.dim() == 2 else rows.view(logits.shape[:-1])
-
-    @staticmethod
-    def backward(ctx, gloss):
-        if torch.is_grad_enabled():
-            return _TopkDistillFn._once(ctx, gloss)
-        logits, top_index, top_logprob, weight, wsum, tape = ctx.saved_tensors
-        temperature, tail, reduction = ctx.opts
-        dx = ops.TopkDistill.again(logits, top_index, top_logprob, temperature, tail, weight, reduction).backward(gloss, wsum, tape)
-        return dx if logits.dim() == 2 else dx.view(logits.shape), None, None, None, None, None, None
-
-    @staticmethod
-    @once_differentiable
-    def _once(ctx, gloss):      # under create_graph: what comes back refuses to be differentiated again
-        return _TopkDistillFn.backward(ctx, gloss)
+    return TokenLogprobs(*torch_ops.token_logprobs(logits, targets, k, temperature, ignore_index, entropy))
 
 
 def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *, temperature: float = 1.0,
@@ -110,11 +50,7 @@ def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob
     loss is f32 and not multiplied by temperature^2.  A row of -inf throughout counts with loss and gradient 0.
 
     Differentiable once, in the logits only.  The result does not depend on the order in which workgroups run."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _TopkDistillFn.apply(logits, top_index, top_logprob, temperature, tail, weight, reduction)
-    op = ops.TopkDistill(logits, top_index, top_logprob, temperature, tail, weight, reduction)
-    rows, loss, _, _ = op.forward(reduction != "none", False)
-    return loss if loss is not None else rows.view(logits.shape[:-1])
+    return torch_ops.topk_distillation(logits, top_index, top_logprob, temperature, tail, weight, reduction)
 
 
 def topk_distillation_grad(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *,
@@ -123,7 +59,4 @@ def topk_distillation_grad(logits: torch.Tensor, top_index: torch.Tensor, top_lo
     """(loss, scale * d loss / d logits) of topk_distillation ('mean' or 'sum') in one pass over the logits, for a loop
     that runs the model's backward itself: ``loss, d = topk_distillation_grad(logits, ..., scale=1 / grad_acc)``,
     ``logits.backward(d)``.  The gradient has the logits' type and shape."""
-    if reduction == "none":
-        raise ValueError("topk_distillation_grad: reduction must be 'mean' or 'sum'")
-    loss, dx = ops.TopkDistill(logits.detach(), top_index, top_logprob, temperature, tail, weight, reduction).step(scale)
-    return loss, dx if logits.dim() == 2 else dx.view(logits.shape)
+    return torch_ops.topk_distillation_grad(logits, top_index, top_logprob, temperature, tail, weight, reduction, scale)

@@ -1,7 +1,8 @@
 """Torch-tensor front end of the C ABI: allocates outputs/workspaces with torch (device memory
 and streams are torch's job here), passes raw device pointers and the current stream.
 
-Every function requires CUDA(HIP) tensors; nothing here computes on the host.
+Every function requires CUDA(HIP) tensors; nothing here computes on the host.  (The operators of norm.py and logits.py,
+which eager programs call one by one, have their front end in csrc/torch_ops.cpp.)
 """
 from __future__ import annotations
 
@@ -147,102 +148,6 @@ def ln_bwd(dy, x, mean, rstd, gamma, dres, dgamma, dbeta, dres_colsum, accumulat
         defer.append(colsum_job(ws, ws.numel() // (3 * d), 3 * d,
                                 [(dgamma, 0, d), (dbeta, d, 2 * d), (dres_colsum, 2 * d, 3 * d)], accumulate))
     return (dx, dxb) if with_bf16 else dx
-
-
-# ----------------------------------------------------------------------------- rows of any width and type
-# These operators are called one by one from programs of their own (the encoder's run inside recorded launch chains), so
-# the host's part counts: one look at each property of a tensor, few allocations, no context manager on the way.
-SCM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-NORM_MAX_D = 16384
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream       # of a device, as a number
-_empty, _empty_like = torch.empty, torch.empty_like
-
-
-def _device_of(t: torch.Tensor, *others) -> int:
-    """the index of the device that t and the others (tensors or None) share"""
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError("expected device tensors; scmomer_amd has no CPU path")
-    for o in others:
-        if o is not None and o.get_device() != dev:
-            raise ValueError(f"tensors on different devices: {t.device} and {o.device}")
-    return dev
-
-
-def _on_device(dev: int, entry, *args):
-    """entry(*args, stream) on the device's current stream; a launch goes to the current device, so that is changed for
-    the call where the tensors are on another one"""
-    if dev == _current_device():
-        return entry(*args, _raw_stream(dev))
-    with torch.cuda.device(dev):
-        return entry(*args, _raw_stream(dev))
-
-
-def rows_of(t: torch.Tensor, name: str) -> torch.Tensor:
-    """[T, D] form of a tensor [..., D] of one of SCM_TYPES: a view where one row stride describes it (an expanded
-    batch keeps stride 0), a contiguous copy otherwise"""
-    if t.dtype not in SCM_TYPES:
-        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    if t.dim() != 2:
-        if t.dim() < 1 or t.shape[-1] < 1:
-            raise ValueError(f"{name}: expected [..., D] with D >= 1, got {tuple(t.shape)}")
-        t = t.reshape(t.numel() // t.shape[-1], t.shape[-1])
-    if t.stride(1) != 1 and t.shape[1] != 1:
-        t = t.contiguous()
-    return t
-
-
-def norm_fwd(x: torch.Tensor, gamma, beta, eps: float, out_dtype=None, stats: bool = True):
-    """LayerNorm over the last dimension (rows_of(x) is what it reads).  -> (y [T, D], statistics f32 [2, T] = mean and
-    1 / standard deviation, or None when stats is false)"""
-    x = rows_of(x, "x")
-    t, d = x.shape
-    dtype = x.dtype
-    if out_dtype is None:
-        out_dtype = dtype
-    elif out_dtype != dtype and (dtype, out_dtype) != (F32, BF16):
-        raise TypeError(f"layer norm: {dtype} in gives {dtype} out, or bfloat16 from float32 (asked for {out_dtype})")
-    if not 1 <= d <= NORM_MAX_D:
-        raise ValueError(f"layer norm: 1 to {NORM_MAX_D} columns (got {d})")
-    for p, nm in ((gamma, "weight"), (beta, "bias")):
-        if p is not None:
-            if p.dtype != F32:
-                raise TypeError(f"{nm}: expected {F32}, got {p.dtype}")
-            if p.dim() != 1 or p.shape[0] != d or not p.is_contiguous():
-                raise ValueError(f"{nm}: expected a contiguous [{d}], got {tuple(p.shape)}")
-    dev = _device_of(x, gamma, beta)
-    y = _empty((t, d), dtype=out_dtype, device=x.device)
-    st = _empty((2, t), dtype=F32, device=x.device) if stats else None
-    if t:
-        mean = st.data_ptr() if stats else None
-        check(_on_device(dev, lib.scm_norm_fwd, x.data_ptr(), SCM_TYPES[dtype], x.stride(0),
-                         None if gamma is None else gamma.data_ptr(), None if beta is None else beta.data_ptr(), t, d, eps,
-                         y.data_ptr(), SCM_TYPES[out_dtype], mean, mean + 4 * t if stats else None), "scm_norm_fwd")
-    return y, st
-
-
-def norm_bwd(dy: torch.Tensor, x: torch.Tensor, st: torch.Tensor, gamma, want_dx: bool = True, want_dgamma: bool = True,
-             want_dbeta: bool = True):
-    """-> (dx [T, D] in x's type, dgamma f32 [D], dbeta f32 [D]), None for what is not wanted.  dy has the type of
-    norm_fwd's y, st is its statistics."""
-    dy, x = rows_of(dy, "dy"), rows_of(x, "x")
-    t, d = x.shape
-    if dy.shape != x.shape:
-        raise ValueError(f"layer norm: dy {tuple(dy.shape)} for x {tuple(x.shape)}")
-    dev = _device_of(x, dy, st, gamma)
-    device = x.device
-    dx = _empty((t, d), dtype=x.dtype, device=device) if want_dx else None
-    new = _empty if t else torch.zeros      # no rows: the sums are empty
-    dgamma = new(d, dtype=F32, device=device) if want_dgamma else None
-    dbeta = new(d, dtype=F32, device=device) if want_dbeta else None
-    if t and (want_dx or want_dgamma or want_dbeta):
-        ws = _empty(lib.scm_norm_bwd_ws_floats(t, d), dtype=F32, device=device) if want_dgamma or want_dbeta else None
-        mean = st.data_ptr()
-        check(_on_device(dev, lib.scm_norm_bwd, dy.data_ptr(), SCM_TYPES[dy.dtype], dy.stride(0), x.data_ptr(),
-                         SCM_TYPES[x.dtype], x.stride(0), mean, mean + 4 * t, None if gamma is None else gamma.data_ptr(),
-                         t, d, _p(dx), _p(ws), _p(dgamma), _p(dbeta)), "scm_norm_bwd")
-    return dx, dgamma, dbeta
 
 
 def gemm_res_ln_supported(a: torch.Tensor, w: torch.Tensor) -> bool:
@@ -636,187 +541,6 @@ def s1_accuracy(logits: torch.Tensor, labels: torch.Tensor, pad_id: int):
     check(lib.scm_s1_accuracy(_p(logits), _p(labels), b, n, c, pad_id, _p(ratio), _p(counts), _p(ws), _stream()),
           "scm_s1_accuracy")
     return ratio, counts
-
-
-# ----------------------------------------------------------------------------- rows of logits
-LOGITS_MAX_K = 64
-_INF = float("inf")
-
-
-def _logits_rows(logits: torch.Tensor, temperature: float, k: int) -> torch.Tensor:
-    x = rows_of(logits, "logits")
-    if not 1 <= x.shape[1] <= 1 << 30:
-        raise ValueError(f"logits: 1 to 2^30 classes (got {x.shape[1]})")
-    if not 0.0 < temperature < _INF:
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    if not 0 <= k <= LOGITS_MAX_K:
-        raise ValueError(f"at most {LOGITS_MAX_K} entries per row (got {k})")
-    return x
-
-
-def _row_vector(t: torch.Tensor, logits: torch.Tensor, dtype, name: str) -> torch.Tensor:
-    """one value per row of the logits, contiguous"""
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.shape != logits.shape[:-1]:
-        raise ValueError(f"{name}: expected {tuple(logits.shape[:-1])}, got {tuple(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _grad_rows(g, n: int, name: str):
-    """an incoming gradient of n values as contiguous f32, or None"""
-    if g is None:
-        return None
-    if g.numel() != n:
-        raise ValueError(f"gradient of {name}: {g.numel()} values, expected {n}")
-    if g.dtype != F32:
-        g = g.to(F32)
-    return g if g.is_contiguous() else g.contiguous()
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def score_fwd(logits, targets, k: int = 0, temperature: float = 1.0, ignore_index: int = -100, entropy: bool = True,
-              tape: bool = False):
-    """Rows of logits [..., V] -> (logprob [T] or None, entropy [T] or None, lse [T], top_logprob [T, k] or None,
-    top_index int64 [T, k] or None, tape [T, 2] or None); what score_bwd needs is the tape, entropy and top_index"""
-    x = _logits_rows(logits, temperature, k)
-    t, v = x.shape
-    if k > v:
-        raise ValueError(f"{k} alternatives of {v} classes")
-    if targets is not None:
-        targets = _row_vector(targets, logits, torch.int64, "targets")
-    dev = _device_of(x, targets)
-    device = x.device
-    lp = _empty(t, dtype=F32, device=device) if targets is not None else None
-    lse = _empty(t, dtype=F32, device=device)
-    ent = _empty(t, dtype=F32, device=device) if entropy else None
-    tlp = tix = None
-    if k:
-        tlp = _empty((t, k), dtype=F32, device=device)
-        tix = _empty((t, k), dtype=torch.int64, device=device)
-    mz = _empty((t, 2), dtype=F32, device=device) if tape else None
-    if t:
-        n = lib.scm_score_ws_floats(t, v, k)
-        ws = _empty(n, dtype=F32, device=device) if n else None
-        check(_on_device(dev, lib.scm_score_fwd, x.data_ptr(), SCM_TYPES[x.dtype], x.stride(0), t, v, temperature,
-                         _ptr(targets), ignore_index, k, _ptr(lp), lse.data_ptr(), _ptr(ent), _ptr(tlp), _ptr(tix), _ptr(mz),
-                         _ptr(ws)), "scm_score_fwd")
-    return lp, ent, lse, tlp, tix, mz
-
-
-def score_bwd(logits, targets, tape, entropy, top_index, g_logprob, g_entropy, g_lse, g_top, temperature: float = 1.0,
-              ignore_index: int = -100) -> torch.Tensor:
-    """-> the gradient [T, V] in the logits' type; each g_* is a tensor of its output's size or None"""
-    k = top_index.shape[1] if top_index is not None else 0
-    x = _logits_rows(logits, temperature, k)
-    t, v = x.shape
-    g_logprob, g_entropy = _grad_rows(g_logprob, t, "logprob"), _grad_rows(g_entropy, t, "entropy")
-    g_lse, g_top = _grad_rows(g_lse, t, "lse"), _grad_rows(g_top, t * k, "top_logprob")
-    if targets is not None:
-        targets = _row_vector(targets, logits, torch.int64, "targets")
-    dev = _device_of(x, targets, tape, entropy, top_index, g_logprob, g_entropy, g_lse, g_top)
-    dx = _empty((t, v), dtype=x.dtype, device=x.device)
-    if t:
-        check(_on_device(dev, lib.scm_score_bwd, x.data_ptr(), SCM_TYPES[x.dtype], x.stride(0), t, v, temperature,
-                         _ptr(targets), ignore_index, k, tape.data_ptr(), _ptr(entropy), _ptr(top_index), _ptr(g_logprob),
-                         _ptr(g_lse), _ptr(g_entropy), _ptr(g_top), dx.data_ptr()), "scm_score_bwd")
-    return dx
-
-
-class TopkDistill:
-    """The checked operands of one distillation from top log probabilities; see the C ABI for the definition."""
-    __slots__ = ("x", "keep", "common", "dev", "k", "mean")
-
-    def __init__(self, logits, index, logprob, temperature: float, tail: bool, weight, reduction: str):
-        if index.shape != logprob.shape or index.shape[:-1] != logits.shape[:-1] or index.dim() != logits.dim():
-            raise ValueError(f"teacher entries {tuple(index.shape)} and {tuple(logprob.shape)} for logits {tuple(logits.shape)}")
-        self.k = k = index.shape[-1]
-        if k < 1:
-            raise ValueError("no teacher entries")
-        if reduction not in ("mean", "sum", "none"):
-            raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-        self.x = x = _logits_rows(logits, temperature, k)
-        if index.dtype != torch.int64:
-            raise TypeError(f"top_index: expected {torch.int64}, got {index.dtype}")
-        if logprob.dtype != F32:
-            raise TypeError(f"top_logprob: expected {F32}, got {logprob.dtype}")
-        if weight is not None:
-            weight = _row_vector(weight, logits, F32, "weight")
-        if logprob.requires_grad or (weight is not None and weight.requires_grad):
-            raise ValueError("the teacher's log probabilities and the weights take no gradient: detach them")
-        self._take(index, logprob, temperature, tail, weight, reduction)
-
-    @classmethod
-    def again(cls, logits, index, logprob, temperature, tail, weight, reduction):
-        """for operands that have been checked before (those of a forward, in its backward)"""
-        op = cls.__new__(cls)
-        op.x, op.k = rows_of(logits, "logits"), index.shape[-1]
-        if weight is not None and not weight.is_contiguous():
-            weight = weight.contiguous()
-        op._take(index, logprob, temperature, tail, weight, reduction)
-        return op
-
-    def _take(self, index, logprob, temperature, tail, weight, reduction):
-        x = self.x
-        self.dev = _device_of(x, index, logprob, weight)
-        if not index.is_contiguous():
-            index = index.contiguous()
-        if not logprob.is_contiguous():
-            logprob = logprob.contiguous()
-        self.keep = (index, logprob, weight)
-        self.mean = reduction == "mean"
-        self.common = (x.data_ptr(), SCM_TYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], temperature, index.data_ptr(),
-                       logprob.data_ptr(), self.k, int(bool(tail)), _ptr(weight), int(self.mean))
-
-    def _new(self, n):
-        return _empty(n, dtype=F32, device=self.x.device) if n else None
-
-    def forward(self, want_sum: bool, want_tape: bool):
-        """-> (row losses f32 [T], loss f32 [] or None, sum of the weights [1] or None, tape or None)"""
-        t, v = self.x.shape
-        rows = _empty(t, dtype=F32, device=self.x.device)
-        if not t:      # an empty sum; its mean is 0 / 0
-            loss = rows.new_full((), float("nan") if self.mean else 0.0) if want_sum else None
-            return rows, loss, None, None
-        loss = _empty((), dtype=F32, device=self.x.device) if want_sum else None
-        wsum = _empty(1, dtype=F32, device=self.x.device) if want_sum and want_tape else None
-        tape = self._new(lib.scm_topk_distill_tape_floats(t, v, self.k)) if want_tape else None
-        ws = self._new(lib.scm_topk_distill_ws_floats(t, v))
-        check(_on_device(self.dev, lib.scm_topk_distill_fwd, *self.common, rows.data_ptr(), _ptr(loss), _ptr(wsum), _ptr(tape),
-                         _ptr(ws)), "scm_topk_distill_fwd")
-        return rows, loss, wsum, tape
-
-    def backward(self, gloss, wsum, tape):
-        """gloss: the incoming gradient, one value or (reduction 'none') one per row -> dlogits [T, V]"""
-        x = self.x
-        t, v = x.shape
-        per_row = wsum is None
-        dx = _empty((t, v), dtype=x.dtype, device=x.device)
-        if t:
-            gloss = _grad_rows(gloss, t if per_row else 1, "loss")
-            _device_of(x, gloss, wsum, tape)
-            check(_on_device(self.dev, lib.scm_topk_distill_bwd, *self.common, _ptr(wsum), gloss.data_ptr(), int(per_row),
-                             _ptr(tape), dx.data_ptr()), "scm_topk_distill_bwd")
-        return dx
-
-    def step(self, scale: float):
-        """-> (loss f32 [], dlogits [T, V] = scale * its gradient)"""
-        x = self.x
-        t, v = x.shape
-        dx = _empty((t, v), dtype=x.dtype, device=x.device)
-        if not t:
-            return self.forward(True, False)[1], dx
-        loss = _empty((), dtype=F32, device=x.device)
-        buf = self._new(t + 1)      # the rows' losses, the sum of the weights
-        tape = self._new(lib.scm_topk_distill_tape_floats(t, v, self.k))
-        ws = self._new(lib.scm_topk_distill_ws_floats(t, v))
-        p = buf.data_ptr()
-        check(_on_device(self.dev, lib.scm_topk_distill_step, *self.common, scale, p, loss.data_ptr(), p + 4 * t, _ptr(tape),
-                         _ptr(ws), dx.data_ptr()), "scm_topk_distill_step")
-        return loss, dx
 
 
 # ----------------------------------------------------------------------------- cell-embedding tail
