@@ -130,6 +130,7 @@ SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, 
     for (int i = tid; i < n; i += NT) {
       const uint64_t mine = L.cand[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) rank += L.cand[j] > mine;
       if (rank < k) emit(rank, mine);
     }
@@ -196,6 +197,14 @@ __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_l
   const long row = blockIdx.x / S;
   const int seg = blockIdx.x % S, lo = seg * seg_len;
   const W w{(const T*)a.x + row * a.ldx + lo, min(a.V - lo, seg_len)};
+  // the last thread writes the row's numbers (the first wave is busy with the alternatives); its target is here by then
+  const bool writer = S == 1 && threadIdx.x == NT - 1;
+  long long target = -1;
+  float x_target = 0.f;
+  if (writer && a.target) {
+    target = a.target[row];
+    if (target >= 0 && target < a.V) x_target = (float)w.p[target];
+  }
   Stat st = stat_none();
   float best = -INFINITY;
   int at = threadIdx.x;
@@ -228,11 +237,7 @@ __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_l
     }
     return;
   }
-  if (threadIdx.x == 0) {
-    const long long t = a.target ? a.target[row] : 0;
-    const float xt = a.target && t >= 0 && t < a.V ? (float)w.p[t] : 0.f;
-    write_row<ENT>(a, row, st, xt, t);
-  }
+  if (writer) write_row<ENT>(a, row, st, x_target, target);
   if constexpr (TOP) {
     const RowScore r(st, a.inv_t);
     top_of_segment<T, NT>(w, 0, a.k, (int)threadIdx.x * W::E < w.len ? ordered(best) : 0u, at, odd, top,
@@ -247,45 +252,49 @@ __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_l
 // keys reach the q-th largest of the lists' p-th keys; those are collected and ranked by counting.
 template <typename T, bool ENT>
 __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a, int S) {
-  __shared__ uint64_t cand[LOGITS_JOIN_KEYS];
-  __shared__ uint64_t head[LOGITS_MAX_SEGMENTS], thr;
+  __shared__ uint64_t keys[LOGITS_JOIN_KEYS], cand[LOGITS_JOIN_KEYS];   // S k keys at most
+  __shared__ uint64_t thr;
   __shared__ int count;
   const long row = blockIdx.x;
-  const int tid = threadIdx.x, l = tid & 63;
-  Stat st = stat_none();   // every wave joins them all: no exchange between waves
-  for (int i = l; i < S; i += 64) {
-    const float* p = a.part + 3 * (row * S + i);
-    st = stat_join<ENT>(st, Stat{p[0], p[1], p[2]}, a.c);
+  const int tid = threadIdx.x, l = tid & 63, n = S * a.k;
+  // everything that is read, at once: the keys, the segments' statistics (every wave joins them all), the target
+  for (int i = tid; i < n; i += 256) keys[i] = a.part_top[row * n + i];
+  Stat st = stat_none();
+  if (l < S) {   // S <= 64
+    const float* p = a.part + 3 * (row * S + l);
+    st = Stat{p[0], p[1], p[2]};
+  }
+  long long target = -1;
+  float x_target = 0.f;
+  if (tid == 255 && a.target) {
+    target = a.target[row];
+    if (target >= 0 && target < a.V) x_target = (float)((const T*)a.x)[row * a.ldx + target];
   }
   st = stat_wave<ENT>(st, a.c);
-  if (tid == 0) {
-    const long long t = a.target ? a.target[row] : 0;
-    const float xt = a.target && t >= 0 && t < a.V ? (float)((const T*)a.x)[row * a.ldx + t] : 0.f;
-    write_row<ENT>(a, row, st, xt, t);
-  }
+  if (tid == 255) write_row<ENT>(a, row, st, x_target, target);
   if (!a.k) return;
-  const uint64_t* keys = a.part_top + row * S * a.k;
-  const int p = (a.k + S - 1) / S, q = (a.k + p - 1) / p;
-  for (int i = tid; i < S; i += 256) head[i] = keys[(long)i * a.k + p - 1];
   if (tid == 0) { count = 0; thr = 1; }
   __syncthreads();
-  for (int i = tid; i < S; i += 256) {
+  const int p = (a.k + S - 1) / S, q = (a.k + p - 1) / p;
+  if (tid < S) {
+    const uint64_t mine = keys[tid * a.k + p - 1];
     int rank = 0;
-    for (int j = 0; j < S; ++j) rank += head[j] > head[i];
-    if (rank == q - 1 && head[i]) thr = head[i];   // keys are distinct; an empty place (0) bounds nothing
+#pragma unroll 8
+    for (int j = 0; j < S; ++j) rank += keys[j * a.k + p - 1] > mine;
+    if (rank == q - 1 && mine) thr = mine;   // keys are distinct; an empty place (0) bounds nothing
   }
   __syncthreads();
   const uint64_t t = thr;
-  for (int i = tid; i < S * a.k; i += 256) {
-    const uint64_t key = keys[i];
-    if (key >= t) cand[atomicAdd(&count, 1)] = key;   // at most S k <= LOGITS_JOIN_KEYS
-  }
+  for (int i = tid; i < n; i += 256)
+    if (keys[i] >= t) cand[atomicAdd(&count, 1)] = keys[i];
   __syncthreads();
   const RowScore r(st, a.inv_t);
-  for (int i = tid; i < count; i += 256) {
+  const int found = count;
+  for (int i = tid; i < found; i += 256) {
     const uint64_t mine = cand[i];
     int rank = 0;
-    for (int j = 0; j < count; ++j) rank += cand[j] > mine;
+#pragma unroll 8
+    for (int j = 0; j < found; ++j) rank += cand[j] > mine;
     if (rank < a.k) {
       a.top_index[row * a.k + rank] = key_index(mine);
       a.top_logprob[row * a.k + rank] = r.logp(key_value(mine));

@@ -26,15 +26,11 @@ SCM_DEV Stat stat_join(const Stat& a, const Stat& b, float c) {
   if constexpr (ENT) r.h = fa * (a.h + da * a.s) + fb * (b.h + db * b.s);
   return r;
 }
+// Over the 64 lanes, in every lane: the common maximum first, then one rescaling and plain sums.
 template <bool ENT>
-SCM_DEV Stat stat_wave(Stat v, float c) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    Stat w{__shfl_xor(v.m, o), __shfl_xor(v.s, o), 0.f};
-    if constexpr (ENT) w.h = __shfl_xor(v.h, o);
-    v = (threadIdx.x & o) ? stat_join<ENT>(w, v, c) : stat_join<ENT>(v, w, c);   // the same order in both lanes
-  }
-  return v;
+SCM_DEV Stat stat_wave(const Stat& v, float c) {
+  const float m = wave_max(v.m), d = grown(v.m, m, c), f = exp2_fast(d);
+  return {m, wave_sum(v.s * f), ENT ? wave_sum(f * (v.h + d * v.s)) : 0.f};
 }
 // Over the NT threads of the workgroup, in every thread.  red: NT / 64 entries.
 template <bool ENT, int NT>
@@ -43,9 +39,15 @@ SCM_DEV Stat stat_block(Stat v, float c, Stat* red) {
   if constexpr (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  Stat r = red[0];
+  Stat r{LOWEST, 0.f, 0.f};
 #pragma unroll
-  for (int w = 1; w < NT / 64; ++w) r = stat_join<ENT>(r, red[w], c);
+  for (int w = 0; w < NT / 64; ++w) r.m = fmaxf(r.m, red[w].m);
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    const float d = grown(red[w].m, r.m, c), f = exp2_fast(d);
+    r.s += red[w].s * f;
+    if constexpr (ENT) r.h += f * (red[w].h + d * red[w].s);
+  }
   return r;
 }
 
