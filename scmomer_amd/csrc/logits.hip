@@ -5,9 +5,8 @@
 // c = log2(e) / temperature, in f32; threads, waves and workgroups join by rescaling to the larger maximum.  x - m is
 // formed first: a row of the type's lowest value is an ordinary (uniform) row, and -inf weighs nothing.
 //   V <= 64    one thread per row, 64 rows staged through LDS per wave
-//   V <= 2048  one wave per row
-//   else       256 threads per row, and where rows are too few to fill the card a row is split into segments of one
-//              workgroup each, whose partial results a second launch joins in segment order
+//   else       64 to 512 threads per row by its length; where rows are too few to fill the card a row is split into
+//              segments of one workgroup each, whose partial results a second launch joins in segment order
 // What bounds them is HBM, and for 2-byte types the vector ALU nearly as much (an exponential costs four issue slots).
 #include "scm_softmax.hpp"
 
@@ -38,7 +37,7 @@ SCM_DEV uint64_t shfl64(uint64_t v, int mask) {
 // more) are looked at again, by the whole workgroup; what reaches the bound goes to LDS and is ranked there by counting.
 template <int NT>
 struct TopLds {
-  static constexpr int CAP = NT == 64 ? 512 : 1024;
+  static constexpr int CAP = NT == 64 ? 512 : 1024;   // NT >= 2 k: about NT ln 2 + spread at most are expected
   uint64_t cand[CAP];
   uint32_t best[NT];
   int at[NT];
@@ -46,39 +45,50 @@ struct TopLds {
   uint32_t thr;
   int thr_at;
   uint64_t red[NT / 64];
+  uint64_t picked[LOGITS_MAX_K + LOGITS_MAX_K / 8];
 };
 // Low bits of ordered() that carry nothing: the same for all values of one sign of a 16-bit type.
 template <typename T> constexpr int order_spare = 0;
 template <> constexpr int order_spare<bf16> = 16;
 template <> constexpr int order_spare<f16> = 13;
-// Threshold (value, chunk) over the NT maxima, by the first wave: the k-th largest value, and among equal values the
-// chunk up to which the k-th place reaches.  Threads without elements hold value 0.
+// Threshold (value, chunk) over the NT maxima, by the first wave: a value that k to k + k / 8 of them reach, found bit by
+// bit below the bits that they all share; among equal maxima (more than that reach the last value) the chunk up to which
+// the k-th place goes.  Threads without elements hold value 0.
 template <int NT>
 SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
   constexpr int R = NT / 64;
   const int l = threadIdx.x & 63;
-  uint32_t b[R];
+  uint32_t b[R], lo = 0xFFFFFFFFu, hi = 0;
   int at[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) { b[r] = L.best[r * 64 + l]; at[r] = L.at[r * 64 + l]; }
-  uint32_t t = 0;
-  int reach = 64 * R, above = 0;   // how many maxima are >= t, and > t
-  for (int bit = 31; bit >= spare; --bit) {
+  for (int r = 0; r < R; ++r) {
+    b[r] = L.best[r * 64 + l];
+    at[r] = L.at[r * 64 + l];
+    lo = min(lo, b[r]);
+    hi = max(hi, b[r]);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) { lo = min(lo, (uint32_t)__shfl_xor((int)lo, o)); hi = max(hi, (uint32_t)__shfl_xor((int)hi, o)); }
+  // all maxima lie in [lo, hi]; t keeps the invariant: reach of them are >= t, reach >= k (0: fewer than k threads hold
+  // elements, then every element is a candidate)
+  const int shared = lo == hi ? 0 : 32 - __builtin_clz(lo ^ hi);   // bits that differ
+  uint32_t t = shared >= 32 ? 0u : (hi >> shared) << shared;
+  int reach = NT, above = 0, bit = shared - 1;
+  const int enough = k + k / 8;
+  for (; bit >= spare && reach > enough; --bit) {
     const uint32_t cand = t | (1u << bit);
     int n = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] >= cand));
     if (n >= k) { t = cand; reach = n; } else { above = n; }
   }
-  // t is the k-th largest value with its spare low bits 0 (0: fewer than k threads hold elements, every element is a
-  // candidate); maxima from t to t + 2^spare - 1 are the equal ones.  The last bits that were refused count those above.
+  // all bits used and still too many: the maxima from t to t + 2^spare - 1 are equal, `above` lie above them
   const uint32_t top = t | ((1u << spare) - 1u);
   int lim = 0x7FFFFFFF;
-  if (t && reach > k) {
-    // more equal maxima than places: the smallest bound with enough of them at chunks <= lim
-    const int need = k - above;
+  if (t && reach > enough) {
+    const int need = k - above;   // the smallest bound with enough equal maxima at chunks <= lim
     lim = 0;
-    for (int bit = 31 - __builtin_clz(chunks | 1); bit >= 0; --bit) {
+    for (bit = 31 - __builtin_clz(chunks | 1); bit >= 0; --bit) {
       const int cand = lim | (1 << bit);
       int n = 0;
 #pragma unroll
@@ -89,12 +99,52 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
   if (l == 0) { L.thr = t; L.thr_at = lim; }
 }
 
+// Many more candidates than places (rows with fewer chunks than places, ties): the first wave raises the bound to a key
+// that k to k + k / 8 of the n candidates reach (keys are distinct), and those go to picked.  -> how many.
+template <int NT>
+SCM_DEV int top_thin_out(TopLds<NT>& L, int n, int k) {
+  constexpr int R = TopLds<NT>::CAP / 64;
+  const int l = threadIdx.x & 63;
+  __syncthreads();
+  if (threadIdx.x == 0) L.count = 0;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    uint64_t c[R], lo = ~0ull, hi = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      c[r] = r * 64 + l < n ? L.cand[r * 64 + l] : 0;
+      if (c[r]) { lo = c[r] < lo ? c[r] : lo; hi = c[r] > hi ? c[r] : hi; }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t x = shfl64(lo, o), y = shfl64(hi, o);
+      lo = x < lo ? x : lo;
+      hi = y > hi ? y : hi;
+    }
+    int bit = 63 - __builtin_clzll((lo ^ hi) | 1), reach = n;
+    uint64_t t = bit >= 63 ? 0 : (hi >> (bit + 1)) << (bit + 1);
+    for (; bit >= 0 && reach > k + k / 8; --bit) {
+      const uint64_t cand = t | (1ull << bit);
+      int m = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r * 64 < n) m += __builtin_popcountll(__builtin_amdgcn_ballot_w64(c[r] >= cand));
+      if (m >= k) { t = cand; reach = m; }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (c[r] && c[r] >= t) L.picked[atomicAdd(&L.count, 1)] = c[r];   // reach of them: all bits used, it is k
+  }
+  __syncthreads();
+  return L.count;
+}
+
 // Calls emit(rank, key) for the k largest keys of the segment, each from one thread.  best, at: the thread's maximum
 // (0: no elements) and the first of its chunks that holds it.  odd: the segment holds NaN or +inf (or may: then the
 // threads' maxima are not to be used).
-template <typename T, int NT, typename Emit>
-SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, int at, bool odd, TopLds<NT>& L, Emit emit) {
-  constexpr int E = Walk<T, NT>::E, U = Walk<T, NT>::U, SPARE = order_spare<T>;
+template <typename W, typename T, int NT, typename Emit>
+SCM_DEV void top_of_segment(const W& w, int lo, int k, uint32_t best, int at, bool odd, TopLds<NT>& L, Emit emit) {
+  constexpr int E = W::E, U = W::U, SPARE = order_spare<T>;
   const int tid = threadIdx.x;
   const int chunks = (w.len + E - 1) / E;
   L.best[tid] = best;
@@ -125,13 +175,18 @@ SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, 
     }
   }
   __syncthreads();
-  const int n = L.count;
+  int n = L.count;
   if (!odd && n <= TopLds<NT>::CAP) {
+    const uint64_t* list = L.cand;
+    if (n > 128 && n > k + k / 8) {   // ranking reads n keys per candidate
+      n = top_thin_out<NT>(L, n, k);
+      list = L.picked;
+    }
     for (int i = tid; i < n; i += NT) {
-      const uint64_t mine = L.cand[i];
+      const uint64_t mine = list[i];
       int rank = 0;
 #pragma unroll 8
-      for (int j = 0; j < n; ++j) rank += L.cand[j] > mine;
+      for (int j = 0; j < n; ++j) rank += list[j] > mine;
       if (rank < k) emit(rank, mine);
     }
     return;
@@ -143,7 +198,7 @@ SCM_DEV void top_of_segment(const Walk<T, NT>& w, int lo, int k, uint32_t best, 
   for (int r = 0; r < found; ++r) {
     uint64_t mine = 0;
     for (int s = 0; s < w.steps(); ++s) {
-      typename Walk<T, NT>::Raw raw;
+      typename W::Raw raw;
       w.load(s, raw);
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -189,11 +244,11 @@ SCM_DEV void write_row(const ScoreArgs& a, long row, const Stat& st, float x_tar
   if (a.tape) { a.tape[2 * row] = st.m; a.tape[2 * row + 1] = st.s; }
 }
 
-template <typename T, int NT, bool ENT, bool TOP>
+template <typename T, int NT, int EL, bool ENT, bool TOP>
 __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_len) {
   __shared__ Stat red[NT / 64];
   __shared__ TopLds<TOP ? NT : 64> top;
-  typedef Walk<T, NT> W;
+  typedef Walk<T, NT, EL> W;
   const long row = blockIdx.x / S;
   const int seg = blockIdx.x % S, lo = seg * seg_len;
   const W w{(const T*)a.x + row * a.ldx + lo, min(a.V - lo, seg_len)};
@@ -209,7 +264,7 @@ __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_l
   float best = -INFINITY;
   int at = threadIdx.x;
   w.run([&](int s, const typename W::Raw& raw) {
-    float v[32], bm = LOWEST;
+    float v[EL], bm = LOWEST;
     w.values(s, raw, v);
 #pragma unroll
     for (int u = 0; u < W::U; ++u) {
@@ -232,7 +287,7 @@ __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_l
     if constexpr (TOP) {
       uint64_t* out = a.part_top + slot * a.k;
       for (int i = w.len + threadIdx.x; i < a.k; i += NT) out[i] = 0;   // a segment shorter than k
-      top_of_segment<T, NT>(w, lo, a.k, (int)threadIdx.x * W::E < w.len ? ordered(best) : 0u, at, odd, top,
+      top_of_segment<W, T, NT>(w, lo, a.k, (int)threadIdx.x * W::E < w.len ? ordered(best) : 0u, at, odd, top,
                             [&](int rank, uint64_t key) { out[rank] = key; });
     }
     return;
@@ -240,7 +295,7 @@ __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a, int S, int seg_l
   if (writer) write_row<ENT>(a, row, st, x_target, target);
   if constexpr (TOP) {
     const RowScore r(st, a.inv_t);
-    top_of_segment<T, NT>(w, 0, a.k, (int)threadIdx.x * W::E < w.len ? ordered(best) : 0u, at, odd, top,
+    top_of_segment<W, T, NT>(w, 0, a.k, (int)threadIdx.x * W::E < w.len ? ordered(best) : 0u, at, odd, top,
                           [&](int rank, uint64_t key) {
                             a.top_index[row * a.k + rank] = key_index(key);
                             a.top_logprob[row * a.k + rank] = r.logp(key_value(key));
@@ -441,13 +496,13 @@ static int segment_length(int V, int S) { return ((V + S - 1) / S + 31) / 32 * 3
 // segments that really hold elements once the length is rounded
 static int segments_used(int V, int len) { return (V + len - 1) / len; }
 
-template <typename T, int NT>
+template <typename T, int NT, int EL = 32>
 static void launch_score(const ScoreArgs& a, int S, int len, hipStream_t s) {
   const dim3 g((unsigned)(a.T * S)), b(NT);
-  if (a.entropy && a.k) hipLaunchKernelGGL((score_kernel<T, NT, true, true>), g, b, 0, s, a, S, len);
-  else if (a.entropy) hipLaunchKernelGGL((score_kernel<T, NT, true, false>), g, b, 0, s, a, S, len);
-  else if (a.k) hipLaunchKernelGGL((score_kernel<T, NT, false, true>), g, b, 0, s, a, S, len);
-  else hipLaunchKernelGGL((score_kernel<T, NT, false, false>), g, b, 0, s, a, S, len);
+  if (a.entropy && a.k) hipLaunchKernelGGL((score_kernel<T, NT, EL, true, true>), g, b, 0, s, a, S, len);
+  else if (a.entropy) hipLaunchKernelGGL((score_kernel<T, NT, EL, true, false>), g, b, 0, s, a, S, len);
+  else if (a.k) hipLaunchKernelGGL((score_kernel<T, NT, EL, false, true>), g, b, 0, s, a, S, len);
+  else hipLaunchKernelGGL((score_kernel<T, NT, EL, false, false>), g, b, 0, s, a, S, len);
 }
 template <typename T>
 static void score_typed(const ScoreArgs& a, hipStream_t s) {
@@ -457,15 +512,25 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((score_small_kernel<T, false>), g, dim3(64), 0, s, a);
     return;
   }
-  if (a.V <= 2048) return launch_score<T, 64>(a, 1, a.V, s);
   int S = score_segments(a.T, a.V, a.k);
-  const int len = S > 1 ? segment_length(a.V, S) : a.V;
-  S = S > 1 ? segments_used(a.V, len) : 1;
-  launch_score<T, 256>(a, S, len, s);
   if (S > 1) {
+    const int len = segment_length(a.V, S);
+    S = segments_used(a.V, len);
+    launch_score<T, 256>(a, S, len, s);
     if (a.entropy) hipLaunchKernelGGL((score_join_kernel<T, true>), dim3((unsigned)a.T), dim3(256), 0, s, a, S);
     else hipLaunchKernelGGL((score_join_kernel<T, false>), dim3((unsigned)a.T), dim3(256), 0, s, a, S);
+    return;
   }
+  // Threads per row by the row's bytes: more of them shorten the walk, fewer the reductions and the search for the
+  // alternatives behind it, and leave more rows in flight; and at least two threads per alternative, so that the threads'
+  // maxima bound them well.  bf16, k = 8: 20000 x 4000 62 us on 64 threads, 81 on 128; 6000 x 16000 58 on 128, 65 on 64, 68
+  // on 256; 2048 x 65536 62 on 256, 68 on 128 and on 512; 1200 x 131072 72 on 512, 79 on 256.
+  const long bytes = (long)a.V * sizeof(T);
+  if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8>(a, 1, a.V, s);
+  if (bytes <= 16384 && a.k <= 32) return launch_score<T, 64>(a, 1, a.V, s);
+  if (bytes <= 49152) return launch_score<T, 128>(a, 1, a.V, s);
+  if (bytes <= 196608) return launch_score<T, 256>(a, 1, a.V, s);
+  launch_score<T, 512>(a, 1, a.V, s);
 }
 template <typename T, bool STREAM>
 static void score_bwd_typed(const ScoreGradArgs& a, hipStream_t s) {

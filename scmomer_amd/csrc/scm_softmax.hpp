@@ -51,11 +51,11 @@ SCM_DEV Stat stat_block(Stat v, float c, Stat* red) {
   return r;
 }
 
-// Per-thread view of a segment [lo, lo + len) of a row, in steps of 32 elements (U chunks) a thread: chunk u of step s is
+// Per-thread view of a segment [lo, lo + len) of a row, in steps of EL elements (U chunks) a thread: chunk u of step s is
 // chunk (s U + u) NT + tid of the segment.
-template <typename T, int NT>
+template <typename T, int NT, int EL_ = 32>
 struct Walk {
-  static constexpr int E = 16 / sizeof(T), U = 32 / E, STEP = NT * U * E;
+  static constexpr int EL = EL_, E = 16 / sizeof(T), U = EL / E, STEP = NT * EL;
   typedef Chunk<T, E> Raw[U];
   const T* p;
   int len;
@@ -86,7 +86,7 @@ struct Walk {
     }
   }
   // the elements of a step as f32, -inf past the end
-  SCM_DEV void values(int step, const Raw& raw, float (&v)[32]) const {
+  SCM_DEV void values(int step, const Raw& raw, float (&v)[EL]) const {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -112,14 +112,14 @@ SCM_DEV void stay_packed(Chunk<T, E>& c) {
   c = __builtin_bit_cast(Chunk<T, E>, w);
 }
 
-// Adds 32 elements to a thread's running statistics.
-template <bool ENT>
-SCM_DEV void stat_add(Stat& st, const float (&v)[32], float bm, float c) {
+// Adds EL elements, their maximum bm, to a thread's running statistics.
+template <bool ENT, int EL>
+SCM_DEV void stat_add(Stat& st, const float (&v)[EL], float bm, float c) {
   const float m = fmaxf(st.m, bm);
   const float d0 = grown(st.m, m, c), f = exp2_fast(d0);
   float s = st.s * f, h = ENT ? f * (st.h + d0 * st.s) : 0.f;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
+  for (int j = 0; j < EL; ++j) {
     const float d = (v[j] - m) * c, e = exp2_fast(d);
     s += e;
     if constexpr (ENT) h += e * fmaxf(d, -200.f);

@@ -23,36 +23,48 @@ struct DistillRow {
   float loss, m, cr;   // the loss; reference maximum and factor of the gradient in R
   float g;             // lane j: gradient at its named token
 };
+template <int CTRL>
+SCM_DEV double dpp_move_f64(double v) {
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xF, 0xF, true),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, true));
+}
 SCM_DEV double wave_sum_f64(double v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  v += dpp_move_f64<0xB1>(v);
+  v += dpp_move_f64<0x4E>(v);
+  v += dpp_move_f64<0x141>(v);
+  v += dpp_move_f64<0x140>(v);
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
   return v;
 }
-// rest: statistics over R.  idx (< 0: unused), lp, x (the student's logit there) of this lane's entry.
-SCM_DEV DistillRow distill_row(const DistillTopkArgs& a, const Stat& rest, long long idx, float lp, float x) {
+// rest: statistics over R.  idx (-1: unused), lp, x (the student's logit there) of this lane's entry.  beyond: some index
+// lies outside the vocabulary (such entries come as unused).  twice: some token may be named more than once.
+SCM_DEV DistillRow distill_row(const DistillTopkArgs& a, const Stat& rest, int idx, float lp, float x, bool beyond, bool twice) {
   const int lane = threadIdx.x & 63;
   const bool used = idx >= 0;
-  const bool beyond = __builtin_amdgcn_ballot_w64(used && idx >= a.V) != 0;
-  // the first of equal indices, and the sum of q over them
   double q = used ? exp((double)lp) : 0.0;
   const double total = wave_sum_f64(q);
-  float r = 0.f;
+  float r = 0.f, big_a;
   if (a.tail) {
     r = rest.s == 0.f ? 0.f : (float)fmax(0.0, 1.0 - total);
-    if (total != total) r = (float)total;
-  } else if (total > 0.0) {
-    q /= total;
-    lp -= (float)log(total);
+    big_a = (float)total + r;
+  } else {
+    big_a = total > 0.0 ? 1.f : 0.f;
+    if (total > 0.0) { q /= total; lp -= (float)log(total); }
   }
   const float qf = (float)q;
-  float qsum = 0.f;
+  // the first of equal indices, and the sum of q over them
+  float qsum = qf;
   bool first = used;
-  for (int j = 0; j < a.k; ++j) {
-    const long long ij = __shfl(idx, j);
-    const float qj = __shfl(qf, j);
-    if (used && ij == idx) {
-      qsum += qj;
-      if (j < lane) first = false;
+  if (twice) {
+    qsum = 0.f;
+    for (int j = 0; j < a.k; ++j) {
+      const int ij = __builtin_amdgcn_readlane(idx, j);
+      const float qj = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(qf), j));
+      if (used && ij == idx) {
+        qsum += qj;
+        if (j < lane) first = false;
+      }
     }
   }
   // all tokens: R and the named ones
@@ -64,7 +76,6 @@ SCM_DEV DistillRow distill_row(const DistillTopkArgs& a, const Stat& rest, long 
   const float logp = (x - m) * a.inv_t - LN2 * l2;
   float loss = wave_sum(used && qf > 0.f ? qf * (lp - logp) : 0.f);
   if (r > 0.f) loss += r * (logf(r) - ((rest.m - m) * a.inv_t + LN2 * (log2_fast(rest.s) - l2)));
-  const float big_a = (float)wave_sum_f64(q) + r;
   DistillRow o;
   o.loss = loss;
   o.m = rest.m;
@@ -74,6 +85,21 @@ SCM_DEV DistillRow distill_row(const DistillTopkArgs& a, const Stat& rest, long 
   if (beyond || total != total || rest.s != rest.s || z != z) o.loss = o.cr = o.g = __uint_as_float(0x7FC00000u);
   return o;
 }
+// Entry j of a row, in lane j of a wave: index (-1 where it is not used or lies outside), log probability, logit.
+struct Entry { int idx; float lp, x; bool beyond; };
+template <typename T>
+SCM_DEV Entry load_entry(const DistillTopkArgs& a, long row, const T* x) {
+  const int j = threadIdx.x & 63;
+  Entry e{-1, 0.f, 0.f, false};
+  if (j < a.k) {
+    const long long i = a.index[row * a.k + j];
+    e.lp = a.lp[row * a.k + j];
+    e.beyond = i >= a.V;
+    if (i >= 0 && i < a.V) { e.idx = (int)i; e.x = (float)x[i]; }
+  }
+  return e;
+}
+SCM_DEV bool any_lane(bool b) { return __builtin_amdgcn_ballot_w64(b) != 0; }
 // weight of a row, and what its gradient is scaled by
 SCM_DEV float row_scale(const DistillTopkArgs& a, long row, float w) {
   const float g = a.gloss ? a.gloss[a.gloss_rows ? row : 0] : a.scale;
@@ -81,28 +107,29 @@ SCM_DEV float row_scale(const DistillTopkArgs& a, long row, float w) {
 }
 
 // ---------------------------------------------------------------- statistics over R of a segment
-template <int NT>
-struct NamedBits {
-  static constexpr int WORDS = NT == 64 ? 2048 / 32 : DISTILL_SEGMENT / 32;
-  uint32_t w[WORDS];
-};
-// Marks the named tokens of [lo, lo + len).  Ends with a barrier.
-template <int NT>
-SCM_DEV void mark_named(NamedBits<NT>& bits, const int64_t* idx, int k, int lo, int len) {
+// A bit per token of a segment of at most 32 WORDS tokens.
+template <int WORDS>
+struct NamedBits { uint32_t w[WORDS]; };
+// Marks the entries (lane j of the first wave: entry j) that lie in [lo, lo + len).  -> in the first wave: some token is
+// named twice.  Begins after and ends with a barrier.
+template <int NT, int WORDS>
+SCM_DEV bool mark_named(NamedBits<WORDS>& bits, const Entry& e, int lo, int len) {
   for (int i = threadIdx.x; i < (len + 31) / 32; i += NT) bits.w[i] = 0;
   __syncthreads();
-  if ((int)threadIdx.x < k) {
-    const long long i = idx[threadIdx.x] - lo;
-    if (i >= 0 && i < len) atomicOr(&bits.w[i >> 5], 1u << (i & 31));
+  bool again = false;
+  if (threadIdx.x < 64) {
+    const int i = e.idx - lo;
+    if (e.idx >= 0 && i >= 0 && i < len) again = (atomicOr(&bits.w[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1;
+    again = any_lane(again);
   }
   __syncthreads();
+  return again;
 }
-template <typename T, int NT>
-SCM_DEV Stat rest_of_segment(const Walk<T, NT>& w, const NamedBits<NT>& bits, float c) {
-  typedef Walk<T, NT> W;
+template <typename W, int WORDS>
+SCM_DEV Stat rest_of_segment(const W& w, const NamedBits<WORDS>& bits, float c) {
   Stat st = stat_none();
   w.run([&](int s, const typename W::Raw& raw) {
-    float v[32], bm = LOWEST;
+    float v[W::EL], bm = LOWEST;
     w.values(s, raw, v);
 #pragma unroll
     for (int u = 0; u < W::U; ++u) {
@@ -116,7 +143,7 @@ SCM_DEV Stat rest_of_segment(const Walk<T, NT>& w, const NamedBits<NT>& bits, fl
       }
     }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) bm = fmaxf(bm, v[j]);
+    for (int j = 0; j < W::EL; ++j) bm = fmaxf(bm, v[j]);
     stat_add<false>(st, v, bm, c);
   });
   return st;
@@ -144,69 +171,66 @@ SCM_DEV void zero_write(T* dx, int len) {
 }
 
 // ---------------------------------------------------------------- V > 64
+SCM_DEV void write_tape(const DistillTopkArgs& a, long row, float m, float cr, float g) {   // by a wave
+  if (!a.tape) return;
+  const int j = threadIdx.x & 63;
+  if (j == 0) { a.tape[2 * row] = m; a.tape[2 * row + 1] = cr; }
+  if (j < a.k) a.g_top[row * a.k + j] = g;
+}
+
 // GRAD: loss and gradient in one launch (S = 1).  Otherwise the loss, and (tape, g_top given) what the backward reads;
 // with S > 1 the segment's statistics go to part for distill_join_kernel.
-template <typename T, int NT, bool GRAD, bool STREAM = false>
+template <typename T, int NT, int EL, int WORDS, bool GRAD, bool STREAM = false>
 __global__ __launch_bounds__(NT) void distill_kernel(DistillTopkArgs a, int S, int seg_len) {
   __shared__ Stat red[NT / 64];
-  __shared__ NamedBits<NT> bits;
+  __shared__ NamedBits<WORDS> bits;
   __shared__ float row_m, row_cr;
   const long row = blockIdx.x / S;
   const int seg = blockIdx.x % S, lo = seg * seg_len, tid = threadIdx.x;
   const T* x = (const T*)a.x + row * a.ldx;
-  const Walk<T, NT> w{x + lo, min(a.V - lo, seg_len)};
+  const Walk<T, NT, EL> w{x + lo, min(a.V - lo, seg_len)};
   T* dx = GRAD ? (T*)a.dx + row * a.V : nullptr;
   const float wt = a.weight ? a.weight[row] : 1.f;
   if (wt == 0.f) {
     if constexpr (GRAD) zero_write<T, NT>(dx, a.V);
-    if (S == 1) {
+    if (S == 1 && tid < 64) {
       if (tid == 0) a.row_loss[row] = 0.f;
-      if (a.tape && tid < a.k) a.g_top[row * a.k + tid] = 0.f;
-      if (a.tape && tid == 0) a.tape[2 * row] = a.tape[2 * row + 1] = 0.f;
+      write_tape(a, row, 0.f, 0.f, 0.f);
     }
     return;
   }
-  const int64_t* index = a.index + row * a.k;
-  mark_named<NT>(bits, index, a.k, lo, w.len);
-  const Stat st = stat_block<false, NT>(rest_of_segment<T, NT>(w, bits, a.c), a.c, red);
+  Entry en{-1, 0.f, 0.f, false};
+  if (tid < 64) en = load_entry(a, row, x);
+  const bool twice = mark_named<NT>(bits, en, lo, w.len);
+  const Stat st = stat_block<false, NT>(rest_of_segment(w, bits, a.c), a.c, red);
   if (S > 1) {
     if (tid == 0) { a.part[2 * (row * S + seg)] = st.m; a.part[2 * (row * S + seg) + 1] = st.s; }
     return;
   }
-  long long idx = -1;
   float g = 0.f;
   if (tid < 64) {
-    float lp = 0.f, xi = 0.f;
-    if (tid < a.k) {
-      idx = index[tid];
-      lp = a.lp[row * a.k + tid];
-      if (idx >= 0 && idx < a.V) xi = (float)x[idx];
-    }
-    const DistillRow r = distill_row(a, st, idx, lp, xi);
+    const DistillRow r = distill_row(a, st, en.idx, en.lp, en.x, any_lane(en.beyond), twice);
     g = r.g;
     if (tid == 0) { a.row_loss[row] = wt * r.loss; row_m = r.m; row_cr = r.cr; }
-    if (a.tape) {
-      if (tid == 0) { a.tape[2 * row] = r.m; a.tape[2 * row + 1] = r.cr; }
-      if (tid < a.k) a.g_top[row * a.k + tid] = g;
-    }
+    write_tape(a, row, r.m, r.cr, g);
   }
   if constexpr (GRAD) {
     __syncthreads();
     const float sc = row_scale(a, row, wt);
-    distill_write<T, NT, STREAM>(w, dx, 0, row_m, row_cr * sc, a.c);
+    distill_write<T, NT, STREAM>(Walk<T, NT>{x, a.V}, dx, 0, row_m, row_cr * sc, a.c);
     __syncthreads();   // the last store to a named token is this one; equal indices hold equal values
-    if (tid < a.k && idx >= 0 && idx < a.V) dx[idx] = (T)(g * sc);
+    if (en.idx >= 0) dx[en.idx] = (T)(g * sc);
   }
 }
 
-// Loss and gradient of a row that stays in registers between its one read and its one write: STEPS x 32 elements a thread
+// Loss and gradient of a row that stays in registers between its one read and its one write: STEPS x EL elements a thread
 // (at most 64 registers).
-template <typename T, int NT, int STEPS, bool STREAM>
+template <typename T, int NT, int STEPS, bool STREAM, int EL = 32>
 __global__ __launch_bounds__(NT) void distill_resident_kernel(DistillTopkArgs a) {
   __shared__ Stat red[NT / 64];
-  __shared__ uint32_t bits[STEPS * NT];   // STEPS NT 32 tokens
+  __shared__ NamedBits<STEPS * NT * EL / 32> bits;
   __shared__ float row_m, row_cr;
-  typedef Walk<T, NT> W;
+  typedef Walk<T, NT, EL> W;
   constexpr int E = W::E, U = W::U;
   const long row = blockIdx.x;
   const int tid = threadIdx.x;
@@ -221,19 +245,9 @@ __global__ __launch_bounds__(NT) void distill_resident_kernel(DistillTopkArgs a)
   typename W::Raw raw[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) w.load(s, raw[s]);
-  // entries (first wave) and the bits of the named tokens
-  long long idx = -1;
-  float lp = 0.f, xi = 0.f;
-  if (tid < a.k) {
-    idx = a.index[row * a.k + tid];
-    lp = a.lp[row * a.k + tid];
-    if (idx >= 0 && idx < a.V) xi = (float)w.p[idx];
-  }
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s) bits[s * NT + tid] = 0;
-  __syncthreads();
-  if (tid < a.k && idx >= 0 && idx < a.V) atomicOr(&bits[idx >> 5], 1u << (idx & 31));
-  __syncthreads();
+  Entry en{-1, 0.f, 0.f, false};
+  if (tid < 64) en = load_entry(a, row, w.p);
+  const bool twice = mark_named<NT>(bits, en, 0, STEPS * NT * EL);
   // the maximum over R first, then one exponential per element around it; named tokens and what lies past the end
   // become -inf in the registers
   Stat st = stat_none();
@@ -242,7 +256,7 @@ __global__ __launch_bounds__(NT) void distill_resident_kernel(DistillTopkArgs a)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i0 = w.first(s, u), n = a.V - i0;
-      const uint32_t named = (bits[i0 >> 5] >> (i0 & 31)) & ((1u << E) - 1u);
+      const uint32_t named = (bits.w[i0 >> 5] >> (i0 & 31)) & ((1u << E) - 1u);
       if (named || n < E) {
 #pragma unroll
         for (int j = 0; j < E; ++j)
@@ -263,7 +277,7 @@ __global__ __launch_bounds__(NT) void distill_resident_kernel(DistillTopkArgs a)
   st = stat_block<false, NT>(st, a.c, red);
   float g = 0.f;
   if (tid < 64) {
-    const DistillRow r = distill_row(a, st, idx, lp, xi);
+    const DistillRow r = distill_row(a, st, en.idx, en.lp, en.x, any_lane(en.beyond), twice);
     g = r.g;
     if (tid == 0) { a.row_loss[row] = wt * r.loss; row_m = r.m; row_cr = r.cr; }
   }
@@ -279,7 +293,7 @@ __global__ __launch_bounds__(NT) void distill_resident_kernel(DistillTopkArgs a)
       store_chunk<T, E, STREAM>(dx + w.first(s, u), o, a.V - w.first(s, u));
     }
   __syncthreads();   // the last store to a named token is this one; equal indices hold equal values
-  if (tid < a.k && idx >= 0 && idx < a.V) dx[idx] = (T)(g * sc);
+  if (en.idx >= 0) dx[en.idx] = (T)(g * sc);
 }
 
 template <typename T>
@@ -289,27 +303,17 @@ __global__ __launch_bounds__(64) void distill_join_kernel(DistillTopkArgs a, int
   const float wt = a.weight ? a.weight[row] : 1.f;
   if (wt == 0.f) {
     if (tid == 0) a.row_loss[row] = 0.f;
-    if (a.tape && tid < a.k) a.g_top[row * a.k + tid] = 0.f;
-    if (a.tape && tid == 0) a.tape[2 * row] = a.tape[2 * row + 1] = 0.f;
+    write_tape(a, row, 0.f, 0.f, 0.f);
     return;
   }
+  const Entry en = load_entry(a, row, (const T*)a.x + row * a.ldx);
   Stat st = stat_none();
   for (int i = tid; i < S; i += 64)
     st = stat_join<false>(st, Stat{a.part[2 * (row * S + i)], a.part[2 * (row * S + i) + 1], 0.f}, a.c);
   st = stat_wave<false>(st, a.c);
-  long long idx = -1;
-  float lp = 0.f, xi = 0.f;
-  if (tid < a.k) {
-    idx = a.index[row * a.k + tid];
-    lp = a.lp[row * a.k + tid];
-    if (idx >= 0 && idx < a.V) xi = (float)((const T*)a.x)[row * a.ldx + idx];
-  }
-  const DistillRow r = distill_row(a, st, idx, lp, xi);
+  const DistillRow r = distill_row(a, st, en.idx, en.lp, en.x, any_lane(en.beyond), true);
   if (tid == 0) a.row_loss[row] = wt * r.loss;
-  if (a.tape) {
-    if (tid == 0) { a.tape[2 * row] = r.m; a.tape[2 * row + 1] = r.cr; }
-    if (tid < a.k) a.g_top[row * a.k + tid] = r.g;
-  }
+  write_tape(a, row, r.m, r.cr, r.g);
 }
 
 template <typename T, int NT, bool STREAM>
@@ -450,7 +454,9 @@ template <typename T, bool STREAM>
 static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
   constexpr int MAX = 64 / (32 * (int)sizeof(T) / 4);   // steps in 64 registers: 4 for 2-byte types, 2 for f32
   const dim3 g((unsigned)a.T);
-  if (a.V <= 64 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM>), g, dim3(64), 0, s, a);
+  if (a.V <= 64 * 8) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM, 8>), g, dim3(64), 0, s, a);
+  else if (a.V <= 64 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM>), g, dim3(64), 0, s, a);
+  else if (a.V <= 64 * 64) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 2, STREAM>), g, dim3(64), 0, s, a);
   else if (a.V <= 256 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM>), g, dim3(256), 0, s, a);
   else if (a.V <= 256 * 64) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 2, STREAM>), g, dim3(256), 0, s, a);
   else if (a.V <= 256 * 32 * MAX) hipLaunchKernelGGL((distill_resident_kernel<T, 256, MAX, STREAM>), g, dim3(256), 0, s, a);
@@ -472,17 +478,22 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
     a.tape = a.g_top = nullptr;   // for a backward of its own only
     // (512 threads: two workgroups per CU, whose rows fit the last-level cache together; 256: 2048 x 131072 364 us, 512: 334 us)
     if (!launch_resident<T, STREAM>(a, s))
-      hipLaunchKernelGGL((distill_kernel<T, 512, true, STREAM>), dim3((unsigned)a.T), dim3(512), 0, s, a, 1, a.V);
+      hipLaunchKernelGGL((distill_kernel<T, 512, 32, DISTILL_SEGMENT / 32, true, STREAM>), dim3((unsigned)a.T), dim3(512), 0, s, a, 1, a.V);
     return;
   }
   if (loss) {
-    if (a.V <= 2048) {
-      hipLaunchKernelGGL((distill_kernel<T, 64, false>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
-    } else {
-      const int len = S > 1 ? seg_len_of(a.V, S) : a.V;
+    const dim3 g((unsigned)a.T);
+    if (S > 1) {
+      const int len = seg_len_of(a.V, S);
       S = (a.V + len - 1) / len;
-      hipLaunchKernelGGL((distill_kernel<T, 256, false>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
-      if (S > 1) hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)a.T), dim3(64), 0, s, a, S);
+      hipLaunchKernelGGL((distill_kernel<T, 256, 32, DISTILL_SEGMENT / 32, false>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
+      hipLaunchKernelGGL((distill_join_kernel<T>), g, dim3(64), 0, s, a, S);
+    } else if (a.V <= 512) {
+      hipLaunchKernelGGL((distill_kernel<T, 64, 8, 16, false>), g, dim3(64), 0, s, a, 1, a.V);
+    } else if (a.V <= 8192) {   // one wave: 20000 x 4000 bf16 52 us, 256 threads 95 us; 10000 x 8000 45 and 55 us
+      hipLaunchKernelGGL((distill_kernel<T, 64, 32, 256, false>), g, dim3(64), 0, s, a, 1, a.V);
+    } else {
+      hipLaunchKernelGGL((distill_kernel<T, 256, 32, DISTILL_SEGMENT / 32, false>), g, dim3(256), 0, s, a, 1, a.V);
     }
   }
   if (grad) {
