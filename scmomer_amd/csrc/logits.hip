@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a, int S) {
 // ---------------------------------------------------------------- rows of at most 64 logits, one thread each
 template <typename T, bool ENT>
 __global__ __launch_bounds__(64) void score_small_kernel(ScoreArgs a) {
-  __shared__ uint32_t lds[64 * 65];
+  extern __shared__ uint32_t lds[];
   const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
   const long row = (long)blockIdx.x * 64 + threadIdx.x;
   stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, i
 
 template <typename T>
 __global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
-  __shared__ uint32_t lds[64 * 65];
+  extern __shared__ uint32_t lds[];
   const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
   const long row = (long)blockIdx.x * 64 + threadIdx.x;
   stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
@@ -508,8 +508,8 @@ template <typename T>
 static void score_typed(const ScoreArgs& a, hipStream_t s) {
   if (a.V <= 64) {
     const dim3 g((unsigned)((a.T + 63) / 64));
-    if (a.entropy) hipLaunchKernelGGL((score_small_kernel<T, true>), g, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((score_small_kernel<T, false>), g, dim3(64), 0, s, a);
+    if (a.entropy) hipLaunchKernelGGL((score_small_kernel<T, true>), g, dim3(64), small_lds(a.V), s, a);
+    else hipLaunchKernelGGL((score_small_kernel<T, false>), g, dim3(64), small_lds(a.V), s, a);
     return;
   }
   int S = score_segments(a.T, a.V, a.k);
@@ -535,7 +535,7 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
 template <typename T, bool STREAM>
 static void score_bwd_typed(const ScoreGradArgs& a, hipStream_t s) {
   if (a.V <= 64) {
-    hipLaunchKernelGGL((score_bwd_small_kernel<T>), dim3((unsigned)((a.T + 63) / 64)), dim3(64), 0, s, a);
+    hipLaunchKernelGGL((score_bwd_small_kernel<T>), dim3((unsigned)((a.T + 63) / 64)), dim3(64), small_lds(a.V), s, a);
   } else if (a.V <= 2048) {
     hipLaunchKernelGGL((score_bwd_kernel<T, 64, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
   } else {

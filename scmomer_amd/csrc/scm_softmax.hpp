@@ -129,6 +129,7 @@ SCM_DEV void stat_add(Stat& st, const float (&v)[EL], float bm, float c) {
 
 // Rows of at most 64 logits, one thread each: 64 rows go through LDS (row stride odd: no bank conflicts along a
 // column) as f32 bits, read and written along memory.
+constexpr unsigned small_lds(int V) { return 64 * (V | 1) * 4; }
 template <typename T, bool STORE>
 SCM_DEV void stage_rows(T* p, long ld, int rows, int V, uint32_t* lds, int pitch) {
   const int dr = 64 / V, dc = 64 % V;

@@ -336,7 +336,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillTopkArgs a, int 
 // ---------------------------------------------------------------- V <= 64: a thread per row, a bit per token
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
-  __shared__ uint32_t lds[64 * 65];
+  extern __shared__ uint32_t lds[];
   const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
   const long row = (long)blockIdx.x * 64 + threadIdx.x;
   stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
@@ -469,8 +469,8 @@ template <typename T, bool STREAM>
 static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s) {
   if (a.V <= 64) {
     const dim3 g((unsigned)((a.T + 63) / 64));
-    if (grad) hipLaunchKernelGGL((distill_small_kernel<T, true>), g, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((distill_small_kernel<T, false>), g, dim3(64), 0, s, a);
+    if (grad) hipLaunchKernelGGL((distill_small_kernel<T, true>), g, dim3(64), small_lds(a.V), s, a);
+    else hipLaunchKernelGGL((distill_small_kernel<T, false>), g, dim3(64), small_lds(a.V), s, a);
     return;
   }
   int S = distill_segments(a.T, a.V);

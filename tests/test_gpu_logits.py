@@ -86,7 +86,8 @@ def _logits(t, v, dtype, seed, scale=3.0):
 
 SIZES = [(1, 1, 1), (70, 2, 2), (129, 7, 3), (64, 64, 64), (65, 33, 20), (63, 64, 1), (5, 65, 64), (9, 100, 5), (600, 1000, 20),
          (3, 2047, 64), (3, 2048, 7), (700, 2049, 33), (2, 8192, 64), (1, 8193, 64), (520, 8200, 8), (3, 50001, 20),
-         (1, 131072, 64), (40, 16906, 5), (513, 20000, 0), (2, 300007, 50)]
+         (1, 131072, 64), (40, 16906, 5), (513, 20000, 0), (2, 300007, 50), (40, 300, 64), (33, 512, 33), (12, 513, 64),
+         (600, 5000, 64), (520, 9000, 64), (515, 30000, 33), (514, 100000, 40)]
 
 
 @pytest.mark.parametrize("t,v,k", SIZES)
@@ -281,9 +282,9 @@ def test_results_repeat_capture_and_streams(token_logprobs):
             g, = torch.autograd.grad((o.logprob, o.entropy), z, (gl, gh))
             return [a.detach() for a in o] + [g]
         want = both(x)
-        side = torch.cuda.Stream()
-        side.wait_stream(torch.cuda.current_stream())
         xs = x.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())      # after the copy that the other stream reads
         with torch.cuda.stream(side):
             got = both(xs)
         torch.cuda.current_stream().wait_stream(side)

@@ -246,9 +246,9 @@ def test_repeats_streams_and_graphs(L):
             g, = torch.autograd.grad(loss, zg)
             return [loss.detach(), g, *L.topk_distillation_grad(z, idx, lp, weight=w, temperature=2.0)]
         want = all_of(x)
-        side = torch.cuda.Stream()
-        side.wait_stream(torch.cuda.current_stream())
         xs = x.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())      # after the copy that the other stream reads
         with torch.cuda.stream(side):
             got = all_of(xs)
         torch.cuda.current_stream().wait_stream(side)
