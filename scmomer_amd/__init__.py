@@ -9,9 +9,12 @@ from .performer import (FastAttention, FeedForward, Gene2VecPositionalEmbedding,
                         PreLayerNorm, SelfAttention, SequentialSequence, gaussian_orthogonal_random_matrix,
                         linear_attention, softmax_kernel)
 
+from .logits import TokenLogprobs, token_logprobs, topk_distillation, topk_distillation_grad  # noqa: E402,F401
+from .norm import layer_norm  # noqa: E402,F401
 from .rna_encoder import Identity  # noqa: E402,F401
 from .scmomer import StudentEncoder, scMomer  # noqa: E402,F401
 
 __all__ = ["Identity", "StudentEncoder", "scMomer", "FastAttention", "FeedForward", "Gene2VecPositionalEmbedding", "Performer", "PerformerLM",
            "PreLayerNorm", "SelfAttention", "SequentialSequence", "gaussian_orthogonal_random_matrix",
-           "linear_attention", "softmax_kernel"]
+           "linear_attention", "softmax_kernel", "layer_norm", "TokenLogprobs", "token_logprobs", "topk_distillation",
+           "topk_distillation_grad"]

@@ -466,7 +466,9 @@ __global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
   __syncthreads();
   if ((int)threadIdx.x < rows) {
     uint32_t* o = lds + threadIdx.x * pitch;
-    auto add = [&](long long i, float v) { o[i] = __float_as_uint(__uint_as_float(o[i]) + v); };
+    auto add = [&](long long i, float v) {
+      if (i >= 0 && i < V) o[i] = __float_as_uint(__uint_as_float(o[i]) + v);
+    };
     const int k = a.g_top ? a.k : 0;
     float gt = 0.f;
     for (int j = 0; j < k; ++j) gt += a.g_top[row * k + j];
