@@ -315,7 +315,7 @@ int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
  *      not read; loss (one float, may be NULL in the forward) = sum of row_loss, divided by the sum of the weights when
  *      mean; wsum (one float, may be NULL): that sum.  The loss is not multiplied by temperature^2.
  *      tape: scm_topk_distill_tape_floats floats (0 for V <= 64), NULL in the forward where no backward follows;
- *      ws: scm_topk_distill_ws_floats floats.
+ *      ws: scm_topk_distill_ws_floats floats, 8-byte aligned.
  *      bwd: dx [T,V] (x's type, contiguous) = gloss[0] (gloss_rows: gloss[t]) * the gradient of the loss (row_loss).
  *      step: loss, and dx = scale * its gradient, without a backward of its own; a row is read from memory once. */
 int64_t scm_topk_distill_tape_floats(int64_t T, int V, int k);

@@ -306,10 +306,12 @@ int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
 int64_t scm_topk_distill_tape_floats(int64_t T, int V, int k) {
   return T > 0 && V > 64 && k > 0 && k <= LOGITS_MAX_K ? T * (2 + (int64_t)k) : 0;
 }
+// [256][2] doubles for the sums over many rows, then the split rows' statistics
+static int64_t distill_sum_floats(int64_t T) { return T > DISTILL_SUM_ROWS ? 2 * 256 * 2 : 0; }
 int64_t scm_topk_distill_ws_floats(int64_t T, int V) {
-  if (T <= 0 || V <= 64) return 0;
-  const int64_t S = distill_segments(T, V);
-  return S > 1 ? 2 * T * S : 0;
+  if (T <= 0 || V <= 0) return 0;
+  const int64_t S = V <= 64 ? 1 : distill_segments(T, V);
+  return distill_sum_floats(T) + (S > 1 ? 2 * T * S : 0);
 }
 static int distill_topk_args(const char* who, DistillTopkArgs& a, const void* x, int type, int64_t ldx, int64_t T, int V,
                              float temperature, const int64_t* index, const float* logprob, int k, int tail,
@@ -331,7 +333,8 @@ int scm_topk_distill_fwd(const void* x, int type, int64_t ldx, int64_t T, int V,
                                 mean, tape)) return e;
   SCM_REQ(row_loss, "scm_topk_distill_fwd: null pointer");
   SCM_REQ(ws || scm_topk_distill_ws_floats(T, V) == 0, "scm_topk_distill_fwd: null workspace");
-  a.row_loss = row_loss; a.part = ws;
+  SCM_REQ(((uintptr_t)ws & 7) == 0, "scm_topk_distill_fwd: workspace must be 8-byte aligned");
+  a.row_loss = row_loss; a.sums = (double*)ws; a.part = ws ? ws + distill_sum_floats(T) : nullptr;
   SCM_HIP(topk_distill_fwd(a, loss, wsum, (hipStream_t)stream), "scm_topk_distill_fwd");
   return 0;
 }
@@ -356,7 +359,8 @@ int scm_topk_distill_step(const void* x, int type, int64_t ldx, int64_t T, int V
   SCM_REQ(row_loss && loss && dx && (tape || V <= 64), "scm_topk_distill_step: null pointer");
   SCM_REQ(!(mean && weight) || wsum, "scm_topk_distill_step: a weighted mean needs room for the weights' sum");
   SCM_REQ(ws || scm_topk_distill_ws_floats(T, V) == 0, "scm_topk_distill_step: null workspace");
-  a.row_loss = row_loss; a.part = ws; a.scale = scale; a.wsum = weight && mean ? wsum : nullptr; a.dx = dx;
+  SCM_REQ(((uintptr_t)ws & 7) == 0, "scm_topk_distill_step: workspace must be 8-byte aligned");
+  a.row_loss = row_loss; a.sums = (double*)ws; a.part = ws ? ws + distill_sum_floats(T) : nullptr; a.scale = scale; a.wsum = weight && mean ? wsum : nullptr; a.dx = dx;
   SCM_HIP(topk_distill_step(a, loss, wsum, (hipStream_t)stream), "scm_topk_distill_step");
   return 0;
 }

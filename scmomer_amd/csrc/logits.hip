@@ -420,10 +420,10 @@ SCM_DEV float score_dx(const ScoreGrad& r, float x, float c) {
   return exp2_fast(d) * (r.ca + r.cb * fmaxf(d, -200.f));
 }
 
-template <typename T, int NT, bool STREAM>
+template <typename T, int NT, int EL, bool STREAM>
 __global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, int seg_len) {
   __shared__ int target_named;
-  typedef Walk<T, NT> W;
+  typedef Walk<T, NT, EL> W;
   const long row = blockIdx.x / S;
   const int lo = (int)(blockIdx.x % S) * seg_len, tid = threadIdx.x;
   const T* x = (const T*)a.x + row * a.ldx;
@@ -529,6 +529,7 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   // on 256; 2048 x 65536 62 on 256, 68 on 128 and on 512; 1200 x 131072 72 on 512, 79 on 256.
   const long bytes = (long)a.V * sizeof(T);
   if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8>(a, 1, a.V, s);
+  if (a.V <= 1024 && a.k <= 32) return launch_score<T, 64, 16>(a, 1, a.V, s);
   if (bytes <= 16384 && a.k <= 32) return launch_score<T, 64>(a, 1, a.V, s);
   if (bytes <= 49152) return launch_score<T, 128>(a, 1, a.V, s);
   if (bytes <= 196608) return launch_score<T, 256>(a, 1, a.V, s);
@@ -538,12 +539,16 @@ template <typename T, bool STREAM>
 static void score_bwd_typed(const ScoreGradArgs& a, hipStream_t s) {
   if (a.V <= 64) {
     hipLaunchKernelGGL((score_bwd_small_kernel<T>), dim3((unsigned)((a.T + 63) / 64)), dim3(64), small_lds(a.V), s, a);
+  } else if (a.V <= 512) {   // one step of one wave
+    hipLaunchKernelGGL((score_bwd_kernel<T, 64, 8, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+  } else if (a.V <= 1024) {
+    hipLaunchKernelGGL((score_bwd_kernel<T, 64, 16, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
   } else if (a.V <= 2048) {
-    hipLaunchKernelGGL((score_bwd_kernel<T, 64, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+    hipLaunchKernelGGL((score_bwd_kernel<T, 64, 32, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
   } else {
     // the gradient of an element needs the row's two coefficients only: segments at will, 8192 elements are one step
     const int len = logits_bwd_segment(a.T, a.V), S = segments_used(a.V, len);
-    hipLaunchKernelGGL((score_bwd_kernel<T, 256, STREAM>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
+    hipLaunchKernelGGL((score_bwd_kernel<T, 256, 32, STREAM>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
   }
 }
 template <typename T>

@@ -212,6 +212,7 @@ int logits_bwd_segment(long T, int V);
 hipError_t score_fwd(const ScoreArgs& a, hipStream_t s);
 hipError_t score_bwd(const ScoreGradArgs& a, hipStream_t s);
 
+constexpr long DISTILL_SUM_ROWS = 16384;  // rows that one workgroup adds up
 struct DistillTopkArgs {
   const void* x; long ldx; int type; long T; int V, k, tail, mean;
   float c, inv_t;
@@ -220,6 +221,7 @@ struct DistillTopkArgs {
   float* row_loss;                                 // [T]
   float* tape; float* g_top;                       // V > 64: [T][2], [T][k], or null
   float* part;                                     // split rows: [T][S][2]
+  double* sums;                                    // T > DISTILL_SUM_ROWS: [256][2]
   const float* wsum; const float* gloss; int gloss_rows; float scale;   // gradient: gloss or scale
   void* dx;
 };

@@ -50,7 +50,7 @@ SCM_DEV DistillRow distill_row(const DistillTopkArgs& a, const Stat& rest, int i
     big_a = (float)total + r;
   } else {
     big_a = total > 0.0 ? 1.f : 0.f;
-    if (total > 0.0) { q /= total; lp -= (float)log(total); }
+    if (total > 0.0) { q *= 1.0 / total; lp -= logf((float)total); }
   }
   const float qf = (float)q;
   // the first of equal indices, and the sum of q over them
@@ -150,9 +150,8 @@ SCM_DEV Stat rest_of_segment(const W& w, const NamedBits<WORDS>& bits, float c) 
 }
 
 // Gradient of a segment from (m, cr), then the named tokens over it.
-template <typename T, int NT, bool STREAM>
-SCM_DEV void distill_write(const Walk<T, NT>& w, T* dx, int lo, float m, float cr, float c) {
-  typedef Walk<T, NT> W;
+template <typename T, bool STREAM, typename W>
+SCM_DEV void distill_write(const W& w, T* dx, int lo, float m, float cr, float c) {
   w.run([&](int s, const typename W::Raw& raw) {
 #pragma unroll
     for (int u = 0; u < W::U; ++u) {
@@ -217,7 +216,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillTopkArgs a, int S, i
   if constexpr (GRAD) {
     __syncthreads();
     const float sc = row_scale(a, row, wt);
-    distill_write<T, NT, STREAM>(Walk<T, NT>{x, a.V}, dx, 0, row_m, row_cr * sc, a.c);
+    distill_write<T, STREAM>(Walk<T, NT>{x, a.V}, dx, 0, row_m, row_cr * sc, a.c);
     __syncthreads();   // the last store to a named token is this one; equal indices hold equal values
     if (en.idx >= 0) dx[en.idx] = (T)(g * sc);
   }
@@ -316,16 +315,16 @@ __global__ __launch_bounds__(64) void distill_join_kernel(DistillTopkArgs a, int
   write_tape(a, row, r.m, r.cr, r.g);
 }
 
-template <typename T, int NT, bool STREAM>
+template <typename T, int NT, int EL, bool STREAM>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillTopkArgs a, int S, int seg_len) {
   const long row = blockIdx.x / S;
   const int lo = (int)(blockIdx.x % S) * seg_len, tid = threadIdx.x;
-  const Walk<T, NT> w{(const T*)a.x + row * a.ldx + lo, min(a.V - lo, seg_len)};
+  const Walk<T, NT, EL> w{(const T*)a.x + row * a.ldx + lo, min(a.V - lo, seg_len)};
   T* dx = (T*)a.dx + row * a.V;
   const float wt = a.weight ? a.weight[row] : 1.f;
   if (wt == 0.f) { zero_write<T, NT>(dx + lo, w.len); return; }
   const float sc = row_scale(a, row, wt);
-  distill_write<T, NT, STREAM>(w, dx, lo, a.tape[2 * row], a.tape[2 * row + 1] * sc, a.c);
+  distill_write<T, STREAM>(w, dx, lo, a.tape[2 * row], a.tape[2 * row + 1] * sc, a.c);
   __syncthreads();
   if (tid < a.k) {
     const long long i = a.index[row * a.k + tid];
@@ -372,7 +371,7 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
       float r = 0.f, log_total = 0.f;
       double per = 1.0;
       if (a.tail) r = rest.s == 0.f ? 0.f : (float)fmax(0.0, 1.0 - total);
-      else if (total > 0.0) { per = 1.0 / total; log_total = (float)log(total); }
+      else if (total > 0.0) { per = 1.0 / total; log_total = logf((float)total); }
       const float big_a = (float)(total * per) + r;
       for (int j = 0; j < a.k; ++j) {
         const long long i = index[j];
@@ -411,16 +410,45 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
 }
 
 // ---------------------------------------------------------------- sums over the rows
-// out[0] = sum row_loss (mean: / sum weight), wsum_out = sum weight.  One workgroup, f64, a fixed order.
+// f64, in a fixed order: thread, wave, workgroup, workgroups.  part [gridDim.x][2]: this workgroup's sums of row_loss and of
+// weight (either may be null: 0).
+__global__ __launch_bounds__(1024) void distill_part_kernel(const float* __restrict__ row_loss,
+                                                            const float* __restrict__ weight, long T, long per,
+                                                            double* __restrict__ part) {
+  __shared__ double red[2][16];
+  const long lo = blockIdx.x * per, hi = min(T, lo + per);
+  double s = 0.0, w = 0.0;
+#pragma unroll 4
+  for (long i = lo + threadIdx.x; i < hi; i += 1024) {
+    if (row_loss) s += (double)row_loss[i];
+    if (weight) w += (double)weight[i];
+  }
+  s = wave_sum_f64(s);
+  w = wave_sum_f64(w);
+  if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = s; red[1][threadIdx.x >> 6] = w; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = w = 0.0;
+    for (int k = 0; k < 16; ++k) { s += red[0][k]; w += red[1][k]; }
+    part[2 * blockIdx.x] = s;
+    part[2 * blockIdx.x + 1] = w;
+  }
+}
+// out[0] = sum row_loss (mean: / sum weight), wsum_out = sum weight, from n <= 256 pairs or (part null) from the rows.
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ row_loss,
-                                                           const float* __restrict__ weight, long T, int mean,
+                                                           const float* __restrict__ weight, long T,
+                                                           const double* __restrict__ part, int n, int mean,
                                                            float* __restrict__ out, float* __restrict__ wsum_out) {
   __shared__ double red[2][16];
   double s = 0.0, w = 0.0;
+  if (part) {
+    if ((int)threadIdx.x < n) { s = part[2 * threadIdx.x]; w = part[2 * threadIdx.x + 1]; }
+  } else {
 #pragma unroll 8
-  for (long i = threadIdx.x; i < T; i += 1024) {
-    if (row_loss) s += (double)row_loss[i];
-    if (weight) w += (double)weight[i];
+    for (long i = threadIdx.x; i < T; i += 1024) {
+      if (row_loss) s += (double)row_loss[i];
+      if (weight) w += (double)weight[i];
+    }
   }
   s = wave_sum_f64(s);
   w = wave_sum_f64(w);
@@ -455,6 +483,7 @@ static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
   constexpr int MAX = 64 / (32 * (int)sizeof(T) / 4);   // steps in 64 registers: 4 for 2-byte types, 2 for f32
   const dim3 g((unsigned)a.T);
   if (a.V <= 64 * 8) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM, 8>), g, dim3(64), 0, s, a);
+  else if (a.V <= 64 * 16) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM, 16>), g, dim3(64), 0, s, a);
   else if (a.V <= 64 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM>), g, dim3(64), 0, s, a);
   else if (a.V <= 64 * 64) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 2, STREAM>), g, dim3(64), 0, s, a);
   else if (a.V <= 256 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM>), g, dim3(256), 0, s, a);
@@ -490,6 +519,8 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
       hipLaunchKernelGGL((distill_join_kernel<T>), g, dim3(64), 0, s, a, S);
     } else if (a.V <= 512) {
       hipLaunchKernelGGL((distill_kernel<T, 64, 8, 16, false>), g, dim3(64), 0, s, a, 1, a.V);
+    } else if (a.V <= 1024) {
+      hipLaunchKernelGGL((distill_kernel<T, 64, 16, 32, false>), g, dim3(64), 0, s, a, 1, a.V);
     } else if (a.V <= 8192) {   // one wave: 20000 x 4000 bf16 52 us, 256 threads 95 us; 10000 x 8000 45 and 55 us
       hipLaunchKernelGGL((distill_kernel<T, 64, 32, 256, false>), g, dim3(64), 0, s, a, 1, a.V);
     } else {
@@ -497,11 +528,15 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
     }
   }
   if (grad) {
-    if (a.V <= 2048) {
-      hipLaunchKernelGGL((distill_bwd_kernel<T, 64, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+    if (a.V <= 512) {
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 64, 8, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+    } else if (a.V <= 1024) {
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 64, 16, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
+    } else if (a.V <= 2048) {
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 64, 32, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);
     } else {
       const int len = logits_bwd_segment(a.T, a.V), sb = (a.V + len - 1) / len;
-      hipLaunchKernelGGL((distill_bwd_kernel<T, 256, STREAM>), dim3((unsigned)(a.T * sb)), dim3(256), 0, s, a, sb, len);
+      hipLaunchKernelGGL((distill_bwd_kernel<T, 256, 32, STREAM>), dim3((unsigned)(a.T * sb)), dim3(256), 0, s, a, sb, len);
     }
   }
 }
@@ -515,11 +550,22 @@ static void distill_dispatch(const DistillTopkArgs& a, bool loss, bool grad, hip
   else if (a.type == SCM_BF16) distill_sized<bf16>(a, loss, grad, s);
   else distill_sized<f16>(a, loss, grad, s);
 }
+// One workgroup adds up to 16384 rows; more of them (1,000,000 rows: 330 us) go through 4096-row parts at least.
+static void distill_sum(const DistillTopkArgs& a, const float* row_loss, const float* weight, int mean, float* out,
+                        float* wsum_out, hipStream_t s) {
+  int n = 0;
+  if (a.T > DISTILL_SUM_ROWS) {
+    const long per = a.T > 256L * 4096 ? (a.T + 255) / 256 : 4096;
+    n = (int)((a.T + per - 1) / per);
+    hipLaunchKernelGGL(distill_part_kernel, dim3(n), dim3(1024), 0, s, row_loss, weight, a.T, per, a.sums);
+  }
+  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, row_loss, weight, a.T, n ? a.sums : (double*)nullptr, n,
+                     mean, out, wsum_out);
+}
 hipError_t topk_distill_fwd(const DistillTopkArgs& a, float* out, float* wsum_out, hipStream_t s) {
   Traced tr(K_TOPK_DISTILL, 0, s);
   distill_dispatch(a, true, false, s);
-  if (out)
-    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, a.row_loss, a.weight, a.T, a.mean, out, wsum_out);
+  if (out) distill_sum(a, a.row_loss, a.weight, a.mean, out, wsum_out, s);
   return hipGetLastError();
 }
 hipError_t topk_distill_bwd(const DistillTopkArgs& a, hipStream_t s) {
@@ -530,11 +576,9 @@ hipError_t topk_distill_bwd(const DistillTopkArgs& a, hipStream_t s) {
 hipError_t topk_distill_step(const DistillTopkArgs& a, float* out, float* wsum, hipStream_t s) {
   Traced tr(K_TOPK_DISTILL, 0, s);
   // the gradient of a mean needs the weights' sum first
-  if (a.weight && a.mean)
-    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, (const float*)nullptr, a.weight, a.T, 0,
-                       (float*)nullptr, wsum);
+  if (a.weight && a.mean) distill_sum(a, nullptr, a.weight, 0, nullptr, wsum, s);
   distill_dispatch(a, true, true, s);
-  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, a.row_loss, a.weight, a.T, a.mean, out, (float*)nullptr);
+  distill_sum(a, a.row_loss, a.weight, a.mean, out, nullptr, s);
   return hipGetLastError();
 }
 

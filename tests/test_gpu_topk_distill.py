@@ -285,6 +285,28 @@ def test_offsets_past_32_bits(L):
     assert torch.equal(g, dx) and torch.equal(loss, loss2)
 
 
+@pytest.mark.parametrize("t", [16384, 16385, 70001, 1_100_000])
+def test_sums_over_many_rows(L, t):
+    """one workgroup's sum, and parts joined: rows of one known loss each, sums in 64 bits rounded once"""
+    gen = torch.Generator().manual_seed(t)
+    x = torch.randn(t, 3, generator=gen).to(DEV)
+    idx = torch.randint(0, 3, (t, 1), generator=gen).to(DEV)
+    lp = torch.full((t, 1), -0.3, device=DEV)
+    w = torch.rand(t, generator=gen).to(DEV)
+    rows = L.topk_distillation(x, idx, lp, weight=w, reduction="none")
+    for reduction, div in (("sum", 1.0), ("mean", w.double().sum())):
+        want = rows.double().sum() / div
+        for got in (L.topk_distillation(x, idx, lp, weight=w, reduction=reduction),
+                    L.topk_distillation_grad(x, idx, lp, weight=w, reduction=reduction)[0]):
+            assert abs(got.double() - want) <= 2 * U * abs(want)
+    assert abs(L.topk_distillation(x, idx, lp).double() - L.topk_distillation(x, idx, lp, reduction="none").double().mean()) <= 4 * U
+    _, dx = L.topk_distillation_grad(x, idx, lp, weight=w)
+    _, ds = L.topk_distillation_grad(x, idx, lp, weight=w, reduction="sum")
+    # an entry is A p - q - r share with A p, q, r share <= 1, each scaled by the row's weight (and 1 / sum) and rounded
+    # before the difference: 2 roundings a part and one of the scale on either side, 3 parts, 2 x 3 x 3 u of the weight
+    assert ((dx.double() * w.double().sum() - ds.double()).abs() <= 18 * U * w.double()[:, None]).all()
+
+
 def test_refusals(L):
     x, idx, lp, w = _case(4, 90, 3, torch.float32, 1)
     f, s = L.topk_distillation, L.topk_distillation_grad
