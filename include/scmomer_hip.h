@@ -103,7 +103,7 @@ int scm_ln_bwd_noalloc(const float* dy, const float* x, const float* mean, const
 /* ---- LayerNorm of rows of any width, in the types of a wide or half-precision model (the pair above is the residual
  *      stream's: f32, D <= 256).  It has no counterpart in the reference, which leaves its other norms to torch.
  *      x [T,D] with row stride ldx elements (0: one row for all), last dimension contiguous, any alignment; y and dx
- *      contiguous.  Types: f32 -> f32 or bf16, bf16 -> bf16, fp16 -> fp16; gamma, beta (either may be NULL: 1, 0),
+ *      contiguous, apart from the inputs (not in place).  Types: f32 -> f32 or bf16, bf16 -> bf16, fp16 -> fp16; gamma, beta (either may be NULL: 1, 0),
  *      statistics and parameter gradients f32.  0 < D <= 16384, 0 < T < 2^31.
  *      mean, rstd [T]: both, or both NULL where no backward follows. */
 enum { SCM_F32 = 0, SCM_BF16 = 1, SCM_F16 = 2 };
@@ -283,8 +283,8 @@ int scm_linear_attention(const float* qf, const float* kf, const float* v, int64
 
 /* ---- log probabilities read off rows of logits, for any vocabulary (scm_ce_fwd below is the loss of the RNA model's
  *      own <= 8 classes).  No counterpart in the reference.  x [T,V] with row stride ldx elements (0: one row for
- *      all), last dimension contiguous, any alignment, type SCM_F32 / SCM_BF16 / SCM_F16; z = x / temperature;
- *      V <= 2^30.
+ *      all), last dimension contiguous, any alignment, type SCM_F32 / SCM_BF16 / SCM_F16; z = x / temperature,
+ *      2^-126 <= temperature < inf; V <= 2^30.
  *      Per row: lse = log sum exp z (may be NULL); logprob = z[target] - lse (target and logprob: both or neither),
  *      0 where target == ignore_index, NaN for any other target outside [0,V); entropy = -sum p ln p (may be NULL);
  *      the k <= min(64, V) tokens of the largest x in descending order, equal values by ascending index, NaN first,
@@ -295,7 +295,7 @@ int64_t scm_score_ws_floats(int64_t T, int V, int k);
 int scm_score_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* target,
                   int64_t ignore_index, int k, float* logprob, float* lse, float* entropy, float* top_logprob,
                   int64_t* top_index, float* tape, float* ws, void* stream);
-/* dx [T,V] (x's type, contiguous) = the gradient of sum g_logprob logprob + g_lse lse + g_entropy entropy + g_top
+/* dx [T,V] (x's type, contiguous, apart from x) = the gradient of sum g_logprob logprob + g_lse lse + g_entropy entropy + g_top
  * top_logprob (g_*: f32, [T] or [T,k], each may be NULL); entropy, top_index as the forward wrote them (the indices of
  * a row distinct).  Rows of -inf only get 0. */
 int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* target,
@@ -316,7 +316,7 @@ int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
  *      mean; wsum (one float, may be NULL): that sum.  The loss is not multiplied by temperature^2.
  *      tape: scm_topk_distill_tape_floats floats (0 for V <= 64), NULL in the forward where no backward follows;
  *      ws: scm_topk_distill_ws_floats floats, 8-byte aligned.
- *      bwd: dx [T,V] (x's type, contiguous) = gloss[0] (gloss_rows: gloss[t]) * the gradient of the loss (row_loss).
+ *      bwd: dx [T,V] (x's type, contiguous, apart from x) = gloss[0] (gloss_rows: gloss[t]) * the gradient of the loss (row_loss).
  *      step: loss, and dx = scale * its gradient, without a backward of its own; a row is read from memory once. */
 int64_t scm_topk_distill_tape_floats(int64_t T, int V, int k);
 int64_t scm_topk_distill_ws_floats(int64_t T, int V);

@@ -258,7 +258,7 @@ static int logits_check(const char* who, const void* x, int type, int64_t ldx, i
   SCM_REQ(T > 0 && T < ((int64_t)1 << 31) && V > 0 && V <= (1 << 30) && ldx >= 0,
           "%s: need 0 < T < 2^31, 0 < V <= 2^30, ldx >= 0", who);
   SCM_REQ(k >= 0 && k <= LOGITS_MAX_K, "%s: at most %d entries a row (got %d)", who, LOGITS_MAX_K, k);
-  SCM_REQ(temperature > 0.f && temperature < INFINITY, "%s: temperature must be positive and finite", who);
+  SCM_REQ(temperature >= 0x1p-126f && temperature < INFINITY, "%s: temperature must be in [2^-126, inf)", who);
   return 0;
 }
 static float log2e_over(float temperature) { return (float)(1.4426950408889634 / (double)temperature); }

@@ -97,6 +97,29 @@ Tensor once(const Tensor& g) {
   return FirstOnly::apply(g.detach().requires_grad_(true));
 }
 
+// A leaf's accumulator keeps the stream of the graph that made it for as long as a graph holds it.  Where that is the default
+// stream, a backward pass under capture would make that stream wait for a captured event, which no capture allows and
+// which ends the process.  Called by the node whose gradients are due, before anything is launched.
+void check_capture(const Tensor& t) {
+  const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (here.stream() == nullptr) return;   // never under capture
+  if (hipStreamIsCapturing(here.stream(), &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return;
+  }
+  const auto node = torch::autograd::get_current_node();
+  if (status == hipStreamCaptureStatusNone || !node) return;
+  for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& e = node->next_edge(i);
+    if (!e.function || !node->task_should_compute_output(i)) continue;   // no gradient is wanted there
+    const auto s = e.function->stream();
+    TORCH_CHECK(!s || s->id() != 0, "a backward pass under capture reaches ", e.function->name(), " on the default stream, "
+                "which cannot take part: release the eager graph that holds it (its loss and outputs), or run that graph's "
+                "forward pass on another stream than the default one");
+  }
+}
+
 // ---------------------------------------------------------------------------- layer norm
 // -> y, statistics [2, T] (mean, 1 / standard deviation)
 std::tuple<Tensor, Tensor> norm_fwd(const Tensor& x_, const Tensor& w, const Tensor& b, double eps,
@@ -143,6 +166,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const bool want_x = ctx->needs_input_grad(0), want_w = w.defined() && ctx->needs_input_grad(1);
     const bool want_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.defined() ? 2 : 1);
     const c10::DeviceGuard guard(x.device());
+    check_capture(x);
     Tensor dx = want_x ? at::empty(x_.sizes(), x.options()) : Tensor();
     auto sum = [&](bool want) {   // no rows: the sums are empty
       return !want ? Tensor() : t ? floats(x, {d}) : at::zeros({d}, x.options().dtype(at::kFloat));
@@ -170,8 +194,8 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
 Tensor logits_rows(const Tensor& logits, double temperature, int64_t k) {
   Tensor x = rows_of(logits, "logits");
   TORCH_CHECK_VALUE(x.size(1) <= LOGITS_MAX_V, "logits: at most 2^30 classes (got ", x.size(1), ")");
-  TORCH_CHECK_VALUE((float)temperature > 0.f && std::isfinite((float)temperature),
-                    "temperature must be positive and finite, got ", temperature);
+  TORCH_CHECK_VALUE((float)temperature > 0.f && std::isnormal((float)temperature),   // smaller: 1 / temperature overflows
+                    "temperature must be positive, finite and at least 2^-126, got ", temperature);
   TORCH_CHECK_VALUE(k >= 0 && k <= LOGITS_MAX_K, "at most ", LOGITS_MAX_K, " entries per row (got ", k, ")");
   check_device(x, "logits");
   return x;
@@ -240,6 +264,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     const Tensor g_lse = grad_rows(grads[i++], x, t);
     const Tensor g_top = grad_rows(k ? grads[i++] : none, x, t * k);
     const c10::DeviceGuard guard(x.device());
+    check_capture(x);
     Tensor dx = at::empty(logits.sizes(), x.options());
     if (t)
       call(api.score_bwd(x.data_ptr(), type_of(x, "logits"), x.stride(0), t, (int)v, (float)temperature,
@@ -348,6 +373,7 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
     const Distill op(saved[0], saved[1], saved[2], saved[3], ctx->saved_data["temperature"].toDouble(), opts & 1,
                      (Reduction)(opts >> 1), true);
     const c10::DeviceGuard guard(op.x.device());
+    check_capture(op.x);
     Tensor dx = at::empty(saved[0].sizes(), op.x.options());
     if (op.t) {
       const bool per_row = op.red == NONE;

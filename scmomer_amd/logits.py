@@ -2,6 +2,9 @@
 probabilities of given tokens with entropy and top alternatives (token_logprobs), and distillation from a teacher's top
 log probabilities (topk_distillation, topk_distillation_grad).  The RNA model's own masked cross
 entropy over its at most eight expression classes is s1.masked_cross_entropy.
+
+A backward pass of these under capture into a graph is refused while an eager graph on the default stream holds the same
+leaf (its gradient would have to join that stream).
 """
 from __future__ import annotations
 

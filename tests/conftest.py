@@ -13,8 +13,8 @@ GOLDEN = os.path.join(ROOT, "tests", "golden")
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
     # the package has no fallback path: make sure the HIP library exists (hipcc cross-compiles without a GPU)
-    so = os.path.join(ROOT, "scmomer_amd", "libscmomer_hip.so")
-    if not os.path.exists(so):
+    built = [os.path.join(ROOT, "scmomer_amd", so) for so in ("libscmomer_hip.so", "_torch_ops.so")]
+    if not all(os.path.exists(so) for so in built):
         import subprocess
         subprocess.run(["make", "-C", os.path.join(ROOT, "scmomer_amd", "csrc"), "-j8"], check=True)
 

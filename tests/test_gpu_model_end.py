@@ -2,6 +2,8 @@
 (norm, head, token_logprobs with alternatives) and a student (norm, head, topk_distillation) against the same step in 64
 bits; gradients wanted of any subset of the inputs; a graph kept, used twice, differentiated twice, broken by an in-place
 change."""
+import gc
+
 import pytest
 import torch
 
@@ -156,6 +158,36 @@ def test_saved_tensors_may_move(M, name):
         loss = calls[name](z)
     got, = torch.autograd.grad(loss, z)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["norm", "score", "distill"])
+def test_capture_beside_an_eager_graph_of_the_same_leaf(M, name):
+    """The eager graph keeps the leaf's accumulator on the default stream, which cannot take part in a capture: the backward
+    pass is refused; a gradient of other tensors, and the same call once the eager graph is gone, are captured."""
+    x, calls = _calls(M)
+    z = x.detach().requires_grad_()
+    alive = calls[name](z)
+    want, = torch.autograd.grad(alive, z, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other = z.detach().requires_grad_()
+        got, = torch.autograd.grad(calls[name](other), other)
+        with pytest.raises(RuntimeError, match="default stream"):
+            torch.autograd.grad(calls[name](z), z)
+    del alive
+    gc.collect()          # the refusal's traceback holds a graph too
+    again = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(again):
+        got2, = torch.autograd.grad(calls[name](z), z)
+    for _ in range(3):
+        graph.replay()
+        again.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(got2, want)
+        got.zero_()
+        got2.zero_()
+        torch.cuda.synchronize()
 
 
 def test_inference_mode_and_no_grad(M):

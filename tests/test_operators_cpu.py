@@ -61,7 +61,7 @@ def test_token_logprobs_needs_device_tensors():
 
 @pytest.mark.parametrize("change", [dict(x=None), dict(type=3), dict(ldx=-1), dict(T=0), dict(T=1 << 31), dict(V=0),
                                     dict(V=(1 << 30) + 1), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("inf")),
-                                    dict(tau=float("nan")), dict(k=-1), dict(k=65), dict(k=9), dict(target=None),
+                                    dict(tau=float("nan")), dict(tau=1e-38), dict(k=-1), dict(k=65), dict(k=9), dict(target=None),
                                     dict(logprob=None), dict(top=None), dict(index=None), dict(V=100000, k=3, ws=None),
                                     dict(ws_off=4)])
 def test_score_fwd_rejects(change):
