@@ -484,11 +484,13 @@ __global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
 }
 
 // ---------------------------------------------------------------- host launchers
-// Segments per row: 1 where the rows alone fill the card (two workgroups per CU) or a row is short; else enough
-// workgroups for four per CU, of at least 2048 elements (one step of a workgroup is 8192), and no more than the join takes.
+// Segments per row.  One where a row is short or the rows alone keep the card busy: one launch, no partial results (bf16,
+// k = 20: 400 x 131072 33 us against 40 us in 1200 segments; 100 x 131072 19 against 20 in 600; 64 x 65536 14 against 13
+// in 512).  Else about 512 workgroups (twice as many: 100 x 32768 15 us, against 14), of at least 2048 elements, and no
+// more than the join takes.
 int score_segments(long T, int V, int k) {
-  if (V <= 8192 || T >= 512) return 1;
-  long s = (1024 + T - 1) / T, most = (V + 2047) / 2048;
+  if (V <= 8192 || logits_rows_fill(T, V)) return 1;
+  long s = (512 + T - 1) / T, most = (V + 2047) / 2048;
   if (s > most) s = most;
   if (s > LOGITS_MAX_SEGMENTS) s = LOGITS_MAX_SEGMENTS;
   if (k && s * k > LOGITS_JOIN_KEYS) s = LOGITS_JOIN_KEYS / k;
@@ -518,7 +520,10 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   if (S > 1) {
     const int len = segment_length(a.V, S);
     S = segments_used(a.V, len);
-    launch_score<T, 256>(a, S, len, s);
+    // a thread's elements by the segment: 100 x 32768 bf16, k = 20 in segments of about 3000: 16 us with 32, 10 with 16
+    if (len <= 2048) launch_score<T, 256, 8>(a, S, len, s);
+    else if (len <= 4096) launch_score<T, 256, 16>(a, S, len, s);
+    else launch_score<T, 256>(a, S, len, s);
     if (a.entropy) hipLaunchKernelGGL((score_join_kernel<T, true>), dim3((unsigned)a.T), dim3(256), 0, s, a, S);
     else hipLaunchKernelGGL((score_join_kernel<T, false>), dim3((unsigned)a.T), dim3(256), 0, s, a, S);
     return;
@@ -531,6 +536,8 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8>(a, 1, a.V, s);
   if (a.V <= 1024 && a.k <= 32) return launch_score<T, 64, 16>(a, 1, a.V, s);
   if (bytes <= 16384 && a.k <= 32) return launch_score<T, 64>(a, 1, a.V, s);
+  // a workgroup per CU at most, and many alternatives: 64 x 65536 bf16, k = 64 15 us, on 256 threads 21 (k = 20: 15 and 15)
+  if (a.T <= 256 && a.V > 8192 && a.k > 32) return launch_score<T, 512>(a, 1, a.V, s);
   if (bytes <= 49152) return launch_score<T, 128>(a, 1, a.V, s);
   if (bytes <= 196608) return launch_score<T, 256>(a, 1, a.V, s);
   launch_score<T, 512>(a, 1, a.V, s);

@@ -207,6 +207,8 @@ struct ScoreGradArgs {
   const float* g_logprob; const float* g_lse; const float* g_entropy; const float* g_top;   // each may be null
   void* dx;
 };
+// Rows that keep the card busy with one workgroup each.
+inline bool logits_rows_fill(long T, int V) { return T >= 256 || (T >= 64 && V <= 131072); }
 int score_segments(long T, int V, int k);
 int logits_bwd_segment(long T, int V);
 hipError_t score_fwd(const ScoreArgs& a, hipStream_t s);

@@ -464,11 +464,12 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
 }
 
 // ---------------------------------------------------------------- host launchers
-// Segments per row: as for the scores (two workgroups per CU fill the card), and never more tokens than the bits hold.
+// Segments per row: as for the scores, and never more tokens than the bits hold.  Loss of 400 x 50000 bf16 17 us in one
+// segment, 22 in three; loss and gradient 27 and 37 us.
 int distill_segments(long T, int V) {
   const long least = (V + DISTILL_SEGMENT - 1) / DISTILL_SEGMENT;
-  if (V <= 8192 || T >= 512) return (int)least;
-  long s = (1024 + T - 1) / T, most = (V + 2047) / 2048;
+  if (V <= 8192 || logits_rows_fill(T, V)) return (int)least;
+  long s = (512 + T - 1) / T, most = (V + 2047) / 2048;
   if (s > most) s = most;
   if (s > LOGITS_MAX_SEGMENTS) s = LOGITS_MAX_SEGMENTS;
   return (int)(s > least ? s : least);
@@ -515,7 +516,10 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
     if (S > 1) {
       const int len = seg_len_of(a.V, S);
       S = (a.V + len - 1) / len;
-      hipLaunchKernelGGL((distill_kernel<T, 256, 32, DISTILL_SEGMENT / 32, false>), dim3((unsigned)(a.T * S)), dim3(256), 0, s, a, S, len);
+      const dim3 gs((unsigned)(a.T * S));
+      if (len <= 2048) hipLaunchKernelGGL((distill_kernel<T, 256, 8, 64, false>), gs, dim3(256), 0, s, a, S, len);
+      else if (len <= 4096) hipLaunchKernelGGL((distill_kernel<T, 256, 16, 128, false>), gs, dim3(256), 0, s, a, S, len);
+      else hipLaunchKernelGGL((distill_kernel<T, 256, 32, DISTILL_SEGMENT / 32, false>), gs, dim3(256), 0, s, a, S, len);
       hipLaunchKernelGGL((distill_join_kernel<T>), g, dim3(64), 0, s, a, S);
     } else if (a.V <= 512) {
       hipLaunchKernelGGL((distill_kernel<T, 64, 8, 16, false>), g, dim3(64), 0, s, a, 1, a.V);
@@ -523,6 +527,8 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
       hipLaunchKernelGGL((distill_kernel<T, 64, 16, 32, false>), g, dim3(64), 0, s, a, 1, a.V);
     } else if (a.V <= 8192) {   // one wave: 20000 x 4000 bf16 52 us, 256 threads 95 us; 10000 x 8000 45 and 55 us
       hipLaunchKernelGGL((distill_kernel<T, 64, 32, 256, false>), g, dim3(64), 0, s, a, 1, a.V);
+    } else if (a.T <= 256) {   // a workgroup per CU: 100 x 131072 bf16 14.7 us, on 256 threads 20.3
+      hipLaunchKernelGGL((distill_kernel<T, 512, 32, DISTILL_SEGMENT / 32, false>), g, dim3(512), 0, s, a, 1, a.V);
     } else {
       hipLaunchKernelGGL((distill_kernel<T, 256, 32, DISTILL_SEGMENT / 32, false>), g, dim3(256), 0, s, a, 1, a.V);
     }

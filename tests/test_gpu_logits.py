@@ -100,6 +100,16 @@ def test_scores(token_logprobs, t, v, k, dtype):
         _check(token_logprobs(x, target, k=k, temperature=tau), x, target, k, tau)
 
 
+# where rows are split, by the elements of a thread in a segment, and from where on they are not
+@pytest.mark.parametrize("t,v,k", [(40, 16906, 20), (40, 40003, 20), (40, 40003, 0), (30, 131072, 64), (63, 65537, 64),
+                                   (64, 9001, 64), (64, 131072, 20), (64, 131073, 20), (200, 70001, 40), (255, 140001, 8),
+                                   (256, 140001, 3), (257, 9000, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_of_few_rows(token_logprobs, t, v, k, dtype):
+    x, target = _logits(t, v, dtype, t + v)
+    _check(token_logprobs(x, target, k=k), x, target, k, 1.0)
+
+
 @pytest.mark.parametrize("v", [7, 64, 100, 1500, 9000, 40000])
 def test_masks_ties_and_special_values(token_logprobs, v):
     x, target = _logits(12, v, torch.float32, v)

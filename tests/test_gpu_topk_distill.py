@@ -127,6 +127,15 @@ def test_loss_and_gradient(L, t, v, k, dtype, tail):
     _check(L, x, idx, lp, w, 1.0 if t % 2 else 1.7, tail)
 
 
+# where rows are split, by the elements of a thread in a segment, and from where on they are not
+@pytest.mark.parametrize("t,v,k", [(40, 40003, 20), (30, 131072, 64), (63, 16906, 7), (64, 16906, 7), (64, 131072, 20),
+                                   (65, 131073, 5), (256, 140001, 3), (257, 50001, 12)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_few_rows(L, t, v, k, dtype):
+    x, idx, lp, w = _case(t, v, k, dtype, t + v)
+    _check(L, x, idx, lp, w, 1.0, True)
+
+
 @pytest.mark.parametrize("v", [40, 700, 9000, 20000])
 @pytest.mark.parametrize("tail", [True, False])
 def test_conventions(L, v, tail):

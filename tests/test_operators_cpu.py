@@ -137,6 +137,7 @@ def test_topk_distill_workspaces():
     assert lib.scm_topk_distill_ws_floats(1000, 131072) == 0                 # one workgroup per row
     assert lib.scm_topk_distill_ws_floats(1000, 131073) == 4000              # more tokens than a workgroup marks
     assert lib.scm_topk_distill_ws_floats(16384, 7) == 0 and lib.scm_topk_distill_ws_floats(16385, 7) == 1024   # parts of the sums
-    for t in (1, 7, 511):
+    assert lib.scm_topk_distill_ws_floats(64, 131072) == 0
+    for t in (1, 7, 63):
         n = lib.scm_topk_distill_ws_floats(t, 100000)
         assert n % (2 * t) == 0 and 2 <= n // (2 * t) <= 64
