@@ -314,7 +314,7 @@ int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
  *      -inf only has loss and gradient 0.  weight [T] (may be NULL: 1): row_loss = weight * loss, rows of weight 0 are
  *      not read; loss (one float, may be NULL in the forward) = sum of row_loss, divided by the sum of the weights when
  *      mean; wsum (one float, may be NULL): that sum.  The loss is not multiplied by temperature^2.
- *      tape: scm_topk_distill_tape_floats floats (0 for V <= 64), NULL in the forward where no backward follows;
+ *      tape: scm_topk_distill_tape_floats floats (0: none), NULL in the forward where no backward follows;
  *      ws: scm_topk_distill_ws_floats floats, 8-byte aligned.
  *      bwd: dx [T,V] (x's type, contiguous, apart from x) = gloss[0] (gloss_rows: gloss[t]) * the gradient of the loss (row_loss).
  *      step: loss, and dx = scale * its gradient, without a backward of its own; a row is read from memory once. */

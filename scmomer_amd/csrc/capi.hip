@@ -304,13 +304,13 @@ int scm_score_bwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
 }
 
 int64_t scm_topk_distill_tape_floats(int64_t T, int V, int k) {
-  return T > 0 && V > 64 && k > 0 && k <= LOGITS_MAX_K ? T * (2 + (int64_t)k) : 0;
+  return T > 0 && V > 0 && !logits_by_thread(T, V) && k > 0 && k <= LOGITS_MAX_K ? T * (2 + (int64_t)k) : 0;
 }
 // [256][2] doubles for the sums over many rows, then the split rows' statistics
 static int64_t distill_sum_floats(int64_t T) { return T > DISTILL_SUM_ROWS ? 2 * 256 * 2 : 0; }
 int64_t scm_topk_distill_ws_floats(int64_t T, int V) {
   if (T <= 0 || V <= 0) return 0;
-  const int64_t S = V <= 64 ? 1 : distill_segments(T, V);
+  const int64_t S = distill_segments(T, V);
   return distill_sum_floats(T) + (S > 1 ? 2 * T * S : 0);
 }
 static int distill_topk_args(const char* who, DistillTopkArgs& a, const void* x, int type, int64_t ldx, int64_t T, int V,
@@ -322,7 +322,7 @@ static int distill_topk_args(const char* who, DistillTopkArgs& a, const void* x,
   a = DistillTopkArgs{};
   a.x = x; a.ldx = ldx; a.type = type; a.T = T; a.V = V; a.k = k; a.tail = tail != 0; a.mean = mean != 0;
   a.c = log2e_over(temperature); a.inv_t = 1.f / temperature; a.index = index; a.lp = logprob; a.weight = weight;
-  if (tape && V > 64) { a.tape = tape; a.g_top = tape + 2 * T; }
+  if (tape && !logits_by_thread(T, V)) { a.tape = tape; a.g_top = tape + 2 * T; }
   return 0;
 }
 int scm_topk_distill_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
@@ -344,7 +344,7 @@ int scm_topk_distill_bwd(const void* x, int type, int64_t ldx, int64_t T, int V,
   DistillTopkArgs a;
   if (int e = distill_topk_args("scm_topk_distill_bwd", a, x, type, ldx, T, V, temperature, index, logprob, k, tail, weight,
                                 mean, const_cast<float*>(tape))) return e;
-  SCM_REQ(gloss && dx && (tape || V <= 64), "scm_topk_distill_bwd: null pointer");
+  SCM_REQ(gloss && dx && (tape || logits_by_thread(T, V)), "scm_topk_distill_bwd: null pointer");
   SCM_REQ(!(mean && weight) || wsum, "scm_topk_distill_bwd: a weighted mean needs the weights' sum");
   a.gloss = gloss; a.gloss_rows = gloss_rows != 0; a.wsum = weight ? wsum : nullptr; a.dx = dx;
   SCM_HIP(topk_distill_bwd(a, (hipStream_t)stream), "scm_topk_distill_bwd");
@@ -356,7 +356,7 @@ int scm_topk_distill_step(const void* x, int type, int64_t ldx, int64_t T, int V
   DistillTopkArgs a;
   if (int e = distill_topk_args("scm_topk_distill_step", a, x, type, ldx, T, V, temperature, index, logprob, k, tail, weight,
                                 mean, tape)) return e;
-  SCM_REQ(row_loss && loss && dx && (tape || V <= 64), "scm_topk_distill_step: null pointer");
+  SCM_REQ(row_loss && loss && dx && (tape || logits_by_thread(T, V)), "scm_topk_distill_step: null pointer");
   SCM_REQ(!(mean && weight) || wsum, "scm_topk_distill_step: a weighted mean needs room for the weights' sum");
   SCM_REQ(ws || scm_topk_distill_ws_floats(T, V) == 0, "scm_topk_distill_step: null workspace");
   SCM_REQ(((uintptr_t)ws & 7) == 0, "scm_topk_distill_step: workspace must be 8-byte aligned");

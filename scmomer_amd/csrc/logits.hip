@@ -4,9 +4,9 @@
 // The logits are read once, in 16-byte chunks; every thread keeps a running maximum m and s = sum 2^((x - m) c),
 // c = log2(e) / temperature, in f32; threads, waves and workgroups join by rescaling to the larger maximum.  x - m is
 // formed first: a row of the type's lowest value is an ordinary (uniform) row, and -inf weighs nothing.
-//   V <= 64    one thread per row, 64 rows staged through LDS per wave
-//   else       64 to 512 threads per row by its length; where rows are too few to fill the card a row is split into
-//              segments of one workgroup each, whose partial results a second launch joins in segment order
+//   many rows of V <= 64   one thread per row, 64 rows staged through LDS per wave
+//   else                   64 to 512 threads per row by its length; where long rows are too few to fill the card a row is split
+//                          into segments of one workgroup each, whose partial results a second launch joins in segment order
 // What bounds them is HBM, and for 2-byte types the vector ALU nearly as much (an exponential costs four issue slots).
 #include "scm_softmax.hpp"
 
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a, int S) {
   }
 }
 
-// ---------------------------------------------------------------- rows of at most 64 logits, one thread each
+// ---------------------------------------------------------------- short rows, one thread each
 template <typename T, bool ENT>
 __global__ __launch_bounds__(64) void score_small_kernel(ScoreArgs a) {
   extern __shared__ uint32_t lds[];
@@ -369,7 +369,9 @@ __global__ __launch_bounds__(64) void score_small_kernel(ScoreArgs a) {
   uint32_t* o = lds + threadIdx.x * pitch;
   auto x = [&](int i) { return __uint_as_float(o[i]); };
   Stat st = stat_none();
+#pragma unroll 8
   for (int i = 0; i < V; ++i) st.m = fmaxf(st.m, x(i));
+#pragma unroll 8
   for (int i = 0; i < V; ++i) {
     const float d = (x(i) - st.m) * a.c, e = exp2_fast(d);
     st.s += e;
@@ -379,10 +381,12 @@ __global__ __launch_bounds__(64) void score_small_kernel(ScoreArgs a) {
   write_row<ENT>(a, row, st, a.target && t >= 0 && t < V ? x((int)t) : 0.f, t);
   if (!a.k) return;
   const RowScore r(st, a.inv_t);
+#pragma unroll 8
   for (int i = 0; i < V; ++i) o[i] = ordered(x(i));
   for (int j = 0; j < a.k; ++j) {   // k <= V selections, each taken out
     uint32_t b = 0;
     int bi = 0;
+#pragma unroll 8
     for (int i = 0; i < V; ++i)
       if (o[i] > b) { b = o[i]; bi = i; }
     o[bi] = 0;
@@ -510,7 +514,7 @@ static void launch_score(const ScoreArgs& a, int S, int len, hipStream_t s) {
 }
 template <typename T>
 static void score_typed(const ScoreArgs& a, hipStream_t s) {
-  if (a.V <= 64) {
+  if (score_by_thread(a.T, a.V)) {
     const dim3 g((unsigned)((a.T + 63) / 64));
     if (a.entropy) hipLaunchKernelGGL((score_small_kernel<T, true>), g, dim3(64), small_lds(a.V), s, a);
     else hipLaunchKernelGGL((score_small_kernel<T, false>), g, dim3(64), small_lds(a.V), s, a);
@@ -544,7 +548,7 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
 }
 template <typename T, bool STREAM>
 static void score_bwd_typed(const ScoreGradArgs& a, hipStream_t s) {
-  if (a.V <= 64) {
+  if (logits_by_thread(a.T, a.V)) {
     hipLaunchKernelGGL((score_bwd_small_kernel<T>), dim3((unsigned)((a.T + 63) / 64)), dim3(64), small_lds(a.V), s, a);
   } else if (a.V <= 512) {   // one step of one wave
     hipLaunchKernelGGL((score_bwd_kernel<T, 64, 8, STREAM>), dim3((unsigned)a.T), dim3(64), 0, s, a, 1, a.V);

@@ -127,19 +127,33 @@ SCM_DEV void stat_add(Stat& st, const float (&v)[EL], float bm, float c) {
   st = {m, s, h};
 }
 
-// Rows of at most 64 logits, one thread each: 64 rows go through LDS (row stride odd: no bank conflicts along a
-// column) as f32 bits, read and written along memory.
+// Short rows, one thread each: 64 rows go through LDS (row stride odd: no bank conflicts along a column) as f32 bits,
+// read and written along memory, eight elements of a thread on their way at once.
 constexpr unsigned small_lds(int V) { return 64 * (V | 1) * 4; }
 template <typename T, bool STORE>
 SCM_DEV void stage_rows(T* p, long ld, int rows, int V, uint32_t* lds, int pitch) {
+  constexpr int B = 8;
   const int dr = 64 / V, dc = 64 % V;
   int r = threadIdx.x / V, c = threadIdx.x % V;
   while (r < rows) {
-    if constexpr (STORE) p[r * ld + c] = (T)__uint_as_float(lds[r * pitch + c]);
-    else lds[r * pitch + c] = __float_as_uint((float)p[r * ld + c]);
-    r += dr;
-    c += dc;
-    if (c >= V) { c -= V; ++r; }
+    int row[B], col[B];
+    uint32_t v[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      row[b] = r;
+      col[b] = c;
+      const int rr = min(r, rows - 1);   // past the end: some element, not used
+      v[b] = STORE ? lds[rr * pitch + c] : __float_as_uint((float)p[rr * ld + c]);
+      r += dr;
+      c += dc;
+      if (c >= V) { c -= V; ++r; }
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (row[b] < rows) {
+        if constexpr (STORE) p[row[b] * ld + col[b]] = (T)__uint_as_float(v[b]);
+        else lds[row[b] * pitch + col[b]] = v[b];
+      }
   }
 }
 

@@ -169,7 +169,7 @@ SCM_DEV void zero_write(T* dx, int len) {
   for (int i = threadIdx.x * E; i < len; i += NT * E) store_chunk<T, E>(dx + i, none, len - i);
 }
 
-// ---------------------------------------------------------------- V > 64
+// ---------------------------------------------------------------- one to four waves per row, or per segment of one
 SCM_DEV void write_tape(const DistillTopkArgs& a, long row, float m, float cr, float g) {   // by a wave
   if (!a.tape) return;
   const int j = threadIdx.x & 63;
@@ -332,11 +332,31 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillTopkArgs a, int 
   }
 }
 
-// ---------------------------------------------------------------- V <= 64: a thread per row, a bit per token
+// ---------------------------------------------------------------- short rows: a thread per row, a bit per token
+// f(j, index, log probability) for a row's entries, eight of them on their way at once.
+template <typename F>
+SCM_DEV void each_entry(const int64_t* index, const float* lp, int k, F f) {
+  constexpr int B = 8;
+  for (int j = 0; j < k; j += B) {
+    long long i[B];
+    float l[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int jj = min(j + b, k - 1);
+      i[b] = index[jj];
+      l[b] = lp[jj];
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (j + b < k && i[b] >= 0) f(j + b, i[b], l[b]);
+  }
+}
+// LDS: the logits of 64 rows, then q of their entries in f64.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
   extern __shared__ uint32_t lds[];
   const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
+  double* q_of = (double*)(lds + 64 * pitch) + threadIdx.x;   // entry j: q_of[64 j]
   const long row = (long)blockIdx.x * 64 + threadIdx.x;
   stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
   __syncthreads();
@@ -351,18 +371,20 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
       unsigned long long named = 0;
       bool beyond = false;
       double total = 0.0;
-      for (int j = 0; j < a.k; ++j) {
-        const long long i = index[j];
-        if (i < 0) continue;
-        if (i >= V) { beyond = true; continue; }
+      each_entry(index, lps, a.k, [&](int j, long long i, float lp) {
+        if (i >= V) { beyond = true; return; }
         named |= 1ull << i;
-        total += exp((double)lps[j]);
-      }
+        const double q = exp((double)lp);
+        q_of[64 * j] = q;
+        total += q;
+      });
       Stat all = stat_none(), rest = stat_none();
+#pragma unroll 8
       for (int i = 0; i < V; ++i) {
         all.m = fmaxf(all.m, x(i));
         if (!((named >> i) & 1)) rest.m = fmaxf(rest.m, x(i));
       }
+#pragma unroll 8
       for (int i = 0; i < V; ++i) {
         all.s += exp2_fast((x(i) - all.m) * a.c);
         if (!((named >> i) & 1)) rest.s += exp2_fast((x(i) - rest.m) * a.c);
@@ -373,12 +395,11 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
       if (a.tail) r = rest.s == 0.f ? 0.f : (float)fmax(0.0, 1.0 - total);
       else if (total > 0.0) { per = 1.0 / total; log_total = logf((float)total); }
       const float big_a = (float)(total * per) + r;
-      for (int j = 0; j < a.k; ++j) {
-        const long long i = index[j];
-        if (i < 0 || i >= V) continue;
-        const float lp = lps[j], q = (float)(exp((double)lp) * per);
+      each_entry(index, lps, a.k, [&](int j, long long i, float lp) {
+        if (i >= V) return;
+        const float q = (float)(q_of[64 * j] * per);
         if (q > 0.f) loss += q * (lp - log_total - ((x((int)i) - all.m) * a.inv_t - LN2 * l2));
-      }
+      });
       if (r > 0.f) loss += r * (logf(r) - ((rest.m - all.m) * a.inv_t + LN2 * (log2_fast(rest.s) - l2)));
       const bool empty = all.s == 0.f, broken = beyond || total != total || all.s != all.s;
       if (empty) loss = 0.f;
@@ -387,16 +408,16 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
       if constexpr (GRAD) {
         const float sc = row_scale(a, row, wt);
         const float ca = big_a / all.s * sc, cr = rest.s == 0.f ? 0.f : r / rest.s * sc;
+#pragma unroll 8
         for (int i = 0; i < V; ++i) {
           float g = ca * exp2_fast((x(i) - all.m) * a.c);
           if (!((named >> i) & 1) && cr != 0.f) g -= cr * exp2_fast((x(i) - rest.m) * a.c);
           o[i] = __float_as_uint(empty ? 0.f : broken ? __uint_as_float(0x7FC00000u) : g);
         }
         if (!empty && !broken)
-          for (int j = 0; j < a.k; ++j) {
-            const long long i = index[j];
-            if (i >= 0) o[i] = __float_as_uint(x((int)i) - (float)(exp((double)lps[j]) * per) * sc);
-          }
+          each_entry(index, lps, a.k, [&](int j, long long i, float) {
+            o[i] = __float_as_uint(x((int)i) - (float)(q_of[64 * j] * per) * sc);
+          });
       }
     } else if constexpr (GRAD) {
       for (int i = 0; i < V; ++i) o[i] = 0u;
@@ -497,10 +518,11 @@ static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
 }
 template <typename T, bool STREAM>
 static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s) {
-  if (a.V <= 64) {
+  if (logits_by_thread(a.T, a.V)) {
     const dim3 g((unsigned)((a.T + 63) / 64));
-    if (grad) hipLaunchKernelGGL((distill_small_kernel<T, true>), g, dim3(64), small_lds(a.V), s, a);
-    else hipLaunchKernelGGL((distill_small_kernel<T, false>), g, dim3(64), small_lds(a.V), s, a);
+    const unsigned lds = small_lds(a.V) + 64 * a.k * sizeof(double);   // 49 KB at most
+    if (grad) hipLaunchKernelGGL((distill_small_kernel<T, true>), g, dim3(64), lds, s, a);
+    else hipLaunchKernelGGL((distill_small_kernel<T, false>), g, dim3(64), lds, s, a);
     return;
   }
   int S = distill_segments(a.T, a.V);

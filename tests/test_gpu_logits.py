@@ -100,6 +100,14 @@ def test_scores(token_logprobs, t, v, k, dtype):
         _check(token_logprobs(x, target, k=k, temperature=tau), x, target, k, tau)
 
 
+# short rows in numbers (a thread per row), and as many as not yet
+@pytest.mark.parametrize("t,v,k", [(2100, 17, 17), (2200, 17, 3), (4097, 33, 20), (4300, 33, 20), (8192, 64, 5), (8193, 64, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_scores_of_many_short_rows(token_logprobs, t, v, k, dtype):
+    x, target = _logits(t, v, dtype, t + v)
+    _check(token_logprobs(x, target, k=k), x, target, k, 1.0)
+
+
 # where rows are split, by the elements of a thread in a segment, and from where on they are not
 @pytest.mark.parametrize("t,v,k", [(40, 16906, 20), (40, 40003, 20), (40, 40003, 0), (30, 131072, 64), (63, 65537, 64),
                                    (64, 9001, 64), (64, 131072, 20), (64, 131073, 20), (200, 70001, 40), (255, 140001, 8),
@@ -253,6 +261,21 @@ def test_gradients_of_empty_masked_and_broken_rows(token_logprobs, v):
     dx = _grad(token_logprobs, x, target, 3, 1.0, gl, gh, gl, torch.ones(6, 3, device=DEV))
     assert torch.equal(dx[0], torch.zeros_like(dx[0])) and torch.isnan(dx[1]).all() and torch.isnan(dx[4]).all()
     assert torch.isfinite(dx[[2, 3, 5]]).all()
+
+
+@pytest.mark.parametrize("t,v,k", [(3600, 7, 2), (10300, 20, 20), (10200, 20, 0), (32800, 64, 3)])
+def test_gradients_of_many_short_rows(token_logprobs, t, v, k):
+    x, target = _logits(t, v, torch.float32, t)
+    x[::6] = -INF
+    x[2::6] = torch.finfo(torch.float32).min
+    x[3::6, 1:] = -INF
+    target[5] = -100
+    g = torch.randn(3, t, generator=torch.Generator().manual_seed(v)).to(DEV)
+    gt = torch.randn(t, k, generator=torch.Generator().manual_seed(v + 1)).to(DEV) if k else None
+    dx = _grad(token_logprobs, x, target, k, 1.0, g[0], g[1], g[2], gt)
+    assert torch.equal(dx[::6], torch.zeros_like(dx[::6]))
+    keep = torch.arange(t, device=DEV) % 6 != 0
+    _check_grad(dx[keep], x[keep], target[keep], k, 1.0, g[0][keep], g[1][keep], g[2][keep], gt[keep] if k else None)
 
 
 def test_gradient_of_an_expanded_row(token_logprobs):

@@ -136,9 +136,16 @@ def test_few_rows(L, t, v, k, dtype):
     _check(L, x, idx, lp, w, 1.0, True)
 
 
-@pytest.mark.parametrize("v", [40, 700, 9000, 20000])
-@pytest.mark.parametrize("tail", [True, False])
-def test_conventions(L, v, tail):
+# short rows in numbers: a thread per row
+@pytest.mark.parametrize("t,v,k", [(520, 1, 1), (1100, 2, 2), (3700, 7, 3), (8201, 16, 16), (16900, 33, 20), (32800, 64, 64),
+                                   (33001, 64, 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_many_short_rows(L, t, v, k, dtype):
+    x, idx, lp, w = _case(t, v, k, dtype, t + v)
+    _check(L, x, idx, lp, w, 1.3, bool(t % 2))
+
+
+def _odd_rows(v):
     x, idx, lp, w = _case(14, v, 6, torch.float32, v)
     w[:] = 1
     x[0] = -INF                                   # nothing left
@@ -156,12 +163,25 @@ def test_conventions(L, v, tail):
     lp[9] = torch.log_softmax(lp[9], 0)           # the entries hold all of the teacher's mass
     x[10, ::2] = -INF                             # some entries excluded: an infinite loss, a finite gradient
     idx[10, 0] = 2
+    return x, idx, lp, w
+
+
+@pytest.mark.parametrize("tail", [True, False])
+def test_conventions_of_many_short_rows(L, tail):
+    x, idx, lp, w = _odd_rows(40)
+    _check(L, x.repeat(1500, 1), idx.repeat(1500, 1), lp.repeat(1500, 1), w.repeat(1500), 1.0, tail)
+
+
+@pytest.mark.parametrize("v", [40, 700, 9000, 20000])
+@pytest.mark.parametrize("tail", [True, False])
+def test_conventions(L, v, tail):
+    x, idx, lp, w = _odd_rows(v)
     _check(L, x, idx, lp, w, 1.0, tail)
     rows = L.topk_distillation(x, idx, lp, tail=tail, reduction="none")
     assert rows[0] == 0 and abs(rows[2]) <= _terms(v) * U and rows[10] == INF and torch.isfinite(rows[[1, 3, 4, 5, 6, 7, 8, 9]]).all()
 
 
-@pytest.mark.parametrize("t,v", [(4, 40), (4, 700), (4, 9000), (600, 9000)])
+@pytest.mark.parametrize("t,v", [(4, 40), (20500, 40), (4, 700), (4, 9000), (600, 9000)])
 def test_broken_rows_stay_by_themselves(L, t, v):
     x, idx, lp, w = _case(t, v, 4, torch.float32, v)
     idx[0, 1] = v                                 # outside the vocabulary

@@ -133,7 +133,7 @@ def test_topk_distill_rejects(entry, change):
 
 def test_topk_distill_workspaces():
     from scmomer_amd._lib import lib
-    assert lib.scm_topk_distill_tape_floats(10, 64, 5) == 0 and lib.scm_topk_distill_tape_floats(10, 65, 5) == 70
+    assert lib.scm_topk_distill_tape_floats(10, 64, 5) == 70 and lib.scm_topk_distill_tape_floats(100000, 64, 5) == 0
     assert lib.scm_topk_distill_ws_floats(1000, 131072) == 0                 # one workgroup per row
     assert lib.scm_topk_distill_ws_floats(1000, 131073) == 4000              # more tokens than a workgroup marks
     assert lib.scm_topk_distill_ws_floats(16384, 7) == 0 and lib.scm_topk_distill_ws_floats(16385, 7) == 1024   # parts of the sums
