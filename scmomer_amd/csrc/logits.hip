@@ -64,16 +64,17 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
   for (int r = 0; r < R; ++r) {
     b[r] = L.best[r * 64 + l];
     at[r] = L.at[r * 64 + l];
-    lo = min(lo, b[r]);
+    lo = b[r] ? min(lo, b[r]) : lo;
     hi = max(hi, b[r]);
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) { lo = min(lo, (uint32_t)__shfl_xor((int)lo, o)); hi = max(hi, (uint32_t)__shfl_xor((int)hi, o)); }
   // all maxima lie in [lo, hi]; t keeps the invariant: reach of them are >= t, reach >= k (0: fewer than k threads hold
   // elements, then every element is a candidate)
+  const int holders = min(chunks, NT);
   const int shared = lo == hi ? 0 : 32 - __builtin_clz(lo ^ hi);   // bits that differ
-  uint32_t t = shared >= 32 ? 0u : (hi >> shared) << shared;
-  int reach = NT, above = 0, bit = shared - 1;
+  uint32_t t = shared >= 32 || holders < k ? 0u : (hi >> shared) << shared;
+  int reach = holders, above = 0, bit = holders < k ? -1 : shared - 1;
   const int enough = k + k / 8;
   for (; bit >= spare && reach > enough; --bit) {
     const uint32_t cand = t | (1u << bit);
@@ -160,17 +161,22 @@ SCM_DEV void top_of_segment(const W& w, int lo, int k, uint32_t best, int at, bo
     auto in = [&](uint32_t o, int chunk) { return o > thr_top || (o >= thr && chunk <= thr_at); };
     if (best && in(best, at)) L.at[atomicAdd(&L.threads, 1)] = tid;
     __syncthreads();
-    const int per = (chunks + NT - 1) / NT, pairs = L.threads * per;
+    // the bounds as numbers (at or below the order of -inf: every element)
+    const float from = thr <= 0x007FFFFFu ? -INFINITY : unordered(thr), above = unordered(thr_top + 1);
+    const int per = W::EL < 32 ? U : (chunks + NT - 1) / NT, pairs = L.threads * per;
     for (int i = tid; i < pairs; i += NT) {
       const int c = L.at[i / per] + NT * (i % per);
       const Chunk<T, E> raw = load_chunk<T, E>(w.p + (long)c * E, w.len - c * E);
+      const float bound = c <= thr_at ? from : above;
+      uint32_t hits = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const uint32_t o = ordered((float)raw.e[j]);
-        if (in(o, c) && c * E + j < w.len) {
-          const int pos = atomicAdd(&L.count, 1);
-          if (pos < TopLds<NT>::CAP) L.cand[pos] = key_of(o, lo + c * E + j);
-        }
+      for (int j = 0; j < E; ++j) hits |= (uint32_t)((float)raw.e[j] >= bound) << j;
+      if (w.len - c * E < E) hits &= (1u << max(w.len - c * E, 0)) - 1u;
+      while (hits) {   // few: one read again each
+        const int at_hit = c * E + __builtin_ctz(hits);
+        hits &= hits - 1;
+        const int pos = atomicAdd(&L.count, 1);
+        if (pos < TopLds<NT>::CAP) L.cand[pos] = key_of(ordered((float)w.p[at_hit]), lo + at_hit);
       }
     }
   }
