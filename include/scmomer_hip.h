@@ -103,7 +103,8 @@ int scm_ln_bwd_noalloc(const float* dy, const float* x, const float* mean, const
 /* ---- LayerNorm of rows of any width, in the types of a wide or half-precision model (the pair above is the residual
  *      stream's: f32, D <= 256).  It has no counterpart in the reference, which leaves its other norms to torch.
  *      x [T,D] with row stride ldx elements (0: one row for all), last dimension contiguous, any alignment; y and dx
- *      contiguous, apart from the inputs (not in place).  Types: f32 -> f32 or bf16, bf16 -> bf16, fp16 -> fp16; gamma, beta (either may be NULL: 1, 0),
+ *      contiguous, apart from the inputs (not in place).  Types: f32 -> f32 or bf16, bf16 -> bf16, fp16 -> fp16; gamma,
+ *      beta (either may be NULL: 1, 0),
  *      statistics and parameter gradients f32.  0 < D <= 16384, 0 < T < 2^31.
  *      mean, rstd [T]: both, or both NULL where no backward follows. */
 enum { SCM_F32 = 0, SCM_BF16 = 1, SCM_F16 = 2 };

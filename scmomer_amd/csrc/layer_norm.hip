@@ -4,7 +4,7 @@
 // (norm_embed.hip holds the form of the Performer's own residual stream: f32, D <= 256, D % 4 == 0, bf16 out.)
 //
 // Both directions are bound by HBM: a row is held in registers between its one read and its one write, L lanes per
-// row with at most 16 elements each (L = 16, 64: several rows per workgroup, no barrier; L = 256, 512, 1024: one row
+// row with at most 16 elements each (L = 16, 32, 64: several rows per workgroup, no barrier; L = 128 to 1024: one row
 // per workgroup, one barrier per row and direction).  Statistics, sums and parameter gradients are f32.
 #include "scm_chunk.hpp"
 
@@ -16,8 +16,8 @@ constexpr int norm_threads(int L) { return L <= 64 ? 256 : L; }
 // Which columns a lane holds: CPT chunks of E, lane-interleaved over the L lanes of a group.  Chunk c is loaded from column
 // at[c]; its elements from first[c] on are the lane's (the last chunk of a row that is no multiple of E begins E columns
 // before the end, first[c] of them again; E: none are).  So every lane loads and stores whole chunks on one path, without
-// a branch between a load and its use: branches there make the compiler wait for the loads ahead as well (8192 x 4096 bf16:
-// forward 31 -> 29 us, backward 55 -> 47 us).  WHOLE = D >= E; narrower rows go element by element.
+// a branch between a load and its use: branches there make the compiler wait for the loads ahead as well (8192 x 4096 bf16
+// that way: forward 31 us instead of 29, backward 55 instead of 47).  WHOLE = D >= E; narrower rows go element by element.
 template <int E, int L, int CPT, bool WHOLE>
 struct Columns {
   int at[CPT], first[CPT];
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
 
 // ---------------------------------------------------------------- host launchers
 // Lanes per row and elements per lane: 8 elements each as long as 1024 threads hold the row.  (16 elements on half the
-// lanes: 8192 x 4096 bf16 forward 59 us, against 50 us; the registers of a longer slice cost waves.)
+// lanes: 8192 x 4096 bf16 backward 54 us, against 40: the registers of a longer slice cost waves; forward 26 either way.)
 struct NormShape { int L, ept; };
 static NormShape norm_shape(int D) {
   if (D <= 128) return {16, 8};
@@ -316,9 +316,9 @@ static NormShape norm_shape(int D) {
   if (D <= 8192) return {1024, 8};
   return {1024, 16};
 }
-// Workgroups: 1024 threads per CU in either direction, each group going on from row to row with its loads ahead.  More
-// start-up (gamma, beta, first rows) than they hide: forward 8192 x 4096 bf16 with 2048 threads per CU 50 us, 1024: 46 us;
-// fewer of them in the backward pass leave less partial sums but hide less: 512: 74 us, 1024: 58 us.
+// Workgroups: 1024 threads per CU in either direction, each group going on from row to row with its loads ahead.  8192 x 4096
+// bf16 forward: 512 threads per CU 34 us, 1024: 26, 2048: 25; backward (partial sums per workgroup): 38, 36 and 42; f32
+// 84530 x 200 backward 36.6, 34.5 and 38.
 static long norm_blocks(long T, int D) {
   const int nt = norm_threads(norm_shape(D).L), rpb = nt / norm_shape(D).L;
   const long b = (T + rpb - 1) / rpb, cap = 256L * (1024 / nt);

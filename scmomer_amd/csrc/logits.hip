@@ -68,7 +68,10 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
     hi = max(hi, b[r]);
   }
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { lo = min(lo, (uint32_t)__shfl_xor((int)lo, o)); hi = max(hi, (uint32_t)__shfl_xor((int)hi, o)); }
+  for (int o = 1; o < 64; o <<= 1) {
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, o));
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
+  }
   // all maxima lie in [lo, hi]; t keeps the invariant: reach of them are >= t, reach >= k (0: fewer than k threads hold
   // elements, then every element is a candidate)
   const int holders = min(chunks, NT);
@@ -93,7 +96,8 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
       const int cand = lim | (1 << bit);
       int n = 0;
 #pragma unroll
-      for (int r = 0; r < R; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] >= t && b[r] <= top && at[r] < cand));
+      for (int r = 0; r < R; ++r)
+        n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] >= t && b[r] <= top && at[r] < cand));
       if (n < need) lim = cand;
     }
   }
@@ -496,7 +500,7 @@ __global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
 // ---------------------------------------------------------------- host launchers
 // Segments per row.  One where a row is short or the rows alone keep the card busy: one launch, no partial results (bf16,
 // k = 20: 400 x 131072 33 us against 40 us in 1200 segments; 100 x 131072 19 against 20 in 600; 64 x 65536 14 against 13
-// in 512).  Else about 512 workgroups (twice as many: 100 x 32768 15 us, against 14), of at least 2048 elements, and no
+// in 512).  Else about 512 workgroups (twice as many: 30 x 131072 15.1 us, against 14.7), of at least 2048 elements, and no
 // more than the join takes.
 int score_segments(long T, int V, int k) {
   if (V <= 8192 || logits_rows_fill(T, V)) return 1;
@@ -530,7 +534,8 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   if (S > 1) {
     const int len = segment_length(a.V, S);
     S = segments_used(a.V, len);
-    // a thread's elements by the segment: 100 x 32768 bf16, k = 20 in segments of about 3000: 16 us with 32, 10 with 16
+    // a thread's elements by the segment: 3 x 131072 bf16, k = 20 in segments of 2048: 10.0 us with 32, 7.7 with 8; 1100
+    // segments of about 3000: 16.2 with 32, 10.2 with 16
     if (len <= 2048) launch_score<T, 256, 8>(a, S, len, s);
     else if (len <= 4096) launch_score<T, 256, 16>(a, S, len, s);
     else launch_score<T, 256>(a, S, len, s);
@@ -540,8 +545,8 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   }
   // Threads per row by the row's bytes: more of them shorten the walk, fewer the reductions and the search for the
   // alternatives behind it, and leave more rows in flight; and at least two threads per alternative, so that the threads'
-  // maxima bound them well.  bf16, k = 8: 20000 x 4000 62 us on 64 threads, 81 on 128; 6000 x 16000 58 on 128, 65 on 64, 68
-  // on 256; 2048 x 65536 62 on 256, 68 on 128 and on 512; 1200 x 131072 72 on 512, 79 on 256.
+  // maxima bound them well.  bf16, k = 8: 20000 x 4000 55 us on 64 threads, 69 on 128; 6000 x 16000 52 on 128, 59 on 64, 58
+  // on 256; 2048 x 65536 56 on 256, 58 on 128, 61 on 512; 1200 x 131072 68 on 512, 74 on 256.
   const long bytes = (long)a.V * sizeof(T);
   if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8>(a, 1, a.V, s);
   if (a.V <= 1024 && a.k <= 32) return launch_score<T, 64, 16>(a, 1, a.V, s);

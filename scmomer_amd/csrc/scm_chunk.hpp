@@ -57,8 +57,8 @@ SCM_DEV float lanes_sum(float v) {
 }
 
 // Results of more bytes than the L2 caches hold (8 x 4 MB) are written with STREAM: they would push out what is still to be
-// read (layer norm forward of 8192 x 4096 bf16: 46 -> 34 us; gradient of 4096 x 65536 bf16 logits: 203 -> 176 us; loss and
-// gradient of 700 x 131072: 120 -> 99 us).
+// read (8192 x 4096 bf16 layer norm forward: 26 us, 27 without; gradient of 4096 x 65536 bf16 logits: 186 and 214; loss and
+// gradient of 20000 x 4000: 65 and 91, of 2048 x 131072: 251 and 291, of 8192 x 32768: 227 and 222).
 constexpr long STREAM_BYTES = 32L << 20;
 
 }  // namespace scm

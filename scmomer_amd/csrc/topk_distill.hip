@@ -498,8 +498,8 @@ int distill_segments(long T, int V) {
 static int seg_len_of(int V, int S) { return ((V + S - 1) / S + 31) / 32 * 32; }
 
 // Loss and gradient of rows that fit a workgroup's registers.  false: they do not, or (2-byte types above 32768) would
-// leave one workgroup per CU, whose reading, reducing and writing then follow each other: 4096 x 65536 bf16 319 us,
-// against 259 us for the kernel that reads the row again from the last-level cache; 8192 x 32768: 231 against 287 us.
+// leave one workgroup per CU, whose reading, reducing and writing then follow each other: 4096 x 65536 bf16 261 us,
+// against 249 us for the kernel that reads the row again from the last-level cache; 8192 x 32768: 227 against 261 us.
 template <typename T, bool STREAM>
 static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
   constexpr int MAX = 64 / (32 * (int)sizeof(T) / 4);   // steps in 64 registers: 4 for 2-byte types, 2 for f32
@@ -511,8 +511,10 @@ static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
   else if (a.V <= 256 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM>), g, dim3(256), 0, s, a);
   else if (a.V <= 256 * 64) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 2, STREAM>), g, dim3(256), 0, s, a);
   else if (a.V <= 256 * 32 * MAX) hipLaunchKernelGGL((distill_resident_kernel<T, 256, MAX, STREAM>), g, dim3(256), 0, s, a);
-  else if (sizeof(T) == 4 && a.V <= 512 * 64) hipLaunchKernelGGL((distill_resident_kernel<float, 512, 2, STREAM>), g, dim3(512), 0, s, a);
-  else if (sizeof(T) == 4 && a.V <= 1024 * 64) hipLaunchKernelGGL((distill_resident_kernel<float, 1024, 2, STREAM>), g, dim3(1024), 0, s, a);
+  else if (sizeof(T) == 4 && a.V <= 512 * 64)
+    hipLaunchKernelGGL((distill_resident_kernel<float, 512, 2, STREAM>), g, dim3(512), 0, s, a);
+  else if (sizeof(T) == 4 && a.V <= 1024 * 64)
+    hipLaunchKernelGGL((distill_resident_kernel<float, 1024, 2, STREAM>), g, dim3(1024), 0, s, a);
   else return false;
   return true;
 }
@@ -528,9 +530,10 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
   int S = distill_segments(a.T, a.V);
   if (S == 1 && loss && grad) {
     a.tape = a.g_top = nullptr;   // for a backward of its own only
-    // (512 threads: two workgroups per CU, whose rows fit the last-level cache together; 256: 2048 x 131072 364 us, 512: 334 us)
+    // (512 threads: two workgroups per CU, whose rows fit the last-level cache together; 256: 2048 x 131072 300 us, 512: 251 us)
     if (!launch_resident<T, STREAM>(a, s))
-      hipLaunchKernelGGL((distill_kernel<T, 512, 32, DISTILL_SEGMENT / 32, true, STREAM>), dim3((unsigned)a.T), dim3(512), 0, s, a, 1, a.V);
+      hipLaunchKernelGGL((distill_kernel<T, 512, 32, DISTILL_SEGMENT / 32, true, STREAM>), dim3((unsigned)a.T), dim3(512), 0, s,
+                         a, 1, a.V);
     return;
   }
   if (loss) {
@@ -547,7 +550,7 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
       hipLaunchKernelGGL((distill_kernel<T, 64, 8, 16, false>), g, dim3(64), 0, s, a, 1, a.V);
     } else if (a.V <= 1024) {
       hipLaunchKernelGGL((distill_kernel<T, 64, 16, 32, false>), g, dim3(64), 0, s, a, 1, a.V);
-    } else if (a.V <= 8192) {   // one wave: 20000 x 4000 bf16 52 us, 256 threads 95 us; 10000 x 8000 45 and 55 us
+    } else if (a.V <= 8192) {   // one wave: 20000 x 4000 bf16 47 us, 256 threads 89 us; 10000 x 8000 42 and 48 us
       hipLaunchKernelGGL((distill_kernel<T, 64, 32, 256, false>), g, dim3(64), 0, s, a, 1, a.V);
     } else if (a.T <= 256) {   // a workgroup per CU: 100 x 131072 bf16 14.7 us, on 256 threads 20.3
       hipLaunchKernelGGL((distill_kernel<T, 512, 32, DISTILL_SEGMENT / 32, false>), g, dim3(512), 0, s, a, 1, a.V);
