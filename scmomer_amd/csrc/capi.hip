@@ -281,8 +281,9 @@ int scm_score_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float 
   a.x = x; a.ldx = ldx; a.type = type; a.T = T; a.V = V; a.k = k; a.c = log2e_over(temperature); a.inv_t = 1.f / temperature;
   a.target = target; a.ignore = ignore_index; a.logprob = logprob; a.lse = lse; a.entropy = entropy;
   a.top_logprob = top_logprob; a.top_index = top_index; a.tape = tape;
+  a.S = score_segments(T, V, k);
   a.part_top = (unsigned long*)ws;
-  a.part = ws ? ws + 2 * (int64_t)k * T * score_segments(T, V, k) : nullptr;
+  a.part = ws ? ws + 2 * (int64_t)k * T * a.S : nullptr;
   SCM_HIP(score_fwd(a, (hipStream_t)stream), "scm_score_fwd");
   return 0;
 }
@@ -322,7 +323,8 @@ static int distill_topk_args(const char* who, DistillTopkArgs& a, const void* x,
   a = DistillTopkArgs{};
   a.x = x; a.ldx = ldx; a.type = type; a.T = T; a.V = V; a.k = k; a.tail = tail != 0; a.mean = mean != 0;
   a.c = log2e_over(temperature); a.inv_t = 1.f / temperature; a.index = index; a.lp = logprob; a.weight = weight;
-  if (tape && !logits_by_thread(T, V)) { a.tape = tape; a.g_top = tape + 2 * T; }
+  a.rows = T; a.by_thread = logits_by_thread(T, V); a.S = distill_segments(T, V);
+  if (tape && !a.by_thread) { a.tape = tape; a.g_top = tape + 2 * T; }
   return 0;
 }
 int scm_topk_distill_fwd(const void* x, int type, int64_t ldx, int64_t T, int V, float temperature, const int64_t* index,
@@ -344,7 +346,7 @@ int scm_topk_distill_bwd(const void* x, int type, int64_t ldx, int64_t T, int V,
   DistillTopkArgs a;
   if (int e = distill_topk_args("scm_topk_distill_bwd", a, x, type, ldx, T, V, temperature, index, logprob, k, tail, weight,
                                 mean, const_cast<float*>(tape))) return e;
-  SCM_REQ(gloss && dx && (tape || logits_by_thread(T, V)), "scm_topk_distill_bwd: null pointer");
+  SCM_REQ(gloss && dx && (tape || a.by_thread), "scm_topk_distill_bwd: null pointer");
   SCM_REQ(!(mean && weight) || wsum, "scm_topk_distill_bwd: a weighted mean needs the weights' sum");
   a.gloss = gloss; a.gloss_rows = gloss_rows != 0; a.wsum = weight ? wsum : nullptr; a.dx = dx;
   SCM_HIP(topk_distill_bwd(a, (hipStream_t)stream), "scm_topk_distill_bwd");
@@ -356,11 +358,12 @@ int scm_topk_distill_step(const void* x, int type, int64_t ldx, int64_t T, int V
   DistillTopkArgs a;
   if (int e = distill_topk_args("scm_topk_distill_step", a, x, type, ldx, T, V, temperature, index, logprob, k, tail, weight,
                                 mean, tape)) return e;
-  SCM_REQ(row_loss && loss && dx && (tape || logits_by_thread(T, V)), "scm_topk_distill_step: null pointer");
+  SCM_REQ(row_loss && loss && dx && (tape || a.by_thread), "scm_topk_distill_step: null pointer");
   SCM_REQ(!(mean && weight) || wsum, "scm_topk_distill_step: a weighted mean needs room for the weights' sum");
   SCM_REQ(ws || scm_topk_distill_ws_floats(T, V) == 0, "scm_topk_distill_step: null workspace");
   SCM_REQ(((uintptr_t)ws & 7) == 0, "scm_topk_distill_step: workspace must be 8-byte aligned");
-  a.row_loss = row_loss; a.sums = (double*)ws; a.part = ws ? ws + distill_sum_floats(T) : nullptr; a.scale = scale; a.wsum = weight && mean ? wsum : nullptr; a.dx = dx;
+  a.row_loss = row_loss; a.sums = (double*)ws; a.part = ws ? ws + distill_sum_floats(T) : nullptr; a.scale = scale;
+  a.wsum = weight && mean ? wsum : nullptr; a.dx = dx;
   SCM_HIP(topk_distill_step(a, loss, wsum, (hipStream_t)stream), "scm_topk_distill_step");
   return 0;
 }

@@ -10,6 +10,8 @@
 // What bounds them is HBM, and for 2-byte types the vector ALU nearly as much (an exponential costs four issue slots).
 #include "scm_softmax.hpp"
 
+#include <algorithm>
+
 namespace scm {
 
 // ---------------------------------------------------------------- order of the alternatives
@@ -530,7 +532,7 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((score_small_kernel<T, false>), g, dim3(64), small_lds(a.V), s, a);
     return;
   }
-  int S = score_segments(a.T, a.V, a.k);
+  int S = a.S;
   if (S > 1) {
     const int len = segment_length(a.V, S);
     S = segments_used(a.V, len);
@@ -578,24 +580,56 @@ static void score_bwd_sized(const ScoreGradArgs& a, hipStream_t s) {
   if (a.T * a.V * (long)sizeof(T) > STREAM_BYTES) score_bwd_typed<T, true>(a, s);
   else score_bwd_typed<T, false>(a, s);
 }
-// At least 8192 elements per workgroup; longer where that leaves more workgroups than a launch takes (2^31 - 1).
+// At least 8192 elements per workgroup; longer where that leaves more workgroups of 256 threads than a launch takes.
 int logits_bwd_segment(long T, int V) {
   int len = 8192;
-  while ((long)segments_used(V, len) * T > 0x7FFFFFFFL) len *= 2;
+  while ((long)segments_used(V, len) * T >= 1L << 24) len *= 2;
   return len;
 }
-hipError_t score_fwd(const ScoreArgs& a, hipStream_t s) {
+// n rows of a call from row t on.
+static ScoreArgs rows_from(ScoreArgs a, long t, long n) {
+  a.x = (const char*)a.x + t * a.ldx * (a.type == SCM_F32 ? 4 : 2);
+  a.T = n;
+  if (a.target) { a.target += t; a.logprob += t; }
+  if (a.lse) a.lse += t;
+  if (a.entropy) a.entropy += t;
+  if (a.k) { a.top_logprob += t * a.k; a.top_index += t * a.k; }
+  if (a.tape) a.tape += 2 * t;
+  return a;   // the partial results stay: rows are split only where one launch takes them all
+}
+static ScoreGradArgs rows_from(ScoreGradArgs a, long t, long n) {
+  const long size = a.type == SCM_F32 ? 4 : 2;
+  a.x = (const char*)a.x + t * a.ldx * size;
+  a.dx = (char*)a.dx + t * a.V * size;
+  a.T = n;
+  a.tape += 2 * t;
+  if (a.target) a.target += t;
+  if (a.entropy) a.entropy += t;
+  if (a.top_index) a.top_index += t * a.k;
+  if (a.g_logprob) a.g_logprob += t;
+  if (a.g_lse) a.g_lse += t;
+  if (a.g_entropy) a.g_entropy += t;
+  if (a.g_top) a.g_top += t * a.k;
+  return a;
+}
+hipError_t score_fwd(const ScoreArgs& all, hipStream_t s) {
   Traced tr(K_SCORE, 0, s);
-  if (a.type == SCM_F32) score_typed<float>(a, s);
-  else if (a.type == SCM_BF16) score_typed<bf16>(a, s);
-  else score_typed<f16>(a, s);
+  for (long t = 0; t < all.T; t += LOGITS_LAUNCH_ROWS) {
+    const ScoreArgs a = rows_from(all, t, std::min(all.T - t, LOGITS_LAUNCH_ROWS));
+    if (a.type == SCM_F32) score_typed<float>(a, s);
+    else if (a.type == SCM_BF16) score_typed<bf16>(a, s);
+    else score_typed<f16>(a, s);
+  }
   return hipGetLastError();
 }
-hipError_t score_bwd(const ScoreGradArgs& a, hipStream_t s) {
+hipError_t score_bwd(const ScoreGradArgs& all, hipStream_t s) {
   Traced tr(K_SCORE, 0, s);
-  if (a.type == SCM_F32) score_bwd_sized<float>(a, s);
-  else if (a.type == SCM_BF16) score_bwd_sized<bf16>(a, s);
-  else score_bwd_sized<f16>(a, s);
+  for (long t = 0; t < all.T; t += LOGITS_LAUNCH_ROWS) {
+    const ScoreGradArgs a = rows_from(all, t, std::min(all.T - t, LOGITS_LAUNCH_ROWS));
+    if (a.type == SCM_F32) score_bwd_sized<float>(a, s);
+    else if (a.type == SCM_BF16) score_bwd_sized<bf16>(a, s);
+    else score_bwd_sized<f16>(a, s);
+  }
   return hipGetLastError();
 }
 

@@ -197,7 +197,8 @@ struct ScoreArgs {
   float* logprob; float* lse; float* entropy;      // entropy may be null, logprob goes with target
   float* top_logprob; int64_t* top_index;
   float* tape;                        // [T][2] maximum and sum, or null
-  unsigned long* part_top; float* part;            // split rows: [T][S][k] keys, [T][S][3] statistics
+  int S;                              // segments per row
+  unsigned long* part_top; float* part;            // S > 1: [T][S][k] keys, [T][S][3] statistics
 };
 struct ScoreGradArgs {
   const void* x; long ldx; int type; long T; int V, k;
@@ -216,6 +217,8 @@ inline bool logits_rows_fill(long T, int V) { return T >= 256 || (T >= 64 && V <
 //   distillation step  5000 x 64: 25 and 10;                 20000 x 64: 28 and 21;  100000 x 64: 35 and 62
 inline bool score_by_thread(long T, int V) { return V <= 64 && (V <= 16 || T > 128L * V); }
 inline bool logits_by_thread(long T, int V) { return V <= 64 && T > 512L * V; }   // gradients, distillation
+// Rows of one launch: with at most 1024 threads per row fewer than the 2^32 threads that a launch takes.
+constexpr long LOGITS_LAUNCH_ROWS = 1L << 21;
 int score_segments(long T, int V, int k);
 int logits_bwd_segment(long T, int V);
 hipError_t score_fwd(const ScoreArgs& a, hipStream_t s);
@@ -228,8 +231,9 @@ struct DistillTopkArgs {
   const int64_t* index; const float* lp;           // [T][k]
   const float* weight;                             // [T] or null
   float* row_loss;                                 // [T]
-  float* tape; float* g_top;                       // V > 64: [T][2], [T][k], or null
-  float* part;                                     // split rows: [T][S][2]
+  float* tape; float* g_top;                       // by wave: [T][2], [T][k], or null
+  long rows; bool by_thread; int S;                // of the whole call: its rows, their kernel, segments per row
+  float* part;                                     // S > 1: [T][S][2]
   double* sums;                                    // T > DISTILL_SUM_ROWS: [256][2]
   const float* wsum; const float* gloss; int gloss_rows; float scale;   // gradient: gloss or scale
   void* dx;

@@ -14,6 +14,8 @@
 // (one workgroup per row) read a row the second time while it is still in the caches.
 #include "scm_softmax.hpp"
 
+#include <algorithm>
+
 namespace scm {
 
 constexpr int DISTILL_SEGMENT = 131072;   // tokens whose bits fit a workgroup's 16 KB
@@ -103,7 +105,7 @@ SCM_DEV bool any_lane(bool b) { return __builtin_amdgcn_ballot_w64(b) != 0; }
 // weight of a row, and what its gradient is scaled by
 SCM_DEV float row_scale(const DistillTopkArgs& a, long row, float w) {
   const float g = a.gloss ? a.gloss[a.gloss_rows ? row : 0] : a.scale;
-  return g * w * a.inv_t / (a.mean ? (a.wsum ? a.wsum[0] : (float)a.T) : 1.f);
+  return g * w * a.inv_t / (a.mean ? (a.wsum ? a.wsum[0] : (float)a.rows) : 1.f);
 }
 
 // ---------------------------------------------------------------- statistics over R of a segment
@@ -520,14 +522,14 @@ static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
 }
 template <typename T, bool STREAM>
 static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s) {
-  if (logits_by_thread(a.T, a.V)) {
+  if (a.by_thread) {
     const dim3 g((unsigned)((a.T + 63) / 64));
     const unsigned lds = small_lds(a.V) + 64 * a.k * sizeof(double);   // 49 KB at most
     if (grad) hipLaunchKernelGGL((distill_small_kernel<T, true>), g, dim3(64), lds, s, a);
     else hipLaunchKernelGGL((distill_small_kernel<T, false>), g, dim3(64), lds, s, a);
     return;
   }
-  int S = distill_segments(a.T, a.V);
+  int S = a.S;
   if (S == 1 && loss && grad) {
     a.tape = a.g_top = nullptr;   // for a backward of its own only
     // (512 threads: two workgroups per CU, whose rows fit the last-level cache together; 256: 2048 x 131072 300 us, 512: 251 us)
@@ -576,10 +578,24 @@ static void distill_sized(const DistillTopkArgs& a, bool loss, bool grad, hipStr
   if (grad && a.T * a.V * (long)sizeof(T) > STREAM_BYTES) distill_typed<T, true>(a, loss, grad, s);
   else distill_typed<T, false>(a, loss, grad, s);
 }
-static void distill_dispatch(const DistillTopkArgs& a, bool loss, bool grad, hipStream_t s) {
-  if (a.type == SCM_F32) distill_sized<float>(a, loss, grad, s);
-  else if (a.type == SCM_BF16) distill_sized<bf16>(a, loss, grad, s);
-  else distill_sized<f16>(a, loss, grad, s);
+static void distill_dispatch(const DistillTopkArgs& all, bool loss, bool grad, hipStream_t s) {
+  const long size = all.type == SCM_F32 ? 4 : 2, most = std::max(LOGITS_LAUNCH_ROWS / all.S, 1L);
+  for (long t = 0; t < all.T; t += most) {
+    DistillTopkArgs a = all;   // n rows from row t on
+    a.T = std::min(all.T - t, most);
+    a.x = (const char*)a.x + t * a.ldx * size;
+    a.index += t * a.k;
+    a.lp += t * a.k;
+    if (a.weight) a.weight += t;
+    if (a.row_loss) a.row_loss += t;
+    if (a.tape) { a.tape += 2 * t; a.g_top += t * a.k; }
+    if (a.part) a.part += 2 * t * a.S;
+    if (a.gloss_rows) a.gloss += t;
+    if (a.dx) a.dx = (char*)a.dx + t * a.V * size;
+    if (a.type == SCM_F32) distill_sized<float>(a, loss, grad, s);
+    else if (a.type == SCM_BF16) distill_sized<bf16>(a, loss, grad, s);
+    else distill_sized<f16>(a, loss, grad, s);
+  }
 }
 // One workgroup adds up to 16384 rows; more of them (1,000,000 rows: 330 us) go through 4096-row parts at least.
 static void distill_sum(const DistillTopkArgs& a, const float* row_loss, const float* weight, int mean, float* out,

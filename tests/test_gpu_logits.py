@@ -355,6 +355,23 @@ def test_offsets_past_32_bits(token_logprobs):
     assert torch.equal(g[0], g[t // 2]) and abs(g[-1, 5].item()) < 1e-3
 
 
+def test_more_rows_than_a_launch(token_logprobs):
+    """the rows behind the first 2^21 against a call of their own"""
+    t, v, k = (1 << 21) + 1001, 65, 3
+    x = torch.randn(t, v, device=DEV).half()
+    target = torch.randint(0, v, (t,), device=DEV)
+    gl, gt = torch.randn(t, device=DEV), torch.randn(t, k, device=DEV)
+    def both(z, tg, a, b):
+        z = z.detach().requires_grad_()
+        o = token_logprobs(z, tg, k=k)
+        g, = torch.autograd.grad((o.logprob, o.entropy, o.top_logprob), z, (a, a, b))
+        return [e.detach() for e in o] + [g]
+    whole = both(x, target, gl, gt)
+    for cut in (slice(0, 700), slice((1 << 21) - 300, None)):
+        part = both(x[cut], target[cut], gl[cut], gt[cut])
+        assert all(torch.equal(a[cut], b) for a, b in zip(whole, part)), cut
+
+
 def test_refusals(token_logprobs):
     x = torch.randn(3, 20, device=DEV)
     t = torch.zeros(3, dtype=torch.int64, device=DEV)

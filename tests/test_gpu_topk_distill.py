@@ -314,6 +314,32 @@ def test_offsets_past_32_bits(L):
     assert torch.equal(g, dx) and torch.equal(loss, loss2)
 
 
+def test_more_rows_than_a_launch(L):
+    """the rows behind the first 2^21 against a call of their own"""
+    t, v = (1 << 21) + 1001, 65
+    x = torch.randn(t, v, device=DEV).half()
+    idx = torch.rand(t, v, device=DEV).topk(3, 1).indices
+    lp = torch.log_softmax(torch.randn(t, 4, device=DEV), 1)[:, :3].contiguous()
+    w = torch.rand(t, device=DEV)
+    gr = torch.randn(t, device=DEV)
+    def rows(cut):
+        z = x[cut].detach().requires_grad_()
+        o = L.topk_distillation(z, idx[cut], lp[cut], weight=w[cut], reduction="none")
+        g, = torch.autograd.grad(o, z, gr[cut])
+        loss, d = L.topk_distillation_grad(x[cut], idx[cut], lp[cut], weight=w[cut], reduction="sum")
+        return o.detach(), g, d, loss
+    whole = rows(slice(None))
+    for cut in (slice(0, 700), slice((1 << 21) - 300, None)):
+        part = rows(cut)
+        assert all(torch.equal(a[cut], b) for a, b in zip(whole[:3], part[:3])), cut
+    assert abs(whole[3].double() - whole[0].double().sum()) <= U * whole[0].double().sum()
+    # the mean without weights divides by all rows
+    loss, d = L.topk_distillation_grad(x, idx, lp)
+    plain, ds = L.topk_distillation_grad(x[-900:], idx[-900:], lp[-900:], reduction="sum")
+    want = ds.double() / t
+    assert (d[-900:].double() - want).abs().max() <= 2.0 ** -24        # both below the step of a subnormal half
+
+
 @pytest.mark.parametrize("t", [16384, 16385, 70001, 1_100_000])
 def test_sums_over_many_rows(L, t):
     """one workgroup's sum, and parts joined: rows of one known loss each, sums in 64 bits rounded once"""
