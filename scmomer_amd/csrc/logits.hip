@@ -370,38 +370,65 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a, int S) {
 }
 
 // ---------------------------------------------------------------- short rows, one thread each
-template <typename T, bool ENT>
+// N > 0: rows of at most N logits, which stay in registers between the passes; else they are read from LDS in each.
+template <typename T, bool ENT, int N>
 __global__ __launch_bounds__(64) void score_small_kernel(ScoreArgs a) {
   extern __shared__ uint32_t lds[];
   const int V = a.V, pitch = V | 1, rows = (int)min((long)64, a.T - (long)blockIdx.x * 64);
   const long row = (long)blockIdx.x * 64 + threadIdx.x;
+  const long long t = a.target && (int)threadIdx.x < rows ? a.target[row] : 0;   // on its way meanwhile
   stage_rows<const T, false>((const T*)a.x + (long)blockIdx.x * 64 * a.ldx, a.ldx, rows, V, lds, pitch);
   __syncthreads();
   if ((int)threadIdx.x >= rows) return;
   uint32_t* o = lds + threadIdx.x * pitch;
-  auto x = [&](int i) { return __uint_as_float(o[i]); };
+  float held[N > 0 ? N : 1];
+  if constexpr (N > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) held[i] = i < V ? __uint_as_float(o[i]) : -INFINITY;
+  }
+  const float xt = a.target && t >= 0 && t < V ? __uint_as_float(o[(int)t]) : 0.f;
+  auto each = [&](auto f) {   // f(i, x_i); past the end -inf, which adds nothing
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f(i, held[i]);
+    } else {
+#pragma unroll 8
+      for (int i = 0; i < V; ++i) f(i, __uint_as_float(o[i]));
+    }
+  };
   Stat st = stat_none();
-#pragma unroll 8
-  for (int i = 0; i < V; ++i) st.m = fmaxf(st.m, x(i));
-#pragma unroll 8
-  for (int i = 0; i < V; ++i) {
-    const float d = (x(i) - st.m) * a.c, e = exp2_fast(d);
+  each([&](int, float x) { st.m = fmaxf(st.m, x); });
+  each([&](int, float x) {
+    const float d = (x - st.m) * a.c, e = exp2_fast(d);
     st.s += e;
     if constexpr (ENT) st.h += e * fmaxf(d, -200.f);
-  }
-  const long long t = a.target ? a.target[row] : 0;
-  write_row<ENT>(a, row, st, a.target && t >= 0 && t < V ? x((int)t) : 0.f, t);
+  });
+  write_row<ENT>(a, row, st, xt, t);
   if (!a.k) return;
   const RowScore r(st, a.inv_t);
+  uint32_t order[N > 0 ? N : 1];
+  if constexpr (N > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) order[i] = i < V ? ordered(held[i]) : 0u;
+  } else {
 #pragma unroll 8
-  for (int i = 0; i < V; ++i) o[i] = ordered(x(i));
+    for (int i = 0; i < V; ++i) o[i] = ordered(__uint_as_float(o[i]));
+  }
   for (int j = 0; j < a.k; ++j) {   // k <= V selections, each taken out
     uint32_t b = 0;
     int bi = 0;
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (order[i] > b) { b = order[i]; bi = i; }
+#pragma unroll
+      for (int i = 0; i < N; ++i) order[i] = i == bi ? 0u : order[i];
+    } else {
 #pragma unroll 8
-    for (int i = 0; i < V; ++i)
-      if (o[i] > b) { b = o[i]; bi = i; }
-    o[bi] = 0;
+      for (int i = 0; i < V; ++i)
+        if (o[i] > b) { b = o[i]; bi = i; }
+      o[bi] = 0;
+    }
     a.top_index[row * a.k + j] = bi;
     a.top_logprob[row * a.k + j] = r.logp(unordered(b));
   }
@@ -524,13 +551,18 @@ static void launch_score(const ScoreArgs& a, int S, int len, hipStream_t s) {
   else if (a.k) hipLaunchKernelGGL((score_kernel<T, NT, EL, false, true>), g, b, 0, s, a, S, len);
   else hipLaunchKernelGGL((score_kernel<T, NT, EL, false, false>), g, b, 0, s, a, S, len);
 }
+template <typename T, int N>
+static void launch_score_small(const ScoreArgs& a, dim3 g, hipStream_t s) {
+  if (a.entropy) hipLaunchKernelGGL((score_small_kernel<T, true, N>), g, dim3(64), small_lds(a.V), s, a);
+  else hipLaunchKernelGGL((score_small_kernel<T, false, N>), g, dim3(64), small_lds(a.V), s, a);
+}
 template <typename T>
 static void score_typed(const ScoreArgs& a, hipStream_t s) {
   if (score_by_thread(a.T, a.V)) {
     const dim3 g((unsigned)((a.T + 63) / 64));
-    if (a.entropy) hipLaunchKernelGGL((score_small_kernel<T, true>), g, dim3(64), small_lds(a.V), s, a);
-    else hipLaunchKernelGGL((score_small_kernel<T, false>), g, dim3(64), small_lds(a.V), s, a);
-    return;
+    if (a.V <= 8) return launch_score_small<T, 8>(a, g, s);
+    if (a.V <= 16) return launch_score_small<T, 16>(a, g, s);
+    return launch_score_small<T, 0>(a, g, s);
   }
   int S = a.S;
   if (S > 1) {
