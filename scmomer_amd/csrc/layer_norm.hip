@@ -244,7 +244,13 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_bwd_kernel(const TY* __r
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           const float xh = ((float)buf[0].x[c].e[j] - mu) * rs;
-          o[j] = rs * ((float)buf[0].y[c].e[j] * g[c].e[j] - s1 - xh * s2);
+          float gd;
+          {
+#pragma clang fp contract(off)   // the product rounded as it was summed: one column's gradient is 0, not its rounding
+            gd = (float)buf[0].y[c].e[j] * g[c].e[j];
+            gd = gd - s1;
+          }
+          o[j] = rs * (gd - xh * s2);
         }
         cols.template store<STREAM>(dx + row * D, c, o);
       }

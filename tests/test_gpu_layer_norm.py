@@ -156,6 +156,17 @@ def test_strides_batches_and_offsets(layer_norm):
     assert all(torch.equal(ga[k], gb[k]) for k in ga)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_one_column(layer_norm, dtype):
+    """x - mean is 0: the result is the bias and x has no gradient, exactly"""
+    x, dy, w, b = _case(596, 1, dtype, 21)
+    x, w = x.requires_grad_(), (w + 0.3).requires_grad_()
+    y = layer_norm(x, w, b)
+    assert torch.equal(y, b.to(dtype).expand(596, 1))
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert not dx.any() and not dw.any()
+
+
 def test_no_rows(layer_norm):
     x = torch.empty(0, 40, device=DEV, requires_grad=True)
     w = torch.ones(40, device=DEV, requires_grad=True)
