@@ -493,11 +493,11 @@ __global__ __launch_bounds__(NT) void score_bwd_kernel(ScoreGradArgs a, int S, i
     const long long i = a.top_index[row * k + tid];
     float g = a.g_top[row * k + tid];
     if (r.has_target && i == r.target) { g += r.g_target; target_named = 1; }
-    if (i >= lo && i < lo + w.len) dx[i] = (T)(score_dx(r, (float)x[i], a.c) + g * a.inv_t);
+    if (i >= lo && i < lo + w.len) dx[i] = (T)add_product(score_dx(r, (float)x[i], a.c), g, a.inv_t);
   }
   __syncthreads();
   if (tid == 0 && r.has_target && !target_named && r.target >= lo && r.target < lo + w.len)
-    dx[r.target] = (T)(score_dx(r, (float)x[r.target], a.c) + r.g_target * a.inv_t);
+    dx[r.target] = (T)add_product(score_dx(r, (float)x[r.target], a.c), r.g_target, a.inv_t);
 }
 
 template <typename T>
@@ -509,8 +509,8 @@ __global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
   __syncthreads();
   if ((int)threadIdx.x < rows) {
     uint32_t* o = lds + threadIdx.x * pitch;
-    auto add = [&](long long i, float v) {
-      if (i >= 0 && i < V) o[i] = __float_as_uint(__uint_as_float(o[i]) + v);
+    auto add = [&](long long i, float g) {
+      if (i >= 0 && i < V) o[i] = __float_as_uint(add_product(__uint_as_float(o[i]), g, a.inv_t));
     };
     const int k = a.g_top ? a.k : 0;
     float gt = 0.f;
@@ -518,8 +518,8 @@ __global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
     const ScoreGrad r = score_grad(a, row, gt);
     for (int i = 0; i < V; ++i) o[i] = __float_as_uint(score_dx(r, __uint_as_float(o[i]), a.c));
     if (a.tape[2 * row + 1] != 0.f) {
-      for (int j = 0; j < k; ++j) add(a.top_index[row * k + j], a.g_top[row * k + j] * a.inv_t);
-      if (r.has_target) add(r.target, r.g_target * a.inv_t);
+      for (int j = 0; j < k; ++j) add(a.top_index[row * k + j], a.g_top[row * k + j]);
+      if (r.has_target) add(r.target, r.g_target);
     }
   }
   __syncthreads();

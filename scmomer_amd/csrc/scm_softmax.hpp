@@ -9,6 +9,13 @@ constexpr float LOWEST = -3.402823466e38f;
 constexpr float LN2 = 0.6931471805599453f;
 
 SCM_DEV float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+// a + b c with the product rounded, as the terms that may cancel it were: where one token has all the probability its
+// gradient is 0, not the rounding of a product.
+SCM_DEV float add_product(float a, float b, float c) {
+#pragma clang fp contract(off)
+  const float p = b * c;
+  return a + p;
+}
 
 // ---------------------------------------------------------------- softmax statistics
 // m: maximum of the elements (LOWEST where there are none above it), s = sum 2^((x-m)c), h = sum 2^((x-m)c) (x-m)c.

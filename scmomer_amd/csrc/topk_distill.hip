@@ -418,7 +418,7 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
         }
         if (!empty && !broken)
           each_entry(index, lps, a.k, [&](int j, long long i, float) {
-            o[i] = __float_as_uint(x((int)i) - (float)(q_of[64 * j] * per) * sc);
+            o[i] = __float_as_uint(add_product(x((int)i), -(float)(q_of[64 * j] * per), sc));
           });
       }
     } else if constexpr (GRAD) {

@@ -190,6 +190,26 @@ def test_capture_beside_an_eager_graph_of_the_same_leaf(M, name):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("t,v", [(5, 1), (600, 1), (5, 40), (20600, 40), (5, 700), (300, 9000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_one_token_with_all_the_probability(M, t, v, dtype):
+    """its log probability is 0 and nothing has a gradient, exactly"""
+    x = torch.full((t, v), float("-inf"), device=DEV, dtype=dtype)
+    at = torch.randint(0, v, (t,), device=DEV)
+    x.scatter_(1, at[:, None], torch.randn(t, 1, device=DEV).to(dtype))
+    z = x.requires_grad_()
+    o = M.token_logprobs(z, at, k=1, temperature=0.7)
+    g = torch.randn(3, t, device=DEV)
+    dx, = torch.autograd.grad((o.logprob, o.entropy), z, (g[0], g[1]))
+    assert torch.equal(o.top_index[:, 0], at) and not o.logprob.any() and not o.entropy.any() and not dx.any()
+    lp = -torch.rand(t, 1, device=DEV)
+    for tail in (True, False):
+        rows = M.topk_distillation(z, at[:, None], lp, temperature=0.7, tail=tail, reduction="none")
+        dz, = torch.autograd.grad(rows, z, g[2])
+        _, dx = M.topk_distillation_grad(z, at[:, None], lp, temperature=0.7, tail=tail, weight=g[2].abs())
+        assert torch.isfinite(rows).all() and not dz.any() and not dx.any()
+
+
 def test_inference_mode_and_no_grad(M):
     x, calls = _calls(M)
     z = x.detach().requires_grad_()
