@@ -236,6 +236,7 @@ struct DistillTopkArgs {
   float* part;                                     // S > 1: [T][S][2]
   double* sums;                                    // T > DISTILL_SUM_ROWS: [256][2]
   const float* wsum; const float* gloss; int gloss_rows; float scale;   // gradient: gloss or scale
+  bool sum_weights; const float* weights;          // every wave adds the weights of the whole call up by itself (wsum null)
   void* dx;
 };
 int distill_segments(long T, int V);

@@ -339,21 +339,19 @@ struct Distill {
   Tensor no_rows() const {   // an empty sum; its mean is 0 / 0
     return at::full({}, red == MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0, x.options().dtype(at::kFloat));
   }
-  // -> the loss (or the rows' losses, shaped as the logits' rows), the weights' sum, the tape
-  std::tuple<Tensor, Tensor, Tensor> forward(const Tensor& logits, bool backward_follows) const {
+  // -> the loss (or the rows' losses, shaped as the logits' rows), what the backward reads: the weights' sum, the tape
+  std::tuple<Tensor, Tensor> forward(const Tensor& logits, bool backward_follows) const {
     const c10::DeviceGuard guard(x.device());
-    const Tensor rows = red == NONE ? floats(x, row_shape(logits)) : floats(x, {t});
-    if (!t) return {red == NONE ? rows : no_rows(), Tensor(), Tensor()};
-    Tensor loss, wsum, tape;
-    if (red != NONE) loss = floats(x, {});
-    if (backward_follows) {
-      if (red != NONE) wsum = floats(x, {1});
-      tape = scratch(x, api.topk_distill_tape_floats(t, (int)v, (int)k));
-    }
-    const Tensor ws = scratch(x, api.topk_distill_ws_floats(t, (int)v));
-    call(with(api.topk_distill_fwd, ptr(rows), ptr(loss), ptr(wsum), ptr(tape), ptr(ws), stream_of(x)),
-         "scm_topk_distill_fwd");
-    return {red == NONE ? rows : loss, wsum, tape};
+    const Tensor out = floats(x, red == NONE ? row_shape(logits) : at::DimVector());
+    if (!t) return {red == NONE ? out : no_rows(), Tensor()};
+    Tensor keep;
+    if (backward_follows) keep = floats(x, {1 + api.topk_distill_tape_floats(t, (int)v, (int)k)});
+    const int64_t nws = api.topk_distill_ws_floats(t, (int)v);
+    const Tensor ws = scratch(x, nws + (red == NONE ? 0 : t));   // workspace (8-byte aligned), the rows' losses
+    float* const rows = red == NONE ? ptr(out) : ptr(ws) + nws;
+    call(with(api.topk_distill_fwd, rows, red == NONE ? nullptr : ptr(out), red == NONE ? nullptr : ptr(keep),
+              keep.defined() ? ptr(keep) + 1 : nullptr, ptr(ws), stream_of(x)), "scm_topk_distill_fwd");
+    return {out, keep};
   }
 };
 
@@ -362,8 +360,8 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
                         const OptTensor& weight_, double temperature, bool tail, int64_t red) {
     const Tensor weight = opt(weight_);
     const Distill op(logits, index, lp, weight, temperature, tail, (Reduction)red, false);
-    auto [loss, wsum, tape] = op.forward(logits, true);
-    ctx->save_for_backward({logits, index, lp, weight, wsum, tape});
+    auto [loss, keep] = op.forward(logits, true);
+    ctx->save_for_backward({logits, index, lp, weight, keep});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["opts"] = (int64_t)tail + 2 * red;
     return loss;
@@ -379,8 +377,9 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
     if (op.t) {
       const bool per_row = op.red == NONE;
       const Tensor g = grad_rows(grads[0], op.x, per_row ? op.t : 1);
-      call(op.with(api.topk_distill_bwd, ptr(saved[4]), ptr(g), (int)per_row, ptr(saved[5]), dx.data_ptr(),
-                   stream_of(op.x)), "scm_topk_distill_bwd");
+      float* const keep = ptr(saved[4]);
+      call(op.with(api.topk_distill_bwd, keep, ptr(g), (int)per_row, keep + 1, dx.data_ptr(), stream_of(op.x)),
+           "scm_topk_distill_bwd");
     }
     return {once(dx), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -405,10 +404,13 @@ std::tuple<Tensor, Tensor> topk_distillation_grad(const Tensor& logits, const Te
   Tensor dx = at::empty(logits.sizes(), op.x.options());
   if (!op.t) return {op.no_rows(), dx};
   Tensor loss = floats(op.x, {});
-  const Tensor buf = floats(op.x, {op.t + 1});   // the rows' losses, the sum of the weights
-  const Tensor tape = scratch(op.x, api.topk_distill_tape_floats(op.t, (int)op.v, (int)op.k));
-  const Tensor ws = scratch(op.x, api.topk_distill_ws_floats(op.t, (int)op.v));
-  call(op.with(api.topk_distill_step, (float)scale, ptr(buf), ptr(loss), ptr(buf) + op.t, ptr(tape), ptr(ws), dx.data_ptr(),
+  // one piece of scratch memory: workspace (8-byte aligned), tape, the rows' losses, the sum of the weights
+  const int64_t nws = api.topk_distill_ws_floats(op.t, (int)op.v);
+  const int64_t ntape = api.topk_distill_tape_floats(op.t, (int)op.v, (int)op.k);
+  const Tensor buf = floats(op.x, {nws + ntape + op.t + 1});
+  float* const ws = ptr(buf);
+  float* const rows = ws + nws + ntape;
+  call(op.with(api.topk_distill_step, (float)scale, rows, ptr(loss), rows + op.t, ws + nws, ws, dx.data_ptr(),
                stream_of(op.x)), "scm_topk_distill_step");
   return {loss, dx};
 }
