@@ -582,6 +582,13 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   // maxima bound them well.  bf16, k = 8: 20000 x 4000 55 us on 64 threads, 69 on 128; 6000 x 16000 52 on 128, 59 on 64, 58
   // on 256; 2048 x 65536 56 on 256, 58 on 128, 61 on 512; 1200 x 131072 68 on 512, 74 on 256.
   const long bytes = (long)a.V * sizeof(T);
+  // few rows: a row in one step of four waves.  bf16: 100 x 3000 k = 20 6.7 us, on 64 threads 8.7; 400 x 6613 k = 32 9.1 and
+  // 14.5; 1000 x 8000 k = 20 10.3 and 14.0, k = 2 10.7 and 9.6
+  if (a.T <= (a.k > 8 ? 1024 : 512) && a.V > 1024 && a.V <= 8192) {
+    if (a.V <= 2048) return launch_score<T, 256, 8>(a, 1, a.V, s);
+    if (a.V <= 4096) return launch_score<T, 256, 16>(a, 1, a.V, s);
+    return launch_score<T, 256>(a, 1, a.V, s);
+  }
   if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8>(a, 1, a.V, s);
   if (a.V <= 1024 && a.k <= 32) return launch_score<T, 64, 16>(a, 1, a.V, s);
   if (bytes <= 16384 && a.k <= 32) return launch_score<T, 64>(a, 1, a.V, s);

@@ -499,11 +499,11 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
 }
 
 // ---------------------------------------------------------------- host launchers
-// Segments per row: as for the scores, and never more tokens than the bits hold.  Loss of 400 x 50000 bf16 17 us in one
-// segment, 22 in three; loss and gradient 27 and 37 us.
+// Segments per row: as for the scores but for rows that one workgroup holds, and never more tokens than the bits take.  Loss
+// of 400 x 50000 bf16 17 us in one segment, 22 in three; loss and gradient 27 and 37; of 4 x 30000 fp16 11 and 13.
 int distill_segments(long T, int V) {
   const long least = (V + DISTILL_SEGMENT - 1) / DISTILL_SEGMENT;
-  if (V <= 8192 || logits_rows_fill(T, V)) return (int)least;
+  if (V <= 32768 || logits_rows_fill(T, V)) return (int)least;
   long s = (512 + T - 1) / T, most = (V + 2047) / 2048;
   if (s > most) s = most;
   if (s > LOGITS_MAX_SEGMENTS) s = LOGITS_MAX_SEGMENTS;
@@ -518,6 +518,16 @@ template <typename T, bool STREAM>
 static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
   constexpr int MAX = 64 / (32 * (int)sizeof(T) / 4);   // steps in 64 registers: 4 for 2-byte types, 2 for f32
   const dim3 g((unsigned)a.T);
+  // Few rows: a row in one step of a large workgroup.  fp16: 100 x 3000 7.2 us, on one wave 10.6; 1000 x 3000 10.5 and 12.8;
+  // 100 x 17339 12.3, in two steps of 256 threads 16.9, but 1000 x 17339 41 and 35.
+  if (a.V > 1024 && (a.V <= 8192 ? a.T <= 1024 : a.V <= 32768 && a.T <= 256)) {
+    if (a.V <= 256 * 8) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM, 8>), g, dim3(256), 0, s, a);
+    else if (a.V <= 256 * 16) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM, 16>), g, dim3(256), 0, s, a);
+    else if (a.V <= 256 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM>), g, dim3(256), 0, s, a);
+    else if (a.V <= 512 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 512, 1, STREAM>), g, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((distill_resident_kernel<T, 1024, 1, STREAM>), g, dim3(1024), 0, s, a);
+    return true;
+  }
   if (a.V <= 64 * 8) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM, 8>), g, dim3(64), 0, s, a);
   else if (a.V <= 64 * 16) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM, 16>), g, dim3(64), 0, s, a);
   else if (a.V <= 64 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM>), g, dim3(64), 0, s, a);
@@ -560,13 +570,16 @@ static void distill_typed(DistillTopkArgs a, bool loss, bool grad, hipStream_t s
       else if (len <= 4096) hipLaunchKernelGGL((distill_kernel<T, 256, 16, 128, false>), gs, dim3(256), 0, s, a, S, len);
       else hipLaunchKernelGGL((distill_kernel<T, 256, 32, DISTILL_SEGMENT / 32, false>), gs, dim3(256), 0, s, a, S, len);
       hipLaunchKernelGGL((distill_join_kernel<T>), g, dim3(64), 0, s, a, S);
+    } else if (a.T <= 1024 && a.V > 1024 && a.V <= 4096) {   // one step: 400 x 3000 fp16 6.8 us, on one wave 8.3
+      if (a.V <= 2048) hipLaunchKernelGGL((distill_kernel<T, 256, 8, 64, false>), g, dim3(256), 0, s, a, 1, a.V);
+      else hipLaunchKernelGGL((distill_kernel<T, 256, 16, 128, false>), g, dim3(256), 0, s, a, 1, a.V);
     } else if (a.V <= 512) {
       hipLaunchKernelGGL((distill_kernel<T, 64, 8, 16, false>), g, dim3(64), 0, s, a, 1, a.V);
     } else if (a.V <= 1024) {
       hipLaunchKernelGGL((distill_kernel<T, 64, 16, 32, false>), g, dim3(64), 0, s, a, 1, a.V);
-    } else if (a.V <= 8192) {   // one wave: 20000 x 4000 bf16 47 us, 256 threads 89 us; 10000 x 8000 42 and 48 us
+    } else if (a.V <= 8192 && a.T > 1024) {   // one wave: 20000 x 4000 bf16 47 us, 256 threads 89 us; 10000 x 8000 42 and 48 us
       hipLaunchKernelGGL((distill_kernel<T, 64, 32, 256, false>), g, dim3(64), 0, s, a, 1, a.V);
-    } else if (a.T <= 256) {   // a workgroup per CU: 100 x 131072 bf16 14.7 us, on 256 threads 20.3
+    } else if (a.T <= 256 && a.V > 8192) {   // a workgroup per CU: 100 x 131072 bf16 14.7 us, on 256 threads 20.3
       hipLaunchKernelGGL((distill_kernel<T, 512, 32, DISTILL_SEGMENT / 32, false>), g, dim3(512), 0, s, a, 1, a.V);
     } else {
       hipLaunchKernelGGL((distill_kernel<T, 256, 32, DISTILL_SEGMENT / 32, false>), g, dim3(256), 0, s, a, 1, a.V);

@@ -129,7 +129,8 @@ def test_loss_and_gradient(L, t, v, k, dtype, tail):
 
 # where rows are split, by the elements of a thread in a segment, and from where on they are not
 @pytest.mark.parametrize("t,v,k", [(40, 40003, 20), (30, 131072, 64), (63, 16906, 7), (64, 16906, 7), (64, 131072, 20),
-                                   (65, 131073, 5), (256, 140001, 3), (257, 50001, 12)])
+                                   (65, 131073, 5), (256, 140001, 3), (257, 50001, 12), (1024, 1500, 9), (1025, 1500, 9),
+                                   (1025, 2500, 64), (1024, 5003, 2), (1025, 5003, 2), (256, 16385, 4), (257, 12001, 4)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_few_rows(L, t, v, k, dtype):
     x, idx, lp, w = _case(t, v, k, dtype, t + v)
