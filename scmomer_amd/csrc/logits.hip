@@ -37,6 +37,7 @@ SCM_DEV uint64_t shfl64(uint64_t v, int mask) {
 // A lower bound of the k-th largest element comes free with the statistics: the k-th largest of the threads' maxima
 // (each thread's maximum is an element of its own).  Only the elements of threads whose maximum reaches it (k or a few
 // more) are looked at again, by the whole workgroup; what reaches the bound goes to LDS and is ranked there by counting.
+struct TopBound { uint32_t value; int chunk; };   // at least value, equal ones at chunks <= chunk
 template <int NT>
 struct TopLds {
   static constexpr int CAP = NT == 64 ? 512 : 1024;   // NT >= 2 k: about NT ln 2 + spread at most are expected
@@ -44,8 +45,7 @@ struct TopLds {
   uint32_t best[NT];
   int at[NT];
   int count, threads;
-  uint32_t thr;
-  int thr_at;
+  TopBound bound;
   uint64_t red[NT / 64];
   uint64_t picked[LOGITS_MAX_K + LOGITS_MAX_K / 8];
 };
@@ -53,27 +53,33 @@ struct TopLds {
 template <typename T> constexpr int order_spare = 0;
 template <> constexpr int order_spare<bf16> = 16;
 template <> constexpr int order_spare<f16> = 13;
+// Minimum and maximum over the 64 lanes, in every lane.
+template <int CTRL>
+SCM_DEV uint32_t dpp_move_u32(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
+SCM_DEV void wave_range(uint32_t& lo, uint32_t& hi) {
+  auto with = [&](uint32_t a, uint32_t b) { lo = min(lo, a); hi = max(hi, b); };
+  with(dpp_move_u32<0xB1>(lo), dpp_move_u32<0xB1>(hi));
+  with(dpp_move_u32<0x4E>(lo), dpp_move_u32<0x4E>(hi));
+  with(dpp_move_u32<0x141>(lo), dpp_move_u32<0x141>(hi));
+  with(dpp_move_u32<0x140>(lo), dpp_move_u32<0x140>(hi));
+  with((uint32_t)__shfl_xor((int)lo, 16), (uint32_t)__shfl_xor((int)hi, 16));
+  with((uint32_t)__shfl_xor((int)lo, 32), (uint32_t)__shfl_xor((int)hi, 32));
+}
 // Threshold (value, chunk) over the NT maxima, by the first wave: a value that k to k + k / 8 of them reach, found bit by
 // bit below the bits that they all share; among equal maxima (more than that reach the last value) the chunk up to which
 // the k-th place goes.  Threads without elements hold value 0.
-template <int NT>
-SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
-  constexpr int R = NT / 64;
-  const int l = threadIdx.x & 63;
-  uint32_t b[R], lo = 0xFFFFFFFFu, hi = 0;
-  int at[R];
+template <int R>
+SCM_DEV TopBound top_threshold(const uint32_t (&b)[R], const int (&at)[R], int k, int chunks, int spare) {
+  constexpr int NT = R * 64;
+  uint32_t lo = 0xFFFFFFFFu, hi = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    b[r] = L.best[r * 64 + l];
-    at[r] = L.at[r * 64 + l];
     lo = b[r] ? min(lo, b[r]) : lo;
     hi = max(hi, b[r]);
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, o));
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
-  }
+  wave_range(lo, hi);
+  lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)lo);
+  hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)hi);
   // all maxima lie in [lo, hi]; t keeps the invariant: reach of them are >= t, reach >= k (0: fewer than k threads hold
   // elements, then every element is a candidate)
   const int holders = min(chunks, NT);
@@ -81,6 +87,13 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
   uint32_t t = shared >= 32 || holders < k ? 0u : (hi >> shared) << shared;
   int reach = holders, above = 0, bit = holders < k ? -1 : shared - 1;
   const int enough = k + k / 8;
+  if (k == 1) {   // the maximum itself
+    t = hi;
+    reach = 0;
+    bit = -1;
+#pragma unroll
+    for (int r = 0; r < R; ++r) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b[r] == hi));
+  }
   for (; bit >= spare && reach > enough; --bit) {
     const uint32_t cand = t | (1u << bit);
     int n = 0;
@@ -103,7 +116,7 @@ SCM_DEV void top_threshold(TopLds<NT>& L, int k, int chunks, int spare) {
       if (n < need) lim = cand;
     }
   }
-  if (l == 0) { L.thr = t; L.thr_at = lim; }
+  return {t, lim};
 }
 
 // Many more candidates than places (rows with fewer chunks than places, ties): the first wave raises the bound to a key
@@ -154,29 +167,57 @@ SCM_DEV void top_of_segment(const W& w, int lo, int k, uint32_t best, int at, bo
   constexpr int E = W::E, U = W::U, SPARE = order_spare<T>;
   const int tid = threadIdx.x;
   const int chunks = (w.len + E - 1) / E;
-  L.best[tid] = best;
-  L.at[tid] = at;
-  if (tid == 0) L.count = L.threads = 0;
-  __syncthreads();
-  if (tid < 64) top_threshold<NT>(L, k, chunks, SPARE);
-  __syncthreads();
-  const uint32_t thr = L.thr, thr_top = thr | ((1u << SPARE) - 1u);
-  const int thr_at = L.thr_at;
+  TopBound bound;
+  if constexpr (NT == 64) {
+    const uint32_t b[1] = {best};
+    const int a[1] = {at};
+    bound = top_threshold(b, a, k, chunks, SPARE);
+    if (tid == 0) L.count = 0;
+  } else {
+    L.best[tid] = best;
+    L.at[tid] = at;
+    if (tid == 0) L.count = L.threads = 0;
+    __syncthreads();
+    if (tid < 64) {
+      uint32_t b[NT / 64];
+      int a[NT / 64];
+#pragma unroll
+      for (int r = 0; r < NT / 64; ++r) { b[r] = L.best[r * 64 + tid]; a[r] = L.at[r * 64 + tid]; }
+      bound = top_threshold(b, a, k, chunks, SPARE);
+      if (tid == 0) L.bound = bound;
+    }
+    __syncthreads();
+    bound = L.bound;
+  }
+  const uint32_t thr = bound.value, thr_top = thr | ((1u << SPARE) - 1u);
+  const int thr_at = bound.chunk;
   if (!odd) {
     // the threads that reach it, then their chunks (thread t: t, t + NT, ...) spread over the whole workgroup
-    auto in = [&](uint32_t o, int chunk) { return o > thr_top || (o >= thr && chunk <= thr_at); };
-    if (best && in(best, at)) L.at[atomicAdd(&L.threads, 1)] = tid;
-    __syncthreads();
+    const bool reaches = best && (best > thr_top || (best >= thr && at <= thr_at));
+    int threads;
+    if constexpr (NT == 64) {
+      const unsigned long mask = __builtin_amdgcn_ballot_w64(reaches);
+      if (reaches) L.at[__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] = tid;
+      threads = __builtin_popcountll(mask);
+      __syncthreads();
+    } else {
+      if (reaches) L.at[atomicAdd(&L.threads, 1)] = tid;
+      __syncthreads();
+      threads = L.threads;
+    }
     // the bounds as numbers (at or below the order of -inf: every element)
     const float from = thr <= 0x007FFFFFu ? -INFINITY : unordered(thr), above = unordered(thr_top + 1);
-    const int per = W::EL < 32 ? U : (chunks + NT - 1) / NT, pairs = L.threads * per;
+    const int per = W::EL < 32 ? U : (chunks + NT - 1) / NT, pairs = threads * per;
+    const float per_inv = 1.f / (float)per;
     for (int i = tid; i < pairs; i += NT) {
-      const int c = L.at[i / per] + NT * (i % per);
+      // i / per: (i + 1/2) / per lies 1 / (2 per) or more from a whole number, further than f32 rounds it for i < 2^20
+      const int nth = W::EL < 32 ? i / U : chunks < 1 << 20 ? (int)(((float)i + 0.5f) * per_inv) : i / per;
+      const int c = L.at[nth] + NT * (i - nth * per);
       const Chunk<T, E> raw = load_chunk<T, E>(w.p + (long)c * E, w.len - c * E);
-      const float bound = c <= thr_at ? from : above;
+      const float least = c <= thr_at ? from : above;
       uint32_t hits = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) hits |= (uint32_t)((float)raw.e[j] >= bound) << j;
+      for (int j = 0; j < E; ++j) hits |= (uint32_t)((float)raw.e[j] >= least) << j;
       if (w.len - c * E < E) hits &= (1u << max(w.len - c * E, 0)) - 1u;
       while (hits) {   // few: one read again each
         const int at_hit = c * E + __builtin_ctz(hits);
