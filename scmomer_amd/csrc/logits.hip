@@ -569,11 +569,11 @@ __global__ __launch_bounds__(64) void score_bwd_small_kernel(ScoreGradArgs a) {
 
 // ---------------------------------------------------------------- host launchers
 // Segments per row.  One where a row is short or the rows alone keep the card busy: one launch, no partial results (bf16,
-// k = 20: 400 x 131072 33 us against 40 us in 1200 segments; 100 x 131072 19 against 20 in 600; 64 x 65536 14 against 13
-// in 512).  Else about 512 workgroups (twice as many: 30 x 131072 15.1 us, against 14.7), of at least 2048 elements, and no
-// more than the join takes.
+// k = 20: 400 x 131072 32 us against 35 us in 800 segments, 400 x 50000 20 and 23; but 100 x 131072 19 and 18 in 600, 64 x
+// 65536 13.7 and 11.5 in 512).  Else about 512 workgroups (twice as many: 30 x 131072 15.1 us, against 14.7), of at least
+// 2048 elements, and no more than the join takes.
 int score_segments(long T, int V, int k) {
-  if (V <= 8192 || logits_rows_fill(T, V)) return 1;
+  if (V <= 8192 || logits_rows_fill(T, V, 128)) return 1;
   long s = (512 + T - 1) / T, most = (V + 2047) / 2048;
   if (s > most) s = most;
   if (s > LOGITS_MAX_SEGMENTS) s = LOGITS_MAX_SEGMENTS;
@@ -609,8 +609,7 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   if (S > 1) {
     const int len = segment_length(a.V, S);
     S = segments_used(a.V, len);
-    // a thread's elements by the segment: 3 x 131072 bf16, k = 20 in segments of 2048: 10.0 us with 32, 7.7 with 8; 1100
-    // segments of about 3000: 16.2 with 32, 10.2 with 16
+    // a thread's elements by the segment: 3 x 131072 bf16, k = 20 in segments of 2048 13.6 us with 32, 12.5 with 8
     if (len <= 2048) launch_score<T, 256, 8>(a, S, len, s);
     else if (len <= 4096) launch_score<T, 256, 16>(a, S, len, s);
     else launch_score<T, 256>(a, S, len, s);
@@ -620,11 +619,11 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   }
   // Threads per row by the row's bytes: more of them shorten the walk, fewer the reductions and the search for the
   // alternatives behind it, and leave more rows in flight; and at least two threads per alternative, so that the threads'
-  // maxima bound them well.  bf16, k = 8: 20000 x 4000 55 us on 64 threads, 69 on 128; 6000 x 16000 52 on 128, 59 on 64, 58
-  // on 256; 2048 x 65536 56 on 256, 58 on 128, 61 on 512; 1200 x 131072 68 on 512, 74 on 256.
+  // maxima bound them well.  bf16, k = 8: 20000 x 4000 52 us on 64 threads, 63 on 128; 6000 x 16000 50 on 128, 57 on 64, 55
+  // on 256; 2048 x 65536 54 on 256, 56 on 128, 59 on 512; 1200 x 131072 68 on 512, 72 on 256.
   const long bytes = (long)a.V * sizeof(T);
-  // few rows: a row in one step of four waves.  bf16: 100 x 3000 k = 20 6.7 us, on 64 threads 8.7; 400 x 6613 k = 32 9.1 and
-  // 14.5; 1000 x 8000 k = 20 10.3 and 14.0, k = 2 10.7 and 9.6
+  // few rows: a row in one step of four waves.  bf16: 100 x 3000 k = 20 7.2 us, on 64 threads 8.3; 400 x 6613 k = 32 8.5 and
+  // 15.0; 1000 x 8000 k = 20 10.1 and 13.7, k = 2 10.7 and 9.6
   if (a.T <= (a.k > 8 ? 1024 : 512) && a.V > 1024 && a.V <= 8192) {
     if (a.V <= 2048) return launch_score<T, 256, 8>(a, 1, a.V, s);
     if (a.V <= 4096) return launch_score<T, 256, 16>(a, 1, a.V, s);
@@ -633,7 +632,7 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
   if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8>(a, 1, a.V, s);
   if (a.V <= 1024 && a.k <= 32) return launch_score<T, 64, 16>(a, 1, a.V, s);
   if (bytes <= 16384 && a.k <= 32) return launch_score<T, 64>(a, 1, a.V, s);
-  // a workgroup per CU at most, and many alternatives: 64 x 65536 bf16, k = 64 15 us, on 256 threads 21 (k = 20: 15 and 15)
+  // a workgroup per CU at most, and many alternatives: 150 x 60000 bf16, k = 64 18 us, on 256 threads 22 (k = 20: 15 and 16)
   if (a.T <= 256 && a.V > 8192 && a.k > 32) return launch_score<T, 512>(a, 1, a.V, s);
   if (bytes <= 49152) return launch_score<T, 128>(a, 1, a.V, s);
   if (bytes <= 196608) return launch_score<T, 256>(a, 1, a.V, s);

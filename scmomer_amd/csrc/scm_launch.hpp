@@ -208,11 +208,11 @@ struct ScoreGradArgs {
   const float* g_logprob; const float* g_lse; const float* g_entropy; const float* g_top;   // each may be null
   void* dx;
 };
-// Rows that keep the card busy with one workgroup each.
-inline bool logits_rows_fill(long T, int V) { return T >= 256 || (T >= 64 && V <= 131072); }
+// Rows that keep the card busy with one workgroup each; few: rows of up to 131072 that do.
+inline bool logits_rows_fill(long T, int V, int few) { return T >= 256 || (T >= few && V <= 131072); }
 // Rows of at most 64 tokens: a thread per row (64 rows through LDS) where they are many.  Its time hardly grows with the
 // rows up to about 100000, that of the kernels for longer rows (a wave per row) does; by T / V the two cross at (f32, us):
-//   scores, k = 2      5000 x 64: 14 by thread,  9 by wave;  20000 x 64: 15 and 24;   5000 x 32: 8 and  9
+//   scores, k = 2      5000 x 64: 14 by thread,  8 by wave;  20000 x 64: 15 and 20;   5000 x 32: 8 and  8
 //   their gradient     5000 x 64: 14 and  5;                 20000 x 64: 15 and 11;  100000 x 64: 22 and 39
 //   distillation step  5000 x 64: 25 and 10;                 20000 x 64: 28 and 21;  100000 x 64: 35 and 62
 inline bool score_by_thread(long T, int V) { return V <= 64 && (V <= 16 || T > 128L * V); }

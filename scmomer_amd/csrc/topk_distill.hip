@@ -503,7 +503,7 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
 // of 400 x 50000 bf16 17 us in one segment, 22 in three; loss and gradient 27 and 37; of 4 x 30000 fp16 11 and 13.
 int distill_segments(long T, int V) {
   const long least = (V + DISTILL_SEGMENT - 1) / DISTILL_SEGMENT;
-  if (V <= 32768 || logits_rows_fill(T, V)) return (int)least;
+  if (V <= 32768 || logits_rows_fill(T, V, 64)) return (int)least;
   long s = (512 + T - 1) / T, most = (V + 2047) / 2048;
   if (s > most) s = most;
   if (s > LOGITS_MAX_SEGMENTS) s = LOGITS_MAX_SEGMENTS;

@@ -110,7 +110,8 @@ def test_scores_of_many_short_rows(token_logprobs, t, v, k, dtype):
 
 # where rows are split, by the elements of a thread in a segment, and from where on they are not
 @pytest.mark.parametrize("t,v,k", [(40, 16906, 20), (40, 40003, 20), (40, 40003, 0), (30, 131072, 64), (63, 65537, 64),
-                                   (64, 9001, 64), (64, 131072, 20), (64, 131073, 20), (200, 70001, 40), (255, 140001, 8),
+                                   (64, 9001, 64), (64, 131072, 20), (127, 131072, 20),
+                                   (128, 131072, 20), (128, 131073, 20), (200, 70001, 40), (255, 140001, 8),
                                    (256, 140001, 3), (257, 9000, 64), (512, 2500, 3), (513, 2500, 3), (513, 2500, 0),
                                    (1024, 5003, 20), (1025, 5003, 20), (1025, 1500, 9), (1025, 2500, 64)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
