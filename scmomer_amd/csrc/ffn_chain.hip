@@ -147,14 +147,22 @@ __global__ __launch_bounds__(512) void ffn_chain_kernel(FfnChainArgs a) {
     for (int m = 0; m < FC_KS; ++m)
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += xr[m][j >> 2][j & 3];
-    const float mean = xhalf_sum(s) * (1.f / D);
-    float q = 0.f;
+    const float sum = xhalf_sum(s), mean = sum * (1.f / D);
+    // the rounding is written out, as at rounded_mul: most columns keep the products in x - mean and in the square exact
+    auto centred = [&](int m, int j) {
+      const float x = xr[m][j >> 2][j & 3];
+      return m == 11 && j >= 6 ? rounded_sub(x, mean) : fmaf(-sum, 1.f / D, x);
+    };
+    float q = rounded_mul(centred(0, 1), centred(0, 1));
 #pragma unroll
     for (int m = 0; m < FC_KS; ++m)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float d = xr[m][j >> 2][j & 3] - mean;
-        q += (m < 12 || half == 0) ? d * d : 0.f;   // columns 200..207 do not exist
+        if (m == 0 && j == 1) continue;
+        const float d = centred(m, j);
+        if (m == 12) q += half == 0 ? rounded_mul(d, d) : 0.f;   // columns 200..207 do not exist
+        else if (m == 11 && j >= 6) q += rounded_mul(d, d);
+        else q = fmaf(d, d, q);
       }
     const float rstd = rsqrtf(xhalf_sum(q) * (1.f / D) + 1e-5f);
     const brsrc rH = make_rsrc(a.h, a.h ? (uint32_t)(((long)(a.M - 1) * a.ldh + D) * 2) : 0u);
@@ -171,7 +179,7 @@ __global__ __launch_bounds__(512) void ffn_chain_kernel(FfnChainArgs a) {
         const float g = j < 4 ? g0[j & 3] : g1[j & 3], b = j < 4 ? b0[j & 3] : b1[j & 3];
         const float c2 = j < 4 ? c0[j & 3] : c1[j & 3];
         const bool in = valid && (m < 12 || half == 0);
-        hv[j] = (bf16)(in ? (xv - mean) * rstd * g + b : 0.f);
+        hv[j] = (bf16)(in ? centred(m, j) * rstd * g + b : 0.f);
         // second-product accumulators start at residual + bias
         if (m < 12 || half == 0) fc_set(Y, m, j, xv + c2);
       }
@@ -256,13 +264,21 @@ __global__ __launch_bounds__(512) void ffn_chain_kernel(FfnChainArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (m < 12 || half == 0) s += fc_get(Y, m, j);
-      mean = xhalf_sum(s) * (1.f / D);
-      float q = 0.f;
+      const float sum = xhalf_sum(s);
+      mean = sum * (1.f / D);
+      const float d1 = fmaf(-sum, 1.f / D, fc_get(Y, 0, 1));
+      float q = rounded_mul(d1, d1);
 #pragma unroll
       for (int m = 0; m < FC_KS; ++m)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (m < 12 || half == 0) { const float d = fc_get(Y, m, j) - mean; q += d * d; }
+          if (m < 11) {
+            const float d = fmaf(-sum, 1.f / D, fc_get(Y, m, j));
+            if (m != 0 || j != 1) q = fmaf(d, d, q);
+          } else if (m < 12 || half == 0) {
+            const float d = rounded_sub(fc_get(Y, m, j), mean);
+            q += rounded_mul(d, d);
+          }
       rstd = rsqrtf(xhalf_sum(q) * (1.f / D) + 1e-5f);
     }
     const brsrc rHn = make_rsrc(a.h_n, ln_next ? (uint32_t)(((long)(a.M - 1) * a.ldhn + D) * 2) : 0u);

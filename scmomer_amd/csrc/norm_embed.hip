@@ -16,6 +16,7 @@ constexpr float LN_EPS = 1e-5f;
 constexpr int MAXV = 8;    // token vocabulary bound (num_tokens = 7)
 constexpr int MAXC = 8;    // head classes bound
 
+// The rounding of the sums below is written out, as at rounded_mul.
 struct RowStats { float mean, rstd; };
 
 SCM_DEV RowStats row_stats(const f32x4& x, bool active, int D) {
@@ -24,7 +25,7 @@ SCM_DEV RowStats row_stats(const f32x4& x, bool active, int D) {
   float q = 0.f;
   if (active) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { const float d = x[j] - mean; q += d * d; }
+    for (int j = 0; j < 4; ++j) { const float d = x[j] - mean; q += rounded_mul(d, d); }
   }
   const float var = wave_sum(q) / (float)D;
   return {mean, rsqrtf(var + LN_EPS)};
@@ -144,9 +145,9 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const float* __restrict__ d
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       xh[j] = (v[j] - mu) * rs;
-      gd[j] = d[j] * g[j];
+      gd[j] = rounded_mul(d[j], g[j]);
       s1 += gd[j];
-      s2 += gd[j] * xh[j];
+      s2 += rounded_mul(gd[j], xh[j]);
     }
     if (!active) { s1 = 0.f; s2 = 0.f; }
     s1 = wave_sum(s1) * invD;
@@ -155,8 +156,8 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const float* __restrict__ d
       f32x4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        o[j] = r[j] + rs * (gd[j] - s1 - xh[j] * s2);
-        ag[j] += d[j] * xh[j];
+        o[j] = fmaf(rs, fmaf(-xh[j], s2, rounded_sub(gd[j], s1)), r[j]);
+        ag[j] = fmaf(d[j], xh[j], ag[j]);
         ab[j] += d[j];
         ar[j] += r[j];
       }
@@ -300,7 +301,11 @@ __global__ __launch_bounds__(256) void head_bwd_kernel(const float* __restrict__
     f32x4 gd;
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { gd[j] = d[j] * g[j]; s1 += gd[j]; s2 += gd[j] * xh[j]; }
+    for (int j = 0; j < 4; ++j) {
+      gd[j] = rounded_mul(d[j], g[j]);
+      s1 += gd[j];
+      s2 += rounded_mul(gd[j], xh[j]);
+    }
     if (!active) { s1 = 0.f; s2 = 0.f; }
     s1 = wave_sum(s1) * invD;
     s2 = wave_sum(s2) * invD;
@@ -308,8 +313,8 @@ __global__ __launch_bounds__(256) void head_bwd_kernel(const float* __restrict__
       f32x4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        o[j] = rs * (gd[j] - s1 - xh[j] * s2);
-        ag[j] += d[j] * xh[j];
+        o[j] = rs * fmaf(-xh[j], s2, rounded_sub(gd[j], s1));
+        ag[j] = fmaf(d[j], xh[j], ag[j]);
         ab[j] += d[j];
       }
       *(f32x4*)(dx + t * D + 4 * l) = o;

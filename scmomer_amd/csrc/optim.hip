@@ -100,10 +100,10 @@ __global__ __launch_bounds__(256) void adam_update_kernel(const AdamItem* __rest
   const float gs = k.grad_scale * scal[0];
   const AdamItem it = items[blockIdx.x];
   for (int i = threadIdx.x; i < it.n; i += 256) {
-    const float g = it.g[i] * gs;
+    const float raw = it.g[i], g = raw * gs;
     float m = it.m[i], v = it.v[i];
-    m = m + (g - m) * k.one_minus_beta1;
-    v = v * k.beta2 + k.one_minus_beta2 * g * g;
+    m = m + rounded_mul(fmaf(raw, gs, -m), k.one_minus_beta1);   // the rounding is written out, as at rounded_mul
+    v = fmaf(g, k.one_minus_beta2 * g, rounded_mul(v, k.beta2));
     const float denom = sqrtf(v) / k.bc2_sqrt + k.eps;
     it.p[i] = it.p[i] - k.step_size * (m / denom);
     it.m[i] = m;

@@ -46,6 +46,18 @@ SCM_DEV f32x16 zero16() {
   return z;
 }
 
+// A product or difference that is not merged into an operation around it.  Where sums of products feed a LayerNorm or a
+// weight, which products are merged (fmaf) and which are rounded first is written out: left to the compiler it changes with
+// the instructions it may pair, and a LayerNorm output moved to its neighbour moves the gradients behind it.
+SCM_DEV float rounded_mul(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+SCM_DEV float rounded_sub(float a, float b) {
+#pragma clang fp contract(off)
+  return a - b;
+}
+
 SCM_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 SCM_DEV float xhalf_sum(float v) { return v + __shfl_xor(v, 32); }
