@@ -8,6 +8,8 @@
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <limits>
@@ -86,6 +88,26 @@ Tensor grad_rows(const Tensor& g, const Tensor& like, int64_t n) {
   return g.to(at::kFloat).contiguous();
 }
 
+// The kernels work on addresses: what hands tensors on without values, or follows a call by its torch operations, sees
+// nothing of them.  Refused are tensors of forward-mode differentiation (their tangent would be lost), tensors with a
+// dispatch of their own (a wrapper has no memory), and calls under a tracer (it would record the allocation of the
+// results only).
+void check_followed(std::initializer_list<std::reference_wrapper<const Tensor>> tensors) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  bool traced = torch::jit::tracer::isTracing();
+  if (TorchDispatchModeTLS::any_modes_set())
+    for (const auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+      traced = traced || TorchDispatchModeTLS::get_mode(key).has_value();
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced, "this operator of scmomer_amd cannot be traced");
+  for (const Tensor& t : tensors) {
+    if (!t.defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "this operator of scmomer_amd has no forward-mode derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.key_set().has(c10::DispatchKey::Python),
+                                "this operator of scmomer_amd takes plain tensors, not subclasses with a dispatch of their own");
+  }
+}
+
 // Gradients that came out of a backward pass under create_graph: they refuse to be differentiated again.
 struct FirstOnly : torch::autograd::Function<FirstOnly> {
   static Tensor forward(AutogradContext*, const Tensor& g) { return g.view_as(g); }
@@ -158,6 +180,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_followed({grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &x_ = saved[0], &w = saved[1], &st = saved[2];
     const Tensor x = rows_of(x_, "x"), dy = rows_of(grads[0], "dy");
@@ -186,6 +209,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps,
                   std::optional<at::ScalarType> out_dtype) {
   const Tensor w = opt(weight), b = opt(bias);
+  check_followed({x, w, b});
   if (at::GradMode::is_enabled() && (needs_grad(x) || needs_grad(w) || needs_grad(b)))
     return LayerNorm::apply(x, weight, bias, eps, out_dtype);
   return std::get<0>(norm_fwd(x, w, b, eps, out_dtype, false));
@@ -251,6 +275,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    for (const Tensor& g : grads) check_followed({g});
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &entropy = saved[2], &top_index = saved[3], &tape = saved[4];
     const double temperature = ctx->saved_data["temperature"].toDouble();
@@ -280,6 +305,7 @@ std::tuple<OptTensor, OptTensor, Tensor, OptTensor, OptTensor> token_logprobs(co
                                                                             int64_t k, double temperature, int64_t ignore,
                                                                             bool entropy) {
   const Tensor targets = opt(targets_);
+  check_followed({logits, targets});
   auto maybe = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
   if (!(at::GradMode::is_enabled() && logits.requires_grad())) {
     const Score o = score_fwd(logits, targets, k, temperature, ignore, entropy, false);
@@ -367,6 +393,7 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_followed({grads[0]});
     const auto saved = ctx->get_saved_variables();
     const int64_t opts = ctx->saved_data["opts"].toInt();
     const Distill op(saved[0], saved[1], saved[2], saved[3], ctx->saved_data["temperature"].toDouble(), opts & 1,
@@ -388,9 +415,11 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
 Tensor topk_distillation(const Tensor& logits, const Tensor& index, const Tensor& lp, double temperature, bool tail,
                          const OptTensor& weight, const std::string& reduction) {
   const Reduction red = reduction_of(reduction);
+  const Tensor w = opt(weight);
+  check_followed({logits, index, lp, w});
   if (at::GradMode::is_enabled() && logits.requires_grad())
     return TopkDistillation::apply(logits, index, lp, weight, temperature, tail, (int64_t)red);
-  return std::get<0>(Distill(logits, index, lp, opt(weight), temperature, tail, red, false).forward(logits, false));
+  return std::get<0>(Distill(logits, index, lp, w, temperature, tail, red, false).forward(logits, false));
 }
 
 std::tuple<Tensor, Tensor> topk_distillation_grad(const Tensor& logits, const Tensor& index, const Tensor& lp,
@@ -399,7 +428,9 @@ std::tuple<Tensor, Tensor> topk_distillation_grad(const Tensor& logits, const Te
   const Reduction red = reduction_of(reduction);
   TORCH_CHECK_VALUE(red != NONE, "topk_distillation_grad: reduction must be 'mean' or 'sum'");
   const at::NoGradGuard no_grad;
-  const Distill op(logits, index, lp, opt(weight), temperature, tail, red, false);
+  const Tensor w = opt(weight);
+  check_followed({logits, index, lp, w});
+  const Distill op(logits, index, lp, w, temperature, tail, red, false);
   const c10::DeviceGuard guard(op.x.device());
   Tensor dx = at::empty(logits.sizes(), op.x.options());
   if (!op.t) return {op.no_rows(), dx};
@@ -443,6 +474,8 @@ PYBIND11_MODULE(_torch_ops, m) {
       PyErr_SetString(PyExc_TypeError, e.what_without_backtrace());
     } catch (const c10::ValueError& e) {
       PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
+    } catch (const c10::NotImplementedError& e) {
+      PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
     }
   });
   m.def("bind", &bind);

@@ -18,6 +18,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     x: f32, bf16 or fp16 on the GPU, 1 <= D <= 16384, any row stride (other layouts are copied first); weight, bias:
     f32 [D] or None (1, 0).  The result has x's type, or bfloat16 from f32 with ``out_dtype=torch.bfloat16``;
     statistics and the gradients of weight and bias are f32.  Gradients do not depend on the order in which
-    workgroups run.  First derivatives only.  A backward pass under capture into a graph is refused while an eager graph
+    workgroups run.  First derivatives only, in reverse mode: under forward-mode differentiation, a tracer (torch.jit.trace,
+    make_fx) or with tensor subclasses that have a dispatch of their own it raises NotImplementedError.  A backward pass under capture into a graph is refused while an eager graph
     on the default stream holds the same leaves (their gradients would have to join that stream)."""
     return torch_ops.layer_norm(x, weight, bias, eps, out_dtype)
