@@ -39,13 +39,24 @@ SCM_DEV double wave_sum_f64(double v) {
   v += __shfl_xor(v, 32);
   return v;
 }
+// Entries of less mass than this together are renormalised relative to the largest of them: their sum and its logarithm
+// would leave the range of f32, and from exp(-745) on of f64.
+constexpr double HARDLY_ANY_MASS = 0x1p-60;
 // rest: statistics over R.  idx (-1: unused), lp, x (the student's logit there) of this lane's entry.  beyond: some index
 // lies outside the vocabulary (such entries come as unused).  twice: some token may be named more than once.
 SCM_DEV DistillRow distill_row(const DistillTopkArgs& a, const Stat& rest, int idx, float lp, float x, bool beyond, bool twice) {
   const int lane = threadIdx.x & 63;
   const bool used = idx >= 0;
   double q = used ? exp((double)lp) : 0.0;
-  const double total = wave_sum_f64(q);
+  double total = wave_sum_f64(q);
+  if (!a.tail && total < HARDLY_ANY_MASS) {   // the same in all lanes
+    const float top = wave_max(used ? lp : -INFINITY);
+    if (top > -INFINITY) {
+      lp -= top;
+      q = used ? exp((double)lp) : 0.0;
+      total = wave_sum_f64(q);
+    }
+  }
   float r = 0.f, big_a;
   if (a.tail) {
     r = rest.s == 0.f ? 0.f : (float)fmax(0.0, 1.0 - total);
@@ -392,6 +403,21 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
         q_of[64 * j] = q;
         total += q;
       });
+      float top = 0.f;   // what the log probabilities are relative to
+      if (!a.tail && total < HARDLY_ANY_MASS) {
+        float most = -INFINITY;
+        each_entry(index, lps, a.k, [&](int, long long i, float lp) { if (i < V) most = fmaxf(most, lp); });
+        if (most > -INFINITY) {
+          top = most;
+          total = 0.0;
+          each_entry(index, lps, a.k, [&](int j, long long i, float lp) {
+            if (i >= V) return;
+            const double q = exp((double)(lp - top));
+            q_of[64 * j] = q;
+            total += q;
+          });
+        }
+      }
       Stat all = stat_none(), rest = stat_none();
 #pragma unroll 8
       for (int i = 0; i < V; ++i) {
@@ -412,7 +438,7 @@ __global__ __launch_bounds__(64) void distill_small_kernel(DistillTopkArgs a) {
       each_entry(index, lps, a.k, [&](int j, long long i, float lp) {
         if (i >= V) return;
         const float q = (float)(q_of[64 * j] * per);
-        if (q > 0.f) loss += q * (lp - log_total - ((x((int)i) - all.m) * a.inv_t - LN2 * l2));
+        if (q > 0.f) loss += q * (lp - top - log_total - ((x((int)i) - all.m) * a.inv_t - LN2 * l2));
       });
       if (r > 0.f) loss += r * (logf(r) - ((rest.m - all.m) * a.inv_t + LN2 * (log2_fast(rest.s) - l2)));
       const bool empty = all.s == 0.f, broken = beyond || total != total || all.s != all.s;
