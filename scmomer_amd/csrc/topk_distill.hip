@@ -663,7 +663,7 @@ static void distill_sum(const DistillTopkArgs& a, const float* row_loss, const f
 hipError_t topk_distill_fwd(const DistillTopkArgs& a, float* out, float* wsum_out, hipStream_t s) {
   Traced tr(K_TOPK_DISTILL, 0, s);
   distill_dispatch(a, true, false, s);
-  if (out) distill_sum(a, a.row_loss, a.weight, a.mean, out, wsum_out, s);
+  if (out || wsum_out) distill_sum(a, out ? a.row_loss : nullptr, a.weight, a.mean, out, wsum_out, s);
   return hipGetLastError();
 }
 hipError_t topk_distill_bwd(const DistillTopkArgs& a, hipStream_t s) {
@@ -678,10 +678,11 @@ hipError_t topk_distill_step(const DistillTopkArgs& all, float* out, float* wsum
   DistillTopkArgs a = all;
   a.sum_weights = a.weight && a.mean && !a.by_thread && a.rows <= 1024;
   a.weights = a.weight;
+  const bool first = a.weight && a.mean && !a.sum_weights;
   if (a.sum_weights) a.wsum = nullptr;
-  else if (a.weight && a.mean) distill_sum(a, nullptr, a.weight, 0, nullptr, wsum, s);
+  else if (first) distill_sum(a, nullptr, a.weight, 0, nullptr, wsum, s);
   distill_dispatch(a, true, true, s);
-  distill_sum(a, a.row_loss, a.weight, a.mean, out, a.sum_weights ? wsum : nullptr, s);
+  distill_sum(a, a.row_loss, a.weight, a.mean, out, first ? nullptr : wsum, s);
   return hipGetLastError();
 }
 

@@ -46,3 +46,28 @@ def test_renormalised_entries_of_hardly_any_mass(L, t, v, k, top):
     xg = x.detach().requires_grad_()
     d2, = torch.autograd.grad(L.topk_distillation(xg, idx, lp, tail=False, weight=w, reduction="sum"), xg)
     _within(d2, g, gtol + 8 * U * g.abs() + 2.0 ** -126, "dx")
+
+
+@pytest.mark.parametrize("t,v", [(5, 40), (21000, 40), (700, 900), (1025, 900), (17000, 100), (3, 100000)])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("mean", [0, 1])
+def test_the_sum_of_the_weights_is_written(t, v, weighted, mean):
+    """by both entry points whenever there is room for it, with and without a loss; U relative: a 64-bit sum rounded once"""
+    from scmomer_amd._lib import check, lib
+    k = 3
+    x, idx, lp, w = _case(t, v, k, torch.float32, t + v)
+    want = w.double().sum() if weighted else torch.tensor(float(t), dtype=torch.float64, device=DEV)
+    p = lambda a: a.data_ptr() if a is not None else None
+    head = (p(x), 0, v, t, v, 1.0, p(idx), p(lp), k, 1, p(w) if weighted else None, mean)
+    rows = torch.empty(t, device=DEV)
+    tape = torch.empty(max(1, lib.scm_topk_distill_tape_floats(t, v, k)), device=DEV)
+    ws = torch.empty(lib.scm_topk_distill_ws_floats(t, v) + 2, device=DEV)
+    loss, dx = torch.empty((), device=DEV), torch.empty_like(x)
+    s = torch.cuda.current_stream().cuda_stream
+    for out in (None, loss):
+        wsum = torch.full((), -7.0, device=DEV)
+        check(lib.scm_topk_distill_fwd(*head, p(rows), p(out), p(wsum), p(tape), p(ws), s), "fwd")
+        assert abs(wsum.double() - want) <= U * want, out
+    wsum = torch.full((), -7.0, device=DEV)
+    check(lib.scm_topk_distill_step(*head, 1.0, p(rows), p(loss), p(wsum), p(tape), p(ws), p(dx), s), "step")
+    assert abs(wsum.double() - want) <= U * want
