@@ -49,8 +49,15 @@ int type_of(const Tensor& t, const char* name) {
     default: TORCH_CHECK_TYPE(false, name, ": expected float32, bfloat16 or float16, got ", t.scalar_type());
   }
 }
+// A tensor whose memory holds its values: a view that only notes a change of sign (the imaginary part of a conjugate) and
+// a gradient that is only noted to be zero get theirs written.
+Tensor values(const Tensor& t) {
+  if (!t.defined()) return t;
+  return t.is_neg() ? t.resolve_neg() : t._is_zerotensor() ? t.clone() : t;
+}
 // [T, D] form of [..., D]: a view where one row stride describes it (an expanded batch keeps stride 0), else a copy
-Tensor rows_of(const Tensor& t, const char* name) {
+Tensor rows_of(const Tensor& t_, const char* name) {
+  const Tensor t = values(t_);
   type_of(t, name);
   TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) >= 1, name, ": expected [..., D] with D >= 1, got ", t.sizes());
   Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
@@ -78,14 +85,14 @@ Tensor row_vector(const Tensor& t, const Tensor& logits, at::ScalarType type, co
   TORCH_CHECK_VALUE(t.sizes() == logits.sizes().slice(0, logits.dim() - 1), name, ": expected ",
                     logits.sizes().slice(0, logits.dim() - 1), ", got ", t.sizes());
   on_device_of(logits, t, name);
-  return t.contiguous();
+  return values(t).contiguous();
 }
 // an incoming gradient as n contiguous f32 values (undefined: none)
 Tensor grad_rows(const Tensor& g, const Tensor& like, int64_t n) {
   if (!g.defined()) return g;
   TORCH_CHECK_VALUE(g.numel() == n, "incoming gradient: ", g.numel(), " values, expected ", n);
   on_device_of(like, g, "incoming gradient");
-  return g.to(at::kFloat).contiguous();
+  return values(g).to(at::kFloat).contiguous();
 }
 
 // The kernels work on addresses: what hands tensors on without values, or follows a call by its torch operations, sees
@@ -145,9 +152,9 @@ void check_capture(const Tensor& t) {
 
 // ---------------------------------------------------------------------------- layer norm
 // -> y, statistics [2, T] (mean, 1 / standard deviation)
-std::tuple<Tensor, Tensor> norm_fwd(const Tensor& x_, const Tensor& w, const Tensor& b, double eps,
+std::tuple<Tensor, Tensor> norm_fwd(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps,
                                     std::optional<at::ScalarType> out_dtype, bool stats) {
-  const Tensor x = rows_of(x_, "x");
+  const Tensor x = rows_of(x_, "x"), w = values(w_), b = values(b_);
   const int64_t t = x.size(0), d = x.size(1);
   const auto out = out_dtype.value_or(x.scalar_type());
   TORCH_CHECK_TYPE(out == x.scalar_type() || (x.scalar_type() == at::kFloat && out == at::kBFloat16), "layer norm: ",
@@ -182,8 +189,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_followed({grads[0]});
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x_ = saved[0], &w = saved[1], &st = saved[2];
-    const Tensor x = rows_of(x_, "x"), dy = rows_of(grads[0], "dy");
+    const Tensor &x_ = saved[0], &st = saved[2];
+    const Tensor x = rows_of(x_, "x"), w = values(saved[1]), dy = rows_of(grads[0], "dy");
     on_device_of(x, dy, "dy");
     const int64_t t = x.size(0), d = x.size(1);
     // edges count the tensors that were given
@@ -281,7 +288,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     const double temperature = ctx->saved_data["temperature"].toDouble();
     const int64_t k = top_index.defined() ? top_index.size(-1) : 0;
     const Tensor x = rows_of(logits, "logits");
-    const Tensor targets = saved[1].defined() ? saved[1].contiguous() : saved[1];
+    const Tensor targets = saved[1].defined() ? values(saved[1]).contiguous() : saved[1];
     const int64_t t = x.size(0), v = x.size(1);
     size_t i = 0;
     const Tensor none;
@@ -351,8 +358,8 @@ struct Distill {
     x = checked ? rows_of(logits, "logits") : logits_rows(logits, temperature, k);
     on_device_of(x, index_, "top_index");
     on_device_of(x, lp_, "top_logprob");
-    index = index_.contiguous();
-    lp = lp_.contiguous();
+    index = values(index_).contiguous();
+    lp = values(lp_).contiguous();
     weight = row_vector(weight_, logits, at::kFloat, "weight");
     t = x.size(0);
     v = x.size(1);

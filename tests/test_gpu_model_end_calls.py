@@ -62,3 +62,42 @@ def test_a_mode_that_only_counts_changes_nothing(M, name):
         got = calls[name](z)
         dg, = torch.autograd.grad(got.sum(), z)
     assert torch.equal(want, got) and torch.equal(dw, dg)
+
+
+def _negated(shape, seed):
+    """f32 of that shape whose memory holds the values with the other sign (a view that notes the change only)"""
+    gen = torch.Generator().manual_seed(seed)
+    z = torch.complex(torch.zeros(shape), torch.randn(shape, generator=gen)).to(DEV)
+    n = z.conj().imag
+    assert n.is_neg()
+    return n, n.clone().resolve_neg()
+
+
+def test_views_that_note_a_sign(M):
+    """every operand with one element a row or one element at all, where no copy for its stride would write the sign"""
+    for t in (1, 5):
+        n, x = _negated((t, 1), t)
+        assert torch.equal(M.token_logprobs(n).lse, M.token_logprobs(x).lse)
+        idx, lp, w = torch.zeros(t, 1, dtype=torch.int64, device=DEV), torch.zeros(t, 1, device=DEV), torch.ones(t, device=DEV)
+        y = torch.ones(t, 1, device=DEV)
+        assert torch.equal(M.topk_distillation(y, idx, n, reduction="none"), M.topk_distillation(y, idx, x, reduction="none"))
+        n1, x1 = _negated((1,), 7)
+        for a, b in ((M.layer_norm(n, n1, n1), M.layer_norm(x, x1, x1)), (M.layer_norm(y, None, n1), M.layer_norm(y, None, x1)),
+                     (M.topk_distillation(y[:1], idx[:1], lp[:1] - 1, tail=True, weight=n1, reduction="sum"),
+                      M.topk_distillation(y[:1], idx[:1], lp[:1] - 1, tail=True, weight=x1, reduction="sum"))):
+            assert torch.equal(a, b)
+        z = y.clone().requires_grad_()
+        b = torch.zeros(1, device=DEV, requires_grad=True)
+        for f, v in ((lambda: M.layer_norm(z, None, b), b), (lambda: M.token_logprobs(z).lse[:, None], z)):
+            want, = torch.autograd.grad(f(), v, x)
+            got, = torch.autograd.grad(f(), v, n)
+            assert torch.equal(want, got) and want.abs().max() > 0
+
+
+@pytest.mark.parametrize("name", ["norm", "score", "entropy", "distill"])
+def test_an_incoming_gradient_that_is_only_noted_to_be_zero(M, name):
+    x, calls = _calls(M)
+    z = x.detach().requires_grad_()
+    y = calls[name](z)
+    g, = torch.autograd.grad(y, z, torch._efficientzerotensor(tuple(y.shape), device=DEV))
+    assert g.shape == x.shape and not g.any()
