@@ -14,6 +14,8 @@
 #include <cmath>
 #include <limits>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 namespace {
 
@@ -129,7 +131,8 @@ Tensor once(const Tensor& g) {
 
 // A leaf's accumulator keeps the stream of the graph that made it for as long as a graph holds it.  Where that is the default
 // stream, a backward pass under capture would make that stream wait for a captured event, which no capture allows and
-// which ends the process.  Called by the node whose gradients are due, before anything is launched.
+// which ends the process.  Called by the node whose gradients are due, before anything is launched, for all that this
+// backward pass reaches from there: the leaves of a whole model.
 void check_capture(const Tensor& t) {
   const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -138,15 +141,22 @@ void check_capture(const Tensor& t) {
     (void)hipGetLastError();
     return;
   }
-  const auto node = torch::autograd::get_current_node();
-  if (status == hipStreamCaptureStatusNone || !node) return;
-  for (uint32_t i = 0; i < node->num_outputs(); ++i) {
-    const auto& e = node->next_edge(i);
-    if (!e.function || !node->task_should_compute_output(i)) continue;   // no gradient is wanted there
-    const auto s = e.function->stream();
-    TORCH_CHECK(!s || s->id() != 0, "a backward pass under capture reaches ", e.function->name(), " on the default stream, "
-                "which cannot take part: release the eager graph that holds it (its loss and outputs), or run that graph's "
-                "forward pass on another stream than the default one");
+  const auto first = torch::autograd::get_current_node();
+  if (status == hipStreamCaptureStatusNone || !first) return;
+  std::vector<torch::autograd::Node*> todo{first.get()};
+  std::unordered_set<torch::autograd::Node*> seen{first.get()};
+  while (!todo.empty()) {
+    torch::autograd::Node* const node = todo.back();
+    todo.pop_back();
+    for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+      const auto& e = node->next_edge(i);
+      if (!e.function || !node->task_should_compute_output(i) || !seen.insert(e.function.get()).second) continue;
+      const auto s = e.function->stream();
+      TORCH_CHECK(!s || s->id() != 0, "a backward pass under capture reaches ", e.function->name(), " on the default stream, "
+                  "which cannot take part: release the eager graph that holds it (its loss and outputs), or run that graph's "
+                  "forward pass on another stream than the default one");
+      todo.push_back(e.function.get());
+    }
   }
 }
 

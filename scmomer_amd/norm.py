@@ -20,5 +20,5 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     statistics and the gradients of weight and bias are f32.  Gradients do not depend on the order in which
     workgroups run.  First derivatives only, in reverse mode: under forward-mode differentiation, a tracer (torch.jit.trace,
     make_fx) or with tensor subclasses that have a dispatch of their own it raises NotImplementedError.  A backward pass under capture into a graph is refused while an eager graph
-    on the default stream holds the same leaves (their gradients would have to join that stream)."""
+    on the default stream holds a leaf that it reaches (its gradient would have to join that stream)."""
     return torch_ops.layer_norm(x, weight, bias, eps, out_dtype)

@@ -101,3 +101,48 @@ def test_an_incoming_gradient_that_is_only_noted_to_be_zero(M, name):
     y = calls[name](z)
     g, = torch.autograd.grad(y, z, torch._efficientzerotensor(tuple(y.shape), device=DEV))
     assert g.shape == x.shape and not g.any()
+
+
+@pytest.mark.parametrize("name", ["norm", "score", "distill"])
+@pytest.mark.parametrize("layers", [1, 3])
+def test_capture_beside_an_eager_graph_of_a_leaf_further_up(M, name, layers):
+    """The leaf is a weight some products before the operator; its accumulator lives on the default stream for as long as the
+    eager graph does.  Refused then, before anything is launched; captured once that graph is gone, and for a weight that no
+    graph holds."""
+    import gc
+    x, calls = _calls(M)
+    w = torch.rand(6, 300, generator=torch.Generator().manual_seed(1)).to(DEV).requires_grad_()
+
+    def loss(weight):
+        h = x
+        for _ in range(layers):
+            h = h * weight
+        y = calls[name](h)
+        return (y * y).sum()
+    alive = loss(w)
+    want, = torch.autograd.grad(alive, w, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other = w.detach().requires_grad_()
+        got, = torch.autograd.grad(loss(other), other)
+        h = x.detach().requires_grad_()                    # a leaf of its own: the held weight takes no part
+        side, = torch.autograd.grad((calls[name](h * w) ** 2).sum(), h)
+        with pytest.raises(RuntimeError, match="default stream"):
+            torch.autograd.grad(loss(w), w)
+        with pytest.raises(RuntimeError, match="default stream"):
+            loss(w).backward()
+    del alive
+    gc.collect()          # the refusals' tracebacks hold graphs too
+    again = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(again):
+        got2, = torch.autograd.grad(loss(w), w)
+    for _ in range(3):
+        graph.replay()
+        again.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(got2, want) and torch.isfinite(side).all()
+        got.zero_()
+        got2.zero_()
+        torch.cuda.synchronize()
+    assert w.grad is None
