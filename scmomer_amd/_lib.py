@@ -177,7 +177,9 @@ def check(code: int, what: str):
 
 
 def _load_torch_ops():
-    """The torch functions over the C ABI (csrc/torch_ops.cpp), calling into `lib`."""
+    """The torch functions over the C ABI (csrc/torch_ops.cpp), calling into `lib`.  Unlike `lib` they are tied to the torch
+    they were built for, and only norm.py and logits.py use them: `torch_ops` is loaded where one of those is first called,
+    so that everything else needs the library alone."""
     import torch  # noqa: F401  (its libraries first)
     try:
         from . import _torch_ops
@@ -188,4 +190,8 @@ def _load_torch_ops():
     return _torch_ops
 
 
-torch_ops = _load_torch_ops()
+def __getattr__(name):
+    if name != "torch_ops":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    ops = globals()["torch_ops"] = _load_torch_ops()
+    return ops

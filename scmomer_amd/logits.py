@@ -15,7 +15,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from ._lib import torch_ops
+from . import _lib
 
 
 class TokenLogprobs(NamedTuple):
@@ -40,7 +40,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
 
     Differentiable once in the logits, through every output but ``top_index`` (the choice of the alternatives is a
     constant, as for torch.topk)."""
-    return TokenLogprobs(*torch_ops.token_logprobs(logits, targets, k, temperature, ignore_index, entropy))
+    return TokenLogprobs(*_lib.torch_ops.token_logprobs(logits, targets, k, temperature, ignore_index, entropy))
 
 
 def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *, temperature: float = 1.0,
@@ -56,7 +56,7 @@ def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob
     loss is f32 and not multiplied by temperature^2.  A row of -inf throughout counts with loss and gradient 0.
 
     Differentiable once, in the logits only.  The result does not depend on the order in which workgroups run."""
-    return torch_ops.topk_distillation(logits, top_index, top_logprob, temperature, tail, weight, reduction)
+    return _lib.torch_ops.topk_distillation(logits, top_index, top_logprob, temperature, tail, weight, reduction)
 
 
 def topk_distillation_grad(logits: torch.Tensor, top_index: torch.Tensor, top_logprob: torch.Tensor, *,
@@ -65,4 +65,4 @@ def topk_distillation_grad(logits: torch.Tensor, top_index: torch.Tensor, top_lo
     """(loss, scale * d loss / d logits) of topk_distillation ('mean' or 'sum') in one pass over the logits, for a loop
     that runs the model's backward itself: ``loss, d = topk_distillation_grad(logits, ..., scale=1 / grad_acc)``,
     ``logits.backward(d)``.  The gradient has the logits' type and shape."""
-    return torch_ops.topk_distillation_grad(logits, top_index, top_logprob, temperature, tail, weight, reduction, scale)
+    return _lib.torch_ops.topk_distillation_grad(logits, top_index, top_logprob, temperature, tail, weight, reduction, scale)

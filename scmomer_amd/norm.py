@@ -8,7 +8,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import torch_ops
+from . import _lib
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -21,4 +21,4 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     workgroups run.  First derivatives only, in reverse mode: under forward-mode differentiation, a tracer (torch.jit.trace,
     make_fx) or with tensor subclasses that have a dispatch of their own it raises NotImplementedError.  A backward pass under capture into a graph is refused while an eager graph
     on the default stream holds a leaf that it reaches (its gradient would have to join that stream)."""
-    return torch_ops.layer_norm(x, weight, bias, eps, out_dtype)
+    return _lib.torch_ops.layer_norm(x, weight, bias, eps, out_dtype)
