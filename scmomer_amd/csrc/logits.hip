@@ -584,13 +584,17 @@ static int segment_length(int V, int S) { return ((V + S - 1) / S + 31) / 32 * 3
 // segments that really hold elements once the length is rounded
 static int segments_used(int V, int len) { return (V + len - 1) / len; }
 
-template <typename T, int NT, int EL = 32>
+// TOP_ONLY: a shape that is chosen for its alternatives
+template <typename T, int NT, int EL = 32, bool TOP_ONLY = false>
 static void launch_score(const ScoreArgs& a, int S, int len, hipStream_t s) {
   const dim3 g((unsigned)(a.T * S)), b(NT);
-  if (a.entropy && a.k) hipLaunchKernelGGL((score_kernel<T, NT, EL, true, true>), g, b, 0, s, a, S, len);
-  else if (a.entropy) hipLaunchKernelGGL((score_kernel<T, NT, EL, true, false>), g, b, 0, s, a, S, len);
-  else if (a.k) hipLaunchKernelGGL((score_kernel<T, NT, EL, false, true>), g, b, 0, s, a, S, len);
-  else hipLaunchKernelGGL((score_kernel<T, NT, EL, false, false>), g, b, 0, s, a, S, len);
+  if (TOP_ONLY || a.k) {
+    if (a.entropy) hipLaunchKernelGGL((score_kernel<T, NT, EL, true, true>), g, b, 0, s, a, S, len);
+    else hipLaunchKernelGGL((score_kernel<T, NT, EL, false, true>), g, b, 0, s, a, S, len);
+  } else if constexpr (!TOP_ONLY) {
+    if (a.entropy) hipLaunchKernelGGL((score_kernel<T, NT, EL, true, false>), g, b, 0, s, a, S, len);
+    else hipLaunchKernelGGL((score_kernel<T, NT, EL, false, false>), g, b, 0, s, a, S, len);
+  }
 }
 template <typename T, int N>
 static void launch_score_small(const ScoreArgs& a, dim3 g, hipStream_t s) {
@@ -629,7 +633,7 @@ static void score_typed(const ScoreArgs& a, hipStream_t s) {
     if (a.V <= 4096) return launch_score<T, 256, 16>(a, 1, a.V, s);
     return launch_score<T, 256>(a, 1, a.V, s);
   }
-  if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8>(a, 1, a.V, s);
+  if (a.V <= 512) return a.k <= 32 ? launch_score<T, 64, 8>(a, 1, a.V, s) : launch_score<T, 128, 8, true>(a, 1, a.V, s);
   if (a.V <= 1024 && a.k <= 32) return launch_score<T, 64, 16>(a, 1, a.V, s);
   if (bytes <= 16384 && a.k <= 32) return launch_score<T, 64>(a, 1, a.V, s);
   // a workgroup per CU at most, and many alternatives: 150 x 60000 bf16, k = 64 18 us, on 256 threads 22 (k = 20: 15 and 16)

@@ -545,13 +545,13 @@ static bool launch_resident(const DistillTopkArgs& a, hipStream_t s) {
   constexpr int MAX = 64 / (32 * (int)sizeof(T) / 4);   // steps in 64 registers: 4 for 2-byte types, 2 for f32
   const dim3 g((unsigned)a.T);
   // Few rows: a row in one step of a large workgroup.  fp16: 100 x 3000 7.2 us, on one wave 10.6; 1000 x 3000 10.5 and 12.8;
-  // 100 x 17339 12.3, in two steps of 256 threads 16.9, but 1000 x 17339 41 and 35.
+  // 100 x 17339 12.3, in two steps of 256 threads 16.9, but 1000 x 17339 41 and 35.  (Never more than STREAM_BYTES of results.)
   if (a.V > 1024 && (a.V <= 8192 ? a.T <= 1024 : a.V <= 32768 && a.T <= 256)) {
-    if (a.V <= 256 * 8) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM, 8>), g, dim3(256), 0, s, a);
-    else if (a.V <= 256 * 16) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM, 16>), g, dim3(256), 0, s, a);
-    else if (a.V <= 256 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, STREAM>), g, dim3(256), 0, s, a);
-    else if (a.V <= 512 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 512, 1, STREAM>), g, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((distill_resident_kernel<T, 1024, 1, STREAM>), g, dim3(1024), 0, s, a);
+    if (a.V <= 256 * 8) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, false, 8>), g, dim3(256), 0, s, a);
+    else if (a.V <= 256 * 16) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, false, 16>), g, dim3(256), 0, s, a);
+    else if (a.V <= 256 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 256, 1, false>), g, dim3(256), 0, s, a);
+    else if (a.V <= 512 * 32) hipLaunchKernelGGL((distill_resident_kernel<T, 512, 1, false>), g, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((distill_resident_kernel<T, 1024, 1, false>), g, dim3(1024), 0, s, a);
     return true;
   }
   if (a.V <= 64 * 8) hipLaunchKernelGGL((distill_resident_kernel<T, 64, 1, STREAM, 8>), g, dim3(64), 0, s, a);
