@@ -4,7 +4,7 @@
 // The logits are read once, in 16-byte chunks; every thread keeps a running maximum m and s = sum 2^((x - m) c),
 // c = log2(e) / temperature, in f32; threads, waves and workgroups join by rescaling to the larger maximum.  x - m is
 // formed first: a row of the type's lowest value is an ordinary (uniform) row, and -inf weighs nothing.
-//   many rows of V <= 64   one thread per row, 64 rows staged through LDS per wave
+//   V <= 16, and many rows of V <= 64   one thread per row, 64 rows staged through LDS per wave
 //   else                   64 to 512 threads per row by its length; where long rows are too few to fill the card a row is split
 //                          into segments of one workgroup each, whose partial results a second launch joins in segment order
 // What bounds them is HBM, and for 2-byte types the vector ALU nearly as much (an exponential costs four issue slots).

@@ -32,14 +32,16 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
                    ignore_index: int = -100, entropy: bool = True) -> TokenLogprobs:
     """Log probabilities under softmax(logits / temperature), over the last dimension of logits [..., V].
 
-    logits: f32, bf16 or fp16 on the GPU, any row stride; targets: int64 [...] or None.  Everything is computed in f32
-    and returned in f32.  ``logprob``: of the target token, 0 where the target is ``ignore_index``, NaN where it is any
-    other number outside [0, V).  ``top_index`` / ``top_logprob``: the k <= min(64, V) most likely tokens in descending
-    order, equal logits by ascending index (NaN counts as largest).  A row that is -inf throughout has lse and log
-    probabilities -inf, entropy 0 and no gradient; a row with NaN or +inf is NaN.
+    logits: f32, bf16 or fp16 on the GPU, any row stride; targets: int64 [...] or None; temperature: finite and at least
+    2^-126 (below, its reciprocal leaves the range of f32).  Everything is computed in f32 and returned in f32.
+    ``logprob``: of the target token, 0 where the target is ``ignore_index``, NaN where it is any other number outside
+    [0, V).  ``top_index`` / ``top_logprob``: the k <= min(64, V) most likely tokens in descending order, equal logits by
+    ascending index (NaN counts as largest).  A row that is -inf throughout has lse and log probabilities -inf, entropy 0
+    and no gradient; a row with NaN or +inf is NaN.
 
     Differentiable once in the logits, through every output but ``top_index`` (the choice of the alternatives is a
-    constant, as for torch.topk)."""
+    constant, as for torch.topk).  Two calls with the same logits give the same bits; the same row in a call of another
+    number of rows may differ in the last ones (how its sum is split over threads depends on that number)."""
     return TokenLogprobs(*_lib.torch_ops.token_logprobs(logits, targets, k, temperature, ignore_index, entropy))
 
 
@@ -54,8 +56,10 @@ def topk_distillation(logits: torch.Tensor, top_index: torch.Tensor, top_logprob
     tokens; otherwise the entries are renormalised.  ``weight`` f32 [...]: rows of weight 0 (padding) are not looked at.
     reduction 'mean' divides by the sum of the weights (nan when that is 0), 'none' returns weight * loss per row.  The
     loss is f32 and not multiplied by temperature^2.  A row of -inf throughout counts with loss and gradient 0.
+    temperature: as for token_logprobs.
 
-    Differentiable once, in the logits only.  The result does not depend on the order in which workgroups run."""
+    Differentiable once, in the logits only.  The result does not depend on the order in which workgroups run; a row's last
+    bits may depend on the number of rows in the call, as for token_logprobs."""
     return _lib.torch_ops.topk_distillation(logits, top_index, top_logprob, temperature, tail, weight, reduction)
 
 
