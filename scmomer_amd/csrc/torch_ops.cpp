@@ -98,9 +98,9 @@ Tensor grad_rows(const Tensor& g, const Tensor& like, int64_t n) {
 }
 
 // The kernels work on addresses: what hands tensors on without values, or follows a call by its torch operations, sees
-// nothing of them.  Refused are tensors of forward-mode differentiation (their tangent would be lost), tensors with a
-// dispatch of their own (a wrapper has no memory), and calls under a tracer (it would record the allocation of the
-// results only).
+// nothing of them.  Refused are tensors of forward-mode differentiation (their tangent would be lost), wrappers, which have
+// no memory (of subclasses with a dispatch of their own, of torch.func's transforms), and calls under a tracer (it would
+// record the allocation of the results only).
 void check_followed(std::initializer_list<std::reference_wrapper<const Tensor>> tensors) {
   using c10::impl::TorchDispatchModeKey;
   using c10::impl::TorchDispatchModeTLS;
@@ -109,11 +109,13 @@ void check_followed(std::initializer_list<std::reference_wrapper<const Tensor>> 
     for (const auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
       traced = traced || TorchDispatchModeTLS::get_mode(key).has_value();
   TORCH_CHECK_NOT_IMPLEMENTED(!traced, "this operator of scmomer_amd cannot be traced");
+  constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                          c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
   for (const Tensor& t : tensors) {
     if (!t.defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.key_set().has_any(wrappers), "this operator of scmomer_amd takes plain tensors, not those of "
+                                "torch.func's transforms or of subclasses with a dispatch of their own");
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "this operator of scmomer_amd has no forward-mode derivative");
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.key_set().has(c10::DispatchKey::Python),
-                                "this operator of scmomer_amd takes plain tensors, not subclasses with a dispatch of their own");
   }
 }
 
@@ -199,6 +201,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_followed({grads[0]});
     const auto saved = ctx->get_saved_variables();
+    check_capture(saved[0]);
     const Tensor &x_ = saved[0], &st = saved[2];
     const Tensor x = rows_of(x_, "x"), w = values(saved[1]), dy = rows_of(grads[0], "dy");
     on_device_of(x, dy, "dy");
@@ -207,7 +210,6 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const bool want_x = ctx->needs_input_grad(0), want_w = w.defined() && ctx->needs_input_grad(1);
     const bool want_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.defined() ? 2 : 1);
     const c10::DeviceGuard guard(x.device());
-    check_capture(x);
     Tensor dx = want_x ? at::empty(x_.sizes(), x.options()) : Tensor();
     auto sum = [&](bool want) {   // no rows: the sums are empty
       return !want ? Tensor() : t ? floats(x, {d}) : at::zeros({d}, x.options().dtype(at::kFloat));
@@ -294,6 +296,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     for (const Tensor& g : grads) check_followed({g});
     const auto saved = ctx->get_saved_variables();
+    check_capture(saved[0]);
     const Tensor &logits = saved[0], &entropy = saved[2], &top_index = saved[3], &tape = saved[4];
     const double temperature = ctx->saved_data["temperature"].toDouble();
     const int64_t k = top_index.defined() ? top_index.size(-1) : 0;
@@ -307,7 +310,6 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     const Tensor g_lse = grad_rows(grads[i++], x, t);
     const Tensor g_top = grad_rows(k ? grads[i++] : none, x, t * k);
     const c10::DeviceGuard guard(x.device());
-    check_capture(x);
     Tensor dx = at::empty(logits.sizes(), x.options());
     if (t)
       call(api.score_bwd(x.data_ptr(), type_of(x, "logits"), x.stride(0), t, (int)v, (float)temperature,
@@ -412,11 +414,11 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_followed({grads[0]});
     const auto saved = ctx->get_saved_variables();
+    check_capture(saved[0]);
     const int64_t opts = ctx->saved_data["opts"].toInt();
     const Distill op(saved[0], saved[1], saved[2], saved[3], ctx->saved_data["temperature"].toDouble(), opts & 1,
                      (Reduction)(opts >> 1), true);
     const c10::DeviceGuard guard(op.x.device());
-    check_capture(op.x);
     Tensor dx = at::empty(saved[0].sizes(), op.x.options());
     if (op.t) {
       const bool per_row = op.red == NONE;

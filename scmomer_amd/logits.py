@@ -3,8 +3,9 @@ probabilities of given tokens with entropy and top alternatives (token_logprobs)
 log probabilities (topk_distillation, topk_distillation_grad).  The RNA model's own masked cross
 entropy over its at most eight expression classes is s1.masked_cross_entropy.
 
-Differentiable means once and in reverse mode: under forward-mode differentiation, a tracer (torch.jit.trace, make_fx) or
-with tensor subclasses that have a dispatch of their own they raise NotImplementedError, and so does their backward pass.
+Differentiable means once and in reverse mode: under forward-mode differentiation, a tracer (torch.jit.trace, make_fx),
+torch.func's transforms or with tensor subclasses that have a dispatch of their own they raise NotImplementedError, and so
+does their backward pass.
 
 A backward pass of these under capture into a graph is refused while an eager graph on the default stream holds a leaf that
 it reaches (that leaf's gradient would have to join that stream).

@@ -20,8 +20,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     statistics and the gradients of weight and bias are f32.  Results do not depend on the order in which workgroups
     run; a row's last place may depend on the number of rows in the call.
 
-    First derivatives only, in reverse mode: under forward-mode differentiation, a tracer (torch.jit.trace, make_fx) or
-    with tensor subclasses that have a dispatch of their own it raises NotImplementedError.  A backward pass under capture
-    into a graph is refused while an eager graph on the default stream holds a leaf that it reaches (its gradient would
+    First derivatives only, in reverse mode: under forward-mode differentiation, a tracer (torch.jit.trace, make_fx),
+    torch.func's transforms or with tensor subclasses that have a dispatch of their own it raises NotImplementedError.  A
+    backward pass under capture into a graph is refused while an eager graph on the default stream holds a leaf that it reaches (its gradient would
     have to join that stream)."""
     return _lib.torch_ops.layer_norm(x, weight, bias, eps, out_dtype)

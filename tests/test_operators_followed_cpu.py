@@ -73,3 +73,17 @@ def test_a_mode_that_only_counts_is_no_tracer(name):
     from torch.utils.flop_counter import FlopCounterMode
     with FlopCounterMode(display=False), pytest.raises(ValueError, match="device"):
         _calls()[name](torch.randn(2, 8))
+
+
+@pytest.mark.parametrize("name", ["norm", "score", "distill", "step"])
+def test_function_transforms_raise(name):
+    f = _calls()[name]
+    with pytest.raises(NotImplementedError, match="plain tensors"):
+        torch.func.vmap(f)(torch.randn(3, 2, 8))
+    for transform in (torch.func.grad(lambda x: torch.as_tensor(f(x)).sum()), torch.func.jacrev(f)):
+        with pytest.raises(NotImplementedError, match="plain tensors"):
+            transform(torch.randn(2, 8))
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(f, (torch.randn(2, 8),), (torch.randn(2, 8),))
+    with pytest.raises(NotImplementedError, match="plain tensors"):
+        torch.func.functionalize(f)(torch.randn(2, 8))
